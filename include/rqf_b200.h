@@ -695,6 +695,86 @@ int rqf_two_tap_coefficients_backward(const float *log_theta, const float *log_g
                                       float *grad_log_gamma, int64_t n, double dt, double tau,
                                       rqf_stream_t stream);
 
+/* ---- gated delta rule over sequences ----------------------------------- *
+ * No counterpart in the reference, whose recurrences are diagonal.  Value head
+ * h carries a K x V matrix S and reads key head h / (value_heads / key_heads):
+ *
+ *   S_t = a_t S_{t-1} + k_t u_t^T,   a_t = exp(log_decay_t),
+ *   u_t = beta_t (v_t - (a_t S_{t-1})^T k_t),      o_t = scale S_t^T q_t.
+ *
+ * q, k (batch, time, key_heads, K) and v (batch, time, value_heads, V) have
+ * `dtype`; log_decay and beta (batch, time, value_heads) are float32.  Each
+ * has its strides (batch, time, head, in elements); the last axis is dense.
+ * o and all gradients are dense in the same orders, states (batch,
+ * value_heads, K, V) float32.  `lengths` (nullable, device, batch): row b has
+ * that many tokens (taken into 0..time), what stands past them is not read,
+ * o and gradients there are 0 and the state passes.  A log_decay below -200
+ * counts as -200 (its exponential is 0 in 32 bits).
+ * K and V are multiples of 8, K at most 128; q, k, v, o, grad_* start on 16
+ * bytes and their strides are multiples of 16 bytes.  Products take their
+ * operands in halves (two for a 32-bit one) with 32-bit sums: 32-bit accuracy.
+ * Non-finite inputs reach all of their 64-token chunk and what follows.
+ *
+ * context: rqf_gated_delta_context_bytes(problem, save), 256-byte aligned.
+ * With save != 0 the forward keeps in it what the backward needs (the states
+ * that enter each chunk among it); the backward is then given the same
+ * problem, v and context.  Each size is SIZE_MAX for a refused shape. */
+enum { RQF_F32 = 0, RQF_BF16 = 1, RQF_F16 = 2, RQF_C64 = 3 };
+
+typedef struct {
+  int64_t batch, time, key_heads, value_heads, key_dim, value_dim;
+  int64_t q_stride[3], k_stride[3], v_stride[3], g_stride[3], beta_stride[3];
+  const int64_t *lengths;
+  int dtype; /* RQF_F32, RQF_BF16 or RQF_F16 */
+  float scale;
+} rqf_delta_problem;
+
+size_t rqf_gated_delta_context_bytes(const rqf_delta_problem *problem, int save);
+size_t rqf_gated_delta_backward_workspace_bytes(const rqf_delta_problem *problem);
+/* initial_state nullable (zeros); final_state nullable (not written). */
+int rqf_gated_delta_forward(const rqf_delta_problem *problem, const void *q, const void *k,
+                            const void *v, const float *log_decay, const float *beta,
+                            const float *initial_state, void *o, float *final_state, void *context,
+                            int save, rqf_stream_t stream);
+/* grad_final_state nullable (zeros); grad_initial_state nullable (not
+ * written); the other gradients are written in full. */
+int rqf_gated_delta_backward(const rqf_delta_problem *problem, const void *v, const void *context,
+                             const void *grad_o, const float *grad_final_state, void *grad_q,
+                             void *grad_k, void *grad_v, float *grad_log_decay, float *grad_beta,
+                             float *grad_initial_state, void *workspace, rqf_stream_t stream);
+
+/* One token for each row of a batch on float32 states that stay in a pool,
+ * (pool, value_heads, K, V) dense and 16-byte aligned, updated in place.  Row
+ * b works on slots[b] (nullable: slot b); int32, or int64 with slots_64 != 0.
+ * A negative slot is an idle row: o is 0 there and nothing is touched; one
+ * past the pool is that too and latches RQF_ERR_ARGUMENT.  The slots of a call
+ * are distinct.  problem: time, the time strides and lengths are not read, and
+ * q, k, v need no alignment beyond their type's.  o (batch, value_heads, V). */
+int rqf_gated_delta_step(const rqf_delta_problem *problem, const void *q, const void *k,
+                         const void *v, const float *log_decay, const float *beta,
+                         const void *slots, int slots_64, int64_t pool, float *state, void *o,
+                         rqf_stream_t stream);
+
+/* ---- gradient norm and clipping --------------------------------------- *
+ * Replaces clip_model_grad_norm_ (train.py:777-789), the last step before the
+ * optimiser: over n tensors given by host arrays of device pointers, element
+ * counts and types (RQF_F32, RQF_BF16, RQF_F16, RQF_C64),
+ *
+ *   *norm = sqrt(sum |g|^2)      (device float32; squares summed in 64 bits,
+ *                                 in an order that only sizes decide)
+ *   outs[i] = grads[i] * min(1, max_norm / (*norm + 1e-6)),
+ *
+ * each product rounded once.  outs[i] may be grads[i]; else no two tensors
+ * overlap.  Tensors need no alignment beyond their element's.  A norm that is
+ * NaN makes every output NaN, an infinite one 0 (NaN where g is infinite).
+ * `scratch` needs rqf_grad_norm_scratch_bytes(n) bytes, 8-byte aligned. */
+size_t rqf_grad_norm_scratch_bytes(int64_t n);
+int rqf_global_grad_norm(const void *const *grads, const int64_t *numel, const int *dtype,
+                         int64_t n, float *norm, void *scratch, rqf_stream_t stream);
+int rqf_clip_grads(const void *const *grads, void *const *outs, const int64_t *numel,
+                   const int *dtype, int64_t n, float max_norm, float *norm, void *scratch,
+                   rqf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -11,6 +11,8 @@ librqf_b200.so behind the C ABI of include/rqf_b200.h.
 
 from . import _abi
 from ._abi import RQFError, check_device_errors, read_device_error
+from .delta import gated_delta_scan, gated_delta_step
+from .grads import clip_grads_, global_grad_norm
 from .integration import install, uninstall
 from .ops import (
     _triton_chunked_scan,
@@ -34,6 +36,10 @@ __all__ = [
     "read_device_error",
     "install",
     "uninstall",
+    "clip_grads_",
+    "gated_delta_scan",
+    "gated_delta_step",
+    "global_grad_norm",
     "_triton_chunked_scan",
     "_triton_chunked_scan_prospective",
     "fbt_prospective_scan",

@@ -55,6 +55,16 @@ class CoeffOptions(ctypes.Structure):
                 ("param_space", _int), ("clamp_gamma", _int), ("dt", _f64), ("tau", _f64)]
 
 
+class DeltaProblem(ctypes.Structure):
+    """rqf_delta_problem (include/rqf_b200.h)."""
+
+    _fields_ = [("batch", _i64), ("time", _i64), ("key_heads", _i64), ("value_heads", _i64),
+                ("key_dim", _i64), ("value_dim", _i64), ("q_stride", _i64 * 3),
+                ("k_stride", _i64 * 3), ("v_stride", _i64 * 3), ("g_stride", _i64 * 3),
+                ("beta_stride", _i64 * 3), ("lengths", _p), ("dtype", _int), ("scale", _f32)]
+
+
+_pdp = ctypes.POINTER(DeltaProblem)
 _pin = ctypes.POINTER(SelectiveInputs)
 _pop = ctypes.POINTER(SelectiveOptions)
 _pcl = ctypes.POINTER(CoeffLeaves)
@@ -156,6 +166,17 @@ SIGNATURES: dict[str, tuple] = {
     "rqf_per_step_cross_entropy": (_int, [_p, _p, _p, _p, _i64, _i64, _i64, _f32, _p]),
     "rqf_per_step_cross_entropy_backward": (
         _int, [_p, _p, _p, _p, _i64, _i64, _i64, _f32, _p]),
+    "rqf_gated_delta_context_bytes": (_sz, [_pdp, _int]),
+    "rqf_gated_delta_backward_workspace_bytes": (_sz, [_pdp]),
+    "rqf_gated_delta_forward": (
+        _int, [_pdp, _p, _p, _p, _p, _p, _p, _p, _p, _p, _int, _p]),
+    "rqf_gated_delta_backward": (
+        _int, [_pdp, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p]),
+    "rqf_gated_delta_step": (
+        _int, [_pdp, _p, _p, _p, _p, _p, _p, _int, _i64, _p, _p, _p]),
+    "rqf_grad_norm_scratch_bytes": (_sz, [_i64]),
+    "rqf_global_grad_norm": (_int, [_p, _p, _p, _i64, _p, _p, _p]),
+    "rqf_clip_grads": (_int, [_p, _p, _p, _p, _i64, _f32, _p, _p, _p]),
 }
 
 _LIB = None

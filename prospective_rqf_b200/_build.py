@@ -5,6 +5,7 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+import tempfile
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -15,7 +16,7 @@ ROOT = PKG.parent
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
 ]
 
 
@@ -38,20 +39,31 @@ def needs_build() -> bool:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile csrc/rqf_b200.cu (which includes the kernel headers) into
+    """Compile every csrc/*.cu (rqf_b200.cu and delta_rule.cu, which include the
+    kernel headers) side by side and link them into
     prospective_rqf_b200/librqf_b200.so."""
     if not force and not needs_build():
         return LIB
+    nvcc = _nvcc()
     tmp = LIB.with_suffix(".so.tmp")
-    cmd = [_nvcc(), *NVCC_FLAGS, "-o", str(tmp), str(CSRC / "rqf_b200.cu")]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-    res = subprocess.run(cmd, capture_output=True, text=True)
+    units = sorted(CSRC.glob("*.cu"))
+    with tempfile.TemporaryDirectory() as work:
+        objects = [str(Path(work) / f"{u.stem}.o") for u in units]
+        running = [subprocess.Popen(
+            [nvcc, *(["-Xptxas=-v"] if verbose else []), *NVCC_FLAGS, "-c", "-o", o, str(u)],
+            stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)
+            for u, o in zip(units, objects)]
+        logs = [p.communicate()[1] for p in running]
+        for u, p, log in zip(units, running, logs):
+            if p.returncode != 0:
+                raise RuntimeError(f"nvcc failed ({p.returncode}) on {u.name}:\n{log}")
+        res = subprocess.run([nvcc, *NVCC_FLAGS, "-shared", "-o", str(tmp), *objects],
+                             capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stderr}")
+        raise RuntimeError(f"nvcc failed to link ({res.returncode}):\n{res.stderr}")
     os.replace(tmp, LIB)
     if verbose:
-        print(res.stderr)
+        print("".join(logs))
     return LIB
 
 

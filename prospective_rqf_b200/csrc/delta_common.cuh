@@ -1,0 +1,294 @@
+// Building blocks of the gated delta rule's chunked kernels: split half
+// operands, tensor-core fragments and the chunk tiles in shared memory.
+//
+// The rule, for each value head with a K x V state S:
+//
+//   S_t = a_t S_{t-1} + k_t u_t^T,  u_t = beta_t (v_t - a_t S_{t-1}^T k_t),  a_t = e^{g_t}
+//   o_t = scale S_t^T q_t
+//
+// Over a chunk of C = 64 tokens, with G the running sum of g inside it, S the
+// state that enters, A_ij = beta_i e^{G_i-G_j} k_i.k_j (i > j), T = (I + A)^{-1}
+// and P_ij = scale e^{G_i-G_j} q_i.k_j (i >= j):
+//
+//   r = beta (v - e^G k S),   u = T r,   o = scale e^G q S + P u,
+//   S' = e^{G_C} S + (e^{G_C-G} k)^T u.
+//
+// Operands.  The products run on the tensor cores (m16n8k16, half inputs,
+// 32-bit sums), yet states, cotangents of the 32-bit inputs and the chain from
+// chunk to chunk have to keep 32-bit accuracy.  So a 32-bit operand enters as
+// two halves, x s = hi + lo + O(2^-22), with s a power of two that puts the
+// largest of a row (or tile) at 2^8: what is left out is at most 2^-33 of that
+// largest.  16-bit inputs are one half exactly after the same scaling (bf16 has
+// 8 significant bits, half 11), so k S costs two products, T r three, and a
+// 32-bit input two more.  Splitting into bf16 parts instead keeps 16 bits of
+// the 22 and measured 4e-6 to 8e-6 from 64 bits in a CPU model of these
+// formulas, against 2e-7 for this split.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace rqf {
+namespace delta {
+
+constexpr int kC = 64;       // tokens of a chunk
+constexpr int kVec = 8;      // coefficient rows kept for a chunk (enum Row)
+constexpr float kMinDecay = -200.f;  // e^-200 is 0 in 32 bits: -inf gates are taken as this
+
+// Coefficient rows of a chunk, 64 floats each.
+enum Row {
+  kRowKS = 0,    // beta e^G kfac: the factor of k S in r
+  kRowBeta = 1,  // beta
+  kRowT = 2,     // 2^t, the scale of T's row
+  kRowP = 3,     // 2^p, the scale of P's row
+  kRowO = 4,     // scale e^G qfac: the factor of q S in o
+  kRowU = 5,     // e^{G_C-G} kfac: the factor of u in the state
+  kRowEG = 6,    // e^G
+  kRowEC = 7     // e^{G_C-G}
+};
+
+template <typename E>
+struct Elem;
+template <>
+struct Elem<float> {
+  static constexpr int kParts = 2;  // halves that hold an input
+  static __device__ __forceinline__ float get(float x) { return x; }
+  static __device__ __forceinline__ float put(float x) { return x; }
+};
+template <>
+struct Elem<__nv_bfloat16> {
+  static constexpr int kParts = 1;
+  static __device__ __forceinline__ float get(__nv_bfloat16 x) { return __bfloat162float(x); }
+  static __device__ __forceinline__ __nv_bfloat16 put(float x) { return __float2bfloat16_rn(x); }
+};
+template <>
+struct Elem<__half> {
+  static constexpr int kParts = 1;
+  static __device__ __forceinline__ float get(__half x) { return __half2float(x); }
+  static __device__ __forceinline__ __half put(float x) { return __float2half_rn(x); }
+};
+
+// Eight consecutive elements (16-byte aligned) as floats.
+template <typename E>
+__device__ __forceinline__ void load8(const E *p, float (&x)[8]) {
+  if constexpr (sizeof(E) == 4) {
+    const float4 a = *reinterpret_cast<const float4 *>(p);
+    const float4 b = *reinterpret_cast<const float4 *>(p + 4);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+    x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  } else {
+    const uint4 a = *reinterpret_cast<const uint4 *>(p);
+    const E *e = reinterpret_cast<const E *>(&a);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = Elem<E>::get(e[i]);
+  }
+}
+
+// Two values next to each other, as a pair in E.
+template <typename E>
+__device__ __forceinline__ void store2(E *p, float x, float y) {
+  if constexpr (sizeof(E) == 4) {
+    *reinterpret_cast<float2 *>(p) = make_float2(x, y);
+  } else {
+    E v[2] = {Elem<E>::put(x), Elem<E>::put(y)};
+    *reinterpret_cast<uint32_t *>(p) = *reinterpret_cast<uint32_t *>(v);
+  }
+}
+
+// ------------------------------------------------------------ power-of-two scales
+// s = 2^(8-e) and 1/s for the largest magnitude m in [2^e, 2^(e+1)).  m = 0
+// takes s = 1; the exponent is held where both s and 1/s are normal.
+struct Scale {
+  float mul, inv;
+};
+__device__ __forceinline__ Scale scale_for(float m) {
+  int e = (int)((__float_as_uint(m) >> 23) & 255u) - 127;
+  e = m == 0.f ? 8 : (e < -110 ? -110 : (e > 126 ? 126 : e));
+  return {__uint_as_float((uint32_t)(127 + 8 - e) << 23),
+          __uint_as_float((uint32_t)(127 + e - 8) << 23)};
+}
+
+// The scale of an operand whose product is added to sums of magnitude `sums`,
+// which are scaled by it too: at most what keeps those sums below 2^25.  An
+// operand so far below its sums loses nothing that they could hold.
+__device__ __forceinline__ Scale scale_beside(float m, float sums) {
+  return scale_for(fmaxf(m, sums * 0x1p-16f));
+}
+
+// Two scaled values as halves, and what the halves leave out as halves again.
+__device__ __forceinline__ uint32_t pack_hi(float x, float y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  hi = *reinterpret_cast<const uint32_t *>(&h);
+  lo = pack_hi(x - f.x, y - f.y);
+}
+__device__ __forceinline__ float2 half2_float2(uint32_t h) {
+  return __half22float2(*reinterpret_cast<const __half2 *>(&h));
+}
+
+__device__ __forceinline__ float quad_max(float m) {
+  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  return fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+}
+__device__ __forceinline__ float quad_sum(float m) {
+  m += __shfl_xor_sync(0xffffffffu, m, 1);
+  return m + __shfl_xor_sync(0xffffffffu, m, 2);
+}
+
+// Largest magnitude of each of the two rows (g and g + 8) that a thread's
+// accumulator tiles x[][4] hold, over the quad that shares the rows.
+template <int NT>
+__device__ __forceinline__ void row_max(const float (&x)[NT][4], float &m0, float &m1) {
+  m0 = m1 = 0.f;
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    m0 = fmaxf(m0, fmaxf(fabsf(x[i][0]), fabsf(x[i][1])));
+    m1 = fmaxf(m1, fmaxf(fabsf(x[i][2]), fabsf(x[i][3])));
+  }
+  m0 = quad_max(m0);
+  m1 = quad_max(m1);
+}
+
+// The A fragment (16 rows x 16 of the contraction) made of accumulator tiles
+// 2 ks and 2 ks + 1, scaled by s0 (rows g) and s1 (rows g + 8) and split.
+template <int NT>
+__device__ __forceinline__ void split_frag(const float (&x)[NT][4], int ks, float s0, float s1,
+                                           uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+  split2(x[2 * ks][0] * s0, x[2 * ks][1] * s0, hi[0], lo[0]);
+  split2(x[2 * ks][2] * s1, x[2 * ks][3] * s1, hi[1], lo[1]);
+  split2(x[2 * ks + 1][0] * s0, x[2 * ks + 1][1] * s0, hi[2], lo[2]);
+  split2(x[2 * ks + 1][2] * s1, x[2 * ks + 1][3] * s1, hi[3], lo[3]);
+}
+
+// ------------------------------------------------------------ tensor-core steps
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                    uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t smem_u32(const void *p) {
+  return (uint32_t)__cvta_generic_to_shared(p);
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+
+// A tile of halves in shared memory, LD to a row, its 16-byte pieces permuted
+// within each row by the row's low bits so that eight rows' same piece lie in
+// different banks.
+template <int LD>
+__device__ __forceinline__ int tile_at(int row, int piece) {
+  constexpr int kPieces = LD / 8;
+  constexpr int kMask = kPieces < 8 ? kPieces - 1 : 7;
+  // rows of 64 bytes share a bank line in pairs: permute by the pair there
+  const int by = kPieces >= 8 ? row : (row >> (kPieces == 4 ? 1 : 2));
+  return row * LD + ((piece ^ (by & kMask)) << 3);
+}
+
+// Fragment addresses, one 8x8 block for each group of eight lanes.
+// b_rows: B from a tile stored [n][k]; x4 gives (b0, b1) of columns n0.. and n0+8...
+template <int LD>
+__device__ __forceinline__ uint32_t b_rows(uint32_t base, int n0, int k0, int lane) {
+  const int m = lane >> 3, r = lane & 7;
+  return base + 2 * tile_at<LD>(n0 + (m >> 1) * 8 + r, (k0 >> 3) + (m & 1));
+}
+// b_cols: B from a tile stored [k][n], to be loaded transposed.
+template <int LD>
+__device__ __forceinline__ uint32_t b_cols(uint32_t base, int k0, int n0, int lane) {
+  const int m = lane >> 3, r = lane & 7;
+  return base + 2 * tile_at<LD>(k0 + (m & 1) * 8 + r, (n0 >> 3) + (m >> 1));
+}
+// a_rows: A from a tile stored [m][k].
+template <int LD>
+__device__ __forceinline__ uint32_t a_rows(uint32_t base, int m0, int k0, int lane) {
+  const int m = lane >> 3, r = lane & 7;
+  return base + 2 * tile_at<LD>(m0 + (m & 1) * 8 + r, (k0 >> 3) + (m >> 1));
+}
+// a_cols: A from a tile stored [k][m], to be loaded transposed.
+template <int LD>
+__device__ __forceinline__ uint32_t a_cols(uint32_t base, int k0, int m0, int lane) {
+  const int m = lane >> 3, r = lane & 7;
+  return base + 2 * tile_at<LD>(k0 + (m >> 1) * 8 + r, (m0 >> 3) + (m & 1));
+}
+
+// ------------------------------------------------------------ asynchronous copies
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// `bytes` of 16 from src, zeros for the rest.
+__device__ __forceinline__ void copy16z(uint32_t dst, const void *src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void copy_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// A whole tile of `rows` rows of LD halves, stored without gaps, by all threads.
+template <int LD>
+__device__ __forceinline__ void copy_tile(uint32_t dst, const __half *src, int rows, int tid,
+                                          int threads) {
+  constexpr int kPieces = LD / 8;
+  for (int i = tid; i < rows * kPieces; i += threads) {
+    const int row = i / kPieces, p = i % kPieces;
+    copy16(dst + 2 * tile_at<LD>(row, p), src + (size_t)i * 8);
+  }
+}
+
+// ------------------------------------------------------------ arguments
+struct Strides {
+  long long b, t, h;  // in elements; the last axis is dense
+};
+
+// One call's tensors and sizes.  n_chunks covers `time`; a row's own length
+// ends it earlier.  State-like buffers are [row][chunk][v][KD] and
+// [row][chunk][v][64], v padded to VP, a multiple of 16.
+struct Args {
+  const void *q, *k, *v, *dout;
+  const float *g, *beta;
+  Strides sq, sk, sv, sg, sb;
+  const long long *lengths;
+  const float *s0, *dsT;  // (B, Hv, K, V)
+  void *o, *dv, *dq, *dk;
+  float *sT, *ds0, *dg, *dbeta;
+  float scale;
+  int batch, hk, hv, rep, kdim, vdim, vp;
+  long long time;
+  int n_chunks;   // chunks of this call's span
+  int n_first;    // the first of them
+  // workspace and saved context
+  __half *khat, *qhat, *tmat, *pmat;
+  float *kfac, *qfac, *vec;
+  double *gsum;
+  float *states, *us, *dstates, *drs, *maxes;
+  float *dq_part, *dk_part;  // (B, T, Hv, K) when key heads are shared
+};
+
+__device__ __forceinline__ long long row_length(const Args &a, int b) {
+  if (a.lengths == nullptr) return a.time;
+  const long long n = a.lengths[b];
+  return n < 0 ? 0 : (n > a.time ? a.time : n);
+}
+
+}  // namespace delta
+}  // namespace rqf

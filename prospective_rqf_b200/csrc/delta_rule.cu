@@ -1,0 +1,268 @@
+// C-ABI entry points of the gated delta rule over sequences (declarations and
+// contracts: include/rqf_b200.h).  A translation unit of its own: nothing here
+// shares device state with the scans.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "../../include/rqf_b200.h"
+#include "delta_backward.cuh"
+#include "delta_prep.cuh"
+#include "delta_scan.cuh"
+
+using namespace rqf::delta;
+
+namespace {
+
+constexpr int64_t kMaxGrid = 0x7fffffffLL;
+constexpr size_t kMaxSmem = 227 * 1024;
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+struct Sizes {
+  int64_t chunks, bhn, bkn, vp;
+  int kd, parts;
+};
+
+// RQF_OK and the derived sizes, or why the shape is refused.
+int sizes_of(const rqf_delta_problem *p, Sizes *s) {
+  if (p == nullptr) return RQF_ERR_ARGUMENT;
+  if (p->batch < 0 || p->time < 0 || p->key_heads <= 0 || p->value_heads <= 0 || p->key_dim <= 0 ||
+      p->value_dim <= 0)
+    return RQF_ERR_SHAPE;
+  if (p->value_heads % p->key_heads != 0 || p->key_dim % 8 != 0 || p->value_dim % 8 != 0 ||
+      p->key_dim > 128)
+    return RQF_ERR_SHAPE;
+  if (p->dtype != RQF_F32 && p->dtype != RQF_BF16 && p->dtype != RQF_F16) return RQF_ERR_ARGUMENT;
+  s->chunks = ceil_div(p->time, kC);
+  s->vp = ceil_div(p->value_dim, 16) * 16;
+  s->kd = p->key_dim <= 32 ? 32 : p->key_dim <= 64 ? 64 : 128;
+  s->parts = p->dtype == RQF_F32 ? 2 : 1;
+  // every grid is a product of these
+  if (p->batch > kMaxGrid || p->value_heads > kMaxGrid || p->value_dim > kMaxGrid || s->chunks > kMaxGrid)
+    return RQF_ERR_SHAPE;
+  const double grid = (double)p->batch * (double)p->value_heads;
+  if (grid * (double)(s->chunks > 0 ? s->chunks : 1) > (double)kMaxGrid ||
+      grid * (double)(s->vp / 16) > (double)kMaxGrid)
+    return RQF_ERR_SHAPE;
+  s->bhn = p->batch * p->value_heads * s->chunks;
+  s->bkn = p->batch * p->key_heads * s->chunks;
+  return RQF_OK;
+}
+
+// Parts of a buffer, each on 256 bytes.
+struct Carver {
+  unsigned char *base;
+  size_t used = 0;
+  template <typename T>
+  void take(T *&to, size_t count) {
+    to = reinterpret_cast<T *>(base + used);
+    used += (count * sizeof(T) + 255) & ~size_t(255);
+  }
+};
+
+// What the forward leaves: the chunks' state-free part, and with `save` what
+// the backward needs besides.
+size_t carve_context(void *buffer, const Sizes &s, bool save, Args *a) {
+  Carver c{static_cast<unsigned char *>(buffer)};
+  c.take(a->khat, (size_t)s.bkn * s.parts * kC * s.kd);
+  c.take(a->qhat, (size_t)s.bkn * s.parts * kC * s.kd);
+  c.take(a->kfac, (size_t)s.bkn * kC);
+  c.take(a->qfac, (size_t)s.bkn * kC);
+  c.take(a->tmat, (size_t)s.bhn * 2 * kC * kC);
+  c.take(a->pmat, (size_t)s.bhn * 2 * kC * kC);
+  c.take(a->vec, (size_t)s.bhn * kVec * kC);
+  a->gsum = nullptr;
+  if (save) {
+    c.take(a->gsum, (size_t)s.bhn * kC);
+    c.take(a->states, (size_t)s.bhn * s.vp * s.kd);
+    c.take(a->us, (size_t)s.bhn * s.vp * kC);
+    c.take(a->maxes, (size_t)s.bhn * kMaxes * (s.vp / 16));
+  }
+  return c.used;
+}
+size_t carve_workspace(void *buffer, const rqf_delta_problem *p, const Sizes &s, Args *a) {
+  Carver c{static_cast<unsigned char *>(buffer)};
+  c.take(a->dstates, (size_t)s.bhn * s.vp * s.kd);
+  c.take(a->drs, (size_t)s.bhn * s.vp * kC);
+  a->dq_part = a->dk_part = nullptr;
+  if (p->value_heads != p->key_heads) {
+    const size_t n = (size_t)p->batch * p->time * p->value_heads * p->key_dim;
+    c.take(a->dq_part, n);
+    c.take(a->dk_part, n);
+  }
+  return c.used;
+}
+
+Strides strides(const int64_t (&s)[3]) { return {s[0], s[1], s[2]}; }
+
+void common_args(const rqf_delta_problem *p, const Sizes &s, Args *a) {
+  *a = Args{};
+  a->sq = strides(p->q_stride), a->sk = strides(p->k_stride), a->sv = strides(p->v_stride);
+  a->sg = strides(p->g_stride), a->sb = strides(p->beta_stride);
+  a->lengths = reinterpret_cast<const long long *>(p->lengths);
+  a->scale = p->scale;
+  a->batch = (int)p->batch, a->hk = (int)p->key_heads, a->hv = (int)p->value_heads;
+  a->rep = a->hv / a->hk, a->kdim = (int)p->key_dim, a->vdim = (int)p->value_dim, a->vp = (int)s.vp;
+  a->time = p->time, a->n_chunks = (int)s.chunks;
+}
+
+int check_inputs(const rqf_delta_problem *p, const void *q, const void *k, const void *v, const float *g,
+                 const float *beta) {
+  if (p->batch * p->time == 0) return RQF_OK;
+  if (!q || !k || !v || !g || !beta) return RQF_ERR_ARGUMENT;
+  const int64_t per = p->dtype == RQF_F32 ? 4 : 8;  // elements of 16 bytes
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v)) return RQF_ERR_ALIGN;
+  for (int i = 0; i < 3; ++i)
+    if (p->q_stride[i] % per || p->k_stride[i] % per || p->v_stride[i] % per) return RQF_ERR_ALIGN;
+  return RQF_OK;
+}
+
+template <typename F>
+int launch(F kernel, int64_t grid, int threads, size_t smem, const Args &a, cudaStream_t st) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return RQF_ERR_LAUNCH;
+  kernel<<<(unsigned)grid, threads, smem, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? RQF_OK : RQF_ERR_LAUNCH;
+}
+
+// CTAs of the pass from chunk to chunk: four warps (64 columns of V) while
+// those are at most one to an SM, eight where there are more.  With eight the
+// chunk's tiles are loaded once for 128 columns and a scheduler has two warps.
+template <typename E, int KD>
+int scan_warps(const Args &a) {
+  constexpr bool fits = scan_smem<E, KD, 8>() <= kMaxSmem;
+  return fits && a.vp > 64 && (int64_t)a.batch * a.hv * ceil_div(a.vp, 64) > 148 ? 8 : 4;
+}
+
+template <typename E, int KD, int W>
+int run_scan(const Args &a, bool save, cudaStream_t st) {
+  const int64_t grid = (int64_t)a.batch * a.hv * ceil_div(a.vp / 16, W);
+  constexpr size_t smem = scan_smem<E, KD, W>();
+  return save ? launch(scan_kernel<E, KD, W, true>, grid, W * 32, smem, a, st)
+              : launch(scan_kernel<E, KD, W, false>, grid, W * 32, smem, a, st);
+}
+template <typename E, int KD>
+int run_forward(const Args &a, bool save, cudaStream_t st) {
+  constexpr int NP = Elem<E>::kParts;
+  if (a.n_chunks > 0) {
+    const int rc = launch(prep_kernel<E, KD>, (int64_t)a.batch * a.hv * a.n_chunks, kPrepThreads,
+                          prep_smem<KD, NP>(), a, st);
+    if (rc != RQF_OK) return rc;
+  }
+  if constexpr (scan_smem<E, KD, 8>() <= kMaxSmem)
+    if (scan_warps<E, KD>(a) == 8) return run_scan<E, KD, 8>(a, save, st);
+  return run_scan<E, KD, 4>(a, save, st);
+}
+template <typename E, int KD, int W>
+int run_scan_backward(const Args &a, cudaStream_t st) {
+  return launch(scan_backward_kernel<E, KD, W>, (int64_t)a.batch * a.hv * ceil_div(a.vp / 16, W), W * 32,
+                scan_smem<E, KD, W>(), a, st);
+}
+template <typename E, int KD>
+int run_backward(const Args &a, cudaStream_t st) {
+  int rc;
+  if constexpr (scan_smem<E, KD, 8>() <= kMaxSmem) {
+    if (scan_warps<E, KD>(a) == 8) rc = run_scan_backward<E, KD, 8>(a, st);
+    else rc = run_scan_backward<E, KD, 4>(a, st);
+  } else {
+    rc = run_scan_backward<E, KD, 4>(a, st);
+  }
+  if (rc != RQF_OK || a.n_chunks == 0) return rc;
+  rc = launch(gradient_kernel<E, KD>, (int64_t)a.batch * a.hv * a.n_chunks, kGradThreads,
+              Grad<KD, Elem<E>::kParts>::kBytes, a, st);
+  if (rc != RQF_OK || a.dq_part == nullptr) return rc;
+  const int64_t rows = a.batch * a.time, pairs = rows * a.hk * (a.kdim / 2);
+  const int64_t blocks = ceil_div(pairs, 256);
+  if (blocks > kMaxGrid) return RQF_ERR_SHAPE;
+  sum_heads_kernel<E><<<(unsigned)blocks, 256, 0, st>>>(a.dq_part, static_cast<E *>(a.dq), rows, a.hk,
+                                                        a.rep, a.kdim);
+  sum_heads_kernel<E><<<(unsigned)blocks, 256, 0, st>>>(a.dk_part, static_cast<E *>(a.dk), rows, a.hk,
+                                                        a.rep, a.kdim);
+  return cudaGetLastError() == cudaSuccess ? RQF_OK : RQF_ERR_LAUNCH;
+}
+
+template <typename F>
+int by_type(int dtype, int kd, F &&f) {
+  const auto by_width = [&](auto e) {
+    return kd == 32    ? f(e, std::integral_constant<int, 32>{})
+           : kd == 64 ? f(e, std::integral_constant<int, 64>{})
+                      : f(e, std::integral_constant<int, 128>{});
+  };
+  return dtype == RQF_F32    ? by_width(float{})
+         : dtype == RQF_BF16 ? by_width(__nv_bfloat16{})
+                             : by_width(__half{});
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t rqf_gated_delta_context_bytes(const rqf_delta_problem *problem, int save) {
+  Sizes s;
+  Args a{};
+  if (sizes_of(problem, &s) != RQF_OK) return SIZE_MAX;
+  return carve_context(nullptr, s, save != 0, &a);
+}
+
+size_t rqf_gated_delta_backward_workspace_bytes(const rqf_delta_problem *problem) {
+  Sizes s;
+  Args a{};
+  if (sizes_of(problem, &s) != RQF_OK) return SIZE_MAX;
+  return carve_workspace(nullptr, problem, s, &a);
+}
+
+int rqf_gated_delta_forward(const rqf_delta_problem *problem, const void *q, const void *k, const void *v,
+                            const float *log_decay, const float *beta, const float *initial_state, void *o,
+                            float *final_state, void *context, int save, rqf_stream_t stream) {
+  Sizes s;
+  int rc = sizes_of(problem, &s);
+  if (rc != RQF_OK) return rc;
+  if (problem->batch == 0) return RQF_OK;
+  if ((rc = check_inputs(problem, q, k, v, log_decay, beta)) != RQF_OK) return rc;
+  if (s.chunks > 0 && (!o || !context)) return RQF_ERR_ARGUMENT;
+  if (!aligned16(o) || !aligned16(context)) return RQF_ERR_ALIGN;
+  if (s.chunks == 0 && final_state == nullptr) return RQF_OK;
+  Args a;
+  common_args(problem, s, &a);
+  a.q = q, a.k = k, a.v = v, a.g = log_decay, a.beta = beta, a.s0 = initial_state, a.o = o;
+  a.sT = final_state;
+  carve_context(context, s, save != 0, &a);
+  return by_type(problem->dtype, s.kd, [&](auto e, auto kd) {
+    return run_forward<decltype(e), decltype(kd)::value>(a, save != 0, reinterpret_cast<cudaStream_t>(stream));
+  });
+}
+
+int rqf_gated_delta_backward(const rqf_delta_problem *problem, const void *v, const void *context,
+                             const void *grad_o, const float *grad_final_state, void *grad_q, void *grad_k,
+                             void *grad_v, float *grad_log_decay, float *grad_beta,
+                             float *grad_initial_state, void *workspace, rqf_stream_t stream) {
+  Sizes s;
+  int rc = sizes_of(problem, &s);
+  if (rc != RQF_OK) return rc;
+  if (problem->batch == 0) return RQF_OK;
+  if (s.chunks > 0 && (!v || !context || !grad_o || !grad_q || !grad_k || !grad_v || !grad_log_decay ||
+                       !grad_beta || !workspace))
+    return RQF_ERR_ARGUMENT;
+  const void *ptrs[] = {v, context, grad_o, grad_q, grad_k, grad_v, workspace};
+  for (const void *p : ptrs)
+    if (!aligned16(p)) return RQF_ERR_ALIGN;
+  const int64_t per = problem->dtype == RQF_F32 ? 4 : 8;
+  for (int i = 0; i < 3; ++i)
+    if (s.chunks > 0 && problem->v_stride[i] % per) return RQF_ERR_ALIGN;
+  if (s.chunks == 0 && grad_initial_state == nullptr) return RQF_OK;
+  Args a;
+  common_args(problem, s, &a);
+  a.v = v, a.dout = grad_o, a.dsT = grad_final_state;
+  a.dq = grad_q, a.dk = grad_k, a.dv = grad_v, a.dg = grad_log_decay, a.dbeta = grad_beta;
+  a.ds0 = grad_initial_state;
+  carve_context(const_cast<void *>(context), s, true, &a);
+  carve_workspace(workspace, problem, s, &a);
+  return by_type(problem->dtype, s.kd, [&](auto e, auto kd) {
+    return run_backward<decltype(e), decltype(kd)::value>(a, reinterpret_cast<cudaStream_t>(stream));
+  });
+}
+
+}  // extern "C"

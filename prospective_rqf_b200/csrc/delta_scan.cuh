@@ -1,0 +1,393 @@
+// The pass from chunk to chunk.  A warp owns 16 columns of V of one value
+// head and keeps that part of the state, transposed (16 x K), in the registers
+// that a tensor-core product sums into, for the whole sequence.  The rows of V
+// never meet, so warps share only the chunk's tiles (k, q, T, P), and each
+// product's sums are laid out as the next one's left operand needs them:
+//
+//   (kS)^T = S^T k^T  ->  r^T  ->  u^T = r^T T^T  ->  o^T, S'^T += u^T k
+//
+// runs with no trip through shared memory.  That is why these products use
+// m16n8k16 and not tcgen05: the chain from one chunk to the next is three
+// dependent products of 64 x 64 x 128 at most, so what counts is the time from
+// one product's sums to the next one's operand.  Tiles come by cp.async, one
+// chunk ahead.
+#pragma once
+
+#include "delta_common.cuh"
+
+namespace rqf {
+namespace delta {
+
+// Shared memory of one chunk: k and q halves, T and P halves, coefficient rows.
+template <int KD, int NP>
+struct Stage {
+  static constexpr int kKq = NP * kC * KD * 2;  // bytes of k or q
+  static constexpr int kK = 0, kQ = kKq, kT = 2 * kKq, kP = kT + 2 * kC * kC * 2;
+  static constexpr int kV = kP + 2 * kC * kC * 2;  // coefficient rows
+  static constexpr int kBytes = kV + kVec * kC * 4;
+};
+template <typename E, int KD, int W>
+constexpr size_t scan_smem() {
+  return 2 * (size_t)Stage<KD, Elem<E>::kParts>::kBytes + (size_t)W * kC * 16 * sizeof(E);
+}
+
+template <int KD, int NP, int THREADS>
+__device__ __forceinline__ void load_stage(uint32_t dst, const Args &a, long long kv_chunk,
+                                           long long chunk, int tid) {
+  using S = Stage<KD, NP>;
+  copy_tile<KD>(dst + S::kK, a.khat + kv_chunk * NP * kC * KD, NP * kC, tid, THREADS);
+  copy_tile<KD>(dst + S::kQ, a.qhat + kv_chunk * NP * kC * KD, NP * kC, tid, THREADS);
+  copy_tile<kC>(dst + S::kT, a.tmat + chunk * 2 * kC * kC, 2 * kC, tid, THREADS);
+  copy_tile<kC>(dst + S::kP, a.pmat + chunk * 2 * kC * kC, 2 * kC, tid, THREADS);
+  const float *vec = a.vec + chunk * kVec * kC;
+  for (int i = tid; i < kVec * kC / 4; i += THREADS) copy16(dst + S::kV + i * 16, vec + i * 4);
+}
+
+// A warp's own 64 x 16 tile of v, o, dO or dv in shared memory, [t][16 of V].
+template <typename E>
+struct WarpTile {
+  static constexpr int kPieces = 16 * sizeof(E) / 16;  // 16-byte pieces of a row: 2 or 4
+  static __device__ __forceinline__ int at(int t, int piece) {
+    return t * 16 * (int)sizeof(E) +
+           16 * (piece ^ (sizeof(E) == 2 ? ((t >> 2) & 1) : ((t >> 1) & 3)));
+  }
+  // rows t0.. of src (row stride `stride`, already at this warp's columns); zeros past
+  // `live` rows and `cols` columns
+  static __device__ __forceinline__ void load(uint32_t tile, const E *src, long long stride,
+                                              int live, int cols, int lane) {
+#pragma unroll
+    for (int i = 0; i < kC * kPieces / 32; ++i) {
+      const int t = (lane + i * 32) / kPieces, p = (lane + i * 32) % kPieces;
+      const int in = cols * (int)sizeof(E) - p * 16;
+      const bool on = t < live && in > 0;
+      copy16z(tile + at(t, p), on ? src + t * stride + p * (16 / sizeof(E)) : src,
+              on ? (in < 16 ? in : 16) : 0);
+    }
+  }
+  // the tile as accumulator tiles of its transpose: x[nt] has V rows g, g + 8 and
+  // tokens nt 8 + 2c, + 1
+  static __device__ __forceinline__ void get(uint32_t tile, const unsigned char *ptr, int lane,
+                                             float (&x)[8][4]) {
+    if constexpr (sizeof(E) == 2) {
+      const int m = lane >> 3, r = lane & 7;
+#pragma unroll
+      for (int np = 0; np < 4; ++np) {
+        uint32_t f[4];
+        ldsm4t(tile + at(np * 16 + (m >> 1) * 8 + r, m & 1), f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const E *e = reinterpret_cast<const E *>(&f[i]);
+          x[2 * np + (i >> 1)][(i & 1) * 2] = Elem<E>::get(e[0]);
+          x[2 * np + (i >> 1)][(i & 1) * 2 + 1] = Elem<E>::get(e[1]);
+        }
+      }
+    } else {
+      const int g = lane >> 2, c = lane & 3;
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int t = nt * 8 + 2 * c + (i & 1), v = g + (i >> 1) * 8;
+          x[nt][i] = *reinterpret_cast<const float *>(ptr + at(t, v >> 2) + (v & 3) * 4);
+        }
+    }
+  }
+  static __device__ __forceinline__ void put(unsigned char *ptr, int lane, const float (&x)[8][4]) {
+    const int g = lane >> 2, c = lane & 3;
+    constexpr int kPer = 16 / sizeof(E);
+#pragma unroll
+    for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = nt * 8 + 2 * c + (i & 1), v = g + (i >> 1) * 8;
+        *reinterpret_cast<E *>(ptr + at(t, v / kPer) + (v % kPer) * sizeof(E)) =
+            Elem<E>::put(x[nt][i]);
+      }
+  }
+  // the tile's first `rows` rows and `cols` columns to dst
+  static __device__ __forceinline__ void store(const unsigned char *ptr, E *dst, long long stride,
+                                               int rows, int cols, int lane) {
+    constexpr int kPer = 16 / sizeof(E);
+#pragma unroll
+    for (int i = 0; i < kC * kPieces / 32; ++i) {
+      const int t = (lane + i * 32) / kPieces, p = (lane + i * 32) % kPieces;
+      if (t < rows && p * kPer < cols)
+        *reinterpret_cast<uint4 *>(dst + t * stride + p * kPer) =
+            *reinterpret_cast<const uint4 *>(ptr + at(t, p));
+    }
+  }
+};
+
+// acc (16 x 64) += A (hi + lo, 16 x 16 of the contraction at ks) times a tile stored [n][k].
+template <int LD, int NP, int NT>
+__device__ __forceinline__ void step_rows(float (&acc)[NT][4], const uint32_t (&hi)[4],
+                                          const uint32_t (&lo)[4], uint32_t tile, uint32_t part,
+                                          int ks, int from, int lane) {
+#pragma unroll
+  for (int np = 0; np < NT / 2; ++np) {
+    if (np < from) continue;
+    uint32_t b[4];
+    ldsm4(b_rows<LD>(tile, np * 16, ks * 16, lane), b);
+    mma(acc[2 * np], hi, b[0], b[1]);
+    mma(acc[2 * np + 1], hi, b[2], b[3]);
+    mma(acc[2 * np], lo, b[0], b[1]);
+    mma(acc[2 * np + 1], lo, b[2], b[3]);
+    if (NP == 2) {
+      ldsm4(b_rows<LD>(tile + part, np * 16, ks * 16, lane), b);
+      mma(acc[2 * np], hi, b[0], b[1]);
+      mma(acc[2 * np + 1], hi, b[2], b[3]);
+    }
+  }
+}
+// The same with a tile stored [k][n], and columns up to `to` pairs.
+template <int LD, int AP, int NP, int NT>
+__device__ __forceinline__ void step_cols(float (&acc)[NT][4], const uint32_t (&hi)[4],
+                                          const uint32_t (&lo)[4], uint32_t tile, uint32_t part,
+                                          int ks, int to, int lane) {
+#pragma unroll
+  for (int np = 0; np < NT / 2; ++np) {
+    if (np > to) continue;
+    uint32_t b[4];
+    ldsm4t(b_cols<LD>(tile, ks * 16, np * 16, lane), b);
+    mma(acc[2 * np], hi, b[0], b[1]);
+    mma(acc[2 * np + 1], hi, b[2], b[3]);
+    if (AP == 2) {
+      mma(acc[2 * np], lo, b[0], b[1]);
+      mma(acc[2 * np + 1], lo, b[2], b[3]);
+    }
+    if (NP == 2) {
+      ldsm4t(b_cols<LD>(tile + part, ks * 16, np * 16, lane), b);
+      mma(acc[2 * np], hi, b[0], b[1]);
+      mma(acc[2 * np + 1], hi, b[2], b[3]);
+    }
+  }
+}
+
+template <int NT>
+__device__ __forceinline__ void zero(float (&x)[NT][4]) {
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[i][j] = 0.f;
+}
+
+// The warp's 16 x KD state against a (K, V) matrix in global memory.
+template <int KD>
+__device__ __forceinline__ void load_state(const float *src, int v0, int kdim, int vdim, int lane,
+                                           float (&S)[KD / 8][4]) {
+  const int g = lane >> 2, c = lane & 3;
+#pragma unroll
+  for (int nt = 0; nt < KD / 8; ++nt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = nt * 8 + 2 * c + (i & 1), v = v0 + g + (i >> 1) * 8;
+      S[nt][i] = src != nullptr && k < kdim && v < vdim ? src[(long long)k * vdim + v] : 0.f;
+    }
+}
+template <int KD>
+__device__ __forceinline__ void store_state(float *dst, int v0, int kdim, int vdim, int lane,
+                                            const float (&S)[KD / 8][4]) {
+  const int g = lane >> 2, c = lane & 3;
+#pragma unroll
+  for (int nt = 0; nt < KD / 8; ++nt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = nt * 8 + 2 * c + (i & 1), v = v0 + g + (i >> 1) * 8;
+      if (k < kdim && v < vdim) dst[(long long)k * vdim + v] = S[nt][i];
+    }
+}
+// Accumulator tiles to a [v][LD] buffer of 32-bit values, at the warp's rows.
+template <int NT>
+__device__ __forceinline__ void save_rows(float *dst, int lane, const float (&x)[NT][4]) {
+  const int g = lane >> 2, c = lane & 3;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    *reinterpret_cast<float2 *>(dst + g * (NT * 8) + nt * 8 + 2 * c) = make_float2(x[nt][0], x[nt][1]);
+    *reinterpret_cast<float2 *>(dst + (g + 8) * (NT * 8) + nt * 8 + 2 * c) =
+        make_float2(x[nt][2], x[nt][3]);
+  }
+}
+
+// Where the backward's last pass finds the largest magnitudes, for its scales.
+enum Max { kMaxS = 0, kMaxU, kMaxDS, kMaxDR, kMaxDO, kMaxes };
+__device__ __forceinline__ void save_max(float *maxes, long long chunk, int which, int warps, int w,
+                                         float m0, float m1, int lane) {
+  float m = fmaxf(m0, m1);
+  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+  if (lane == 0) maxes[(chunk * kMaxes + which) * warps + w] = m;
+}
+
+template <typename E, int KD, int W, bool SAVE>
+__global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
+  constexpr int NP = Elem<E>::kParts;
+  using St = Stage<KD, NP>;
+  using Tile = WarpTile<E>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int c = lane & 3;
+  const int blocks = (a.vp / 16 + W - 1) / W;  // CTAs of a head
+  const long long bh = blockIdx.x / blocks;
+  const int b = (int)(bh / a.hv), h = (int)(bh % a.hv), hk = h / a.rep;
+  const int w = (int)(blockIdx.x % blocks) * W + warp;  // this warp's 16 columns of V
+  const int v0 = w * 16;
+  const bool on = v0 < a.vp;
+  const int cols = min(16, a.vdim - v0);
+  const long long len = row_length(a, b);
+  const int chunks = (int)((len + kC - 1) / kC);
+  const long long kv_first = ((long long)b * a.hk + hk) * a.n_chunks, first = bh * a.n_chunks;
+  const uint32_t base = smem_u32(smem);
+  unsigned char *mine = smem + 2 * St::kBytes + warp * kC * 16 * sizeof(E);
+  const uint32_t tile = smem_u32(mine);
+  const E *v = static_cast<const E *>(a.v) + b * a.sv.b + h * a.sv.h + v0;
+  E *o = static_cast<E *>(a.o) + ((long long)b * a.time * a.hv + h) * a.vdim + v0;
+  const long long so = (long long)a.hv * a.vdim;
+
+  float S[KD / 8][4];
+  load_state<KD>(a.s0 ? a.s0 + bh * a.kdim * a.vdim : nullptr, on ? v0 : a.vdim, a.kdim, a.vdim, lane, S);
+
+  if (chunks > 0) {
+    load_stage<KD, NP, W * 32>(base, a, kv_first, first, tid);
+    copy_commit();
+    if (on) Tile::load(tile, v, a.sv.t, (int)min((long long)kC, len), cols, lane);
+    copy_commit();
+  }
+  for (int n = 0; n < chunks; ++n) {
+    const uint32_t st = base + (n & 1) * St::kBytes;
+    const float *vec = reinterpret_cast<const float *>(smem + (n & 1) * St::kBytes + St::kV);
+    const long long t0 = (long long)n * kC;
+    copy_wait<1>();  // this chunk's tiles; its v may still be on the way
+    __syncthreads();
+    if (n + 1 < chunks)
+      load_stage<KD, NP, W * 32>(base + ((n + 1) & 1) * St::kBytes, a, kv_first + n + 1,
+                                 first + n + 1, tid);
+    copy_commit();
+    if (on) {
+      float m0, m1;
+      row_max(S, m0, m1);
+      const float big0 = m0, big1 = m1;
+      const Scale s0 = scale_for(m0), s1 = scale_for(m1);
+      if (SAVE) {
+        save_rows(a.states + ((first + n) * a.vp + v0) * KD, lane, S);
+        save_max(a.maxes, first + n, kMaxS, a.vp / 16, w, m0, m1, lane);
+      }
+      float r[8][4], qs[8][4];
+      zero(r);
+      zero(qs);
+#pragma unroll
+      for (int ks = 0; ks < KD / 16; ++ks) {
+        uint32_t hi[4], lo[4];
+        split_frag(S, ks, s0.mul, s1.mul, hi, lo);
+        step_rows<KD, NP>(r, hi, lo, st + St::kK, kC * KD * 2, ks, 0, lane);
+        step_rows<KD, NP>(qs, hi, lo, st + St::kQ, kC * KD * 2, ks, 0, lane);
+      }
+      copy_wait<1>();
+      __syncwarp();
+      {
+        float x[8][4];
+        Tile::get(tile, mine, lane, x);
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt) {
+          const float2 f = *reinterpret_cast<const float2 *>(vec + kRowKS * kC + nt * 8 + 2 * c);
+          const float2 be = *reinterpret_cast<const float2 *>(vec + kRowBeta * kC + nt * 8 + 2 * c);
+          r[nt][0] = be.x * x[nt][0] - f.x * (s0.inv * r[nt][0]);
+          r[nt][1] = be.y * x[nt][1] - f.y * (s0.inv * r[nt][1]);
+          r[nt][2] = be.x * x[nt][2] - f.x * (s1.inv * r[nt][2]);
+          r[nt][3] = be.y * x[nt][3] - f.y * (s1.inv * r[nt][3]);
+        }
+      }
+      float u[8][4], y[8][4];
+      uint32_t hi[4], lo[4];
+      row_max(r, m0, m1);
+      Scale x0 = scale_for(m0), x1 = scale_for(m1);
+      zero(u);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        split_frag(r, ks, x0.mul, x1.mul, hi, lo);
+        step_rows<kC, 2>(u, hi, lo, st + St::kT, kC * kC * 2, ks, ks, lane);
+      }
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt) {
+        const float2 f = *reinterpret_cast<const float2 *>(vec + kRowT * kC + nt * 8 + 2 * c);
+        u[nt][0] *= f.x * x0.inv;
+        u[nt][1] *= f.y * x0.inv;
+        u[nt][2] *= f.x * x1.inv;
+        u[nt][3] *= f.y * x1.inv;
+      }
+      row_max(u, m0, m1);
+      if (SAVE) {
+        save_rows(a.us + ((first + n) * a.vp + v0) * kC, lane, u);
+        save_max(a.maxes, first + n, kMaxU, a.vp / 16, w, m0, m1, lane);
+      }
+      x0 = scale_for(m0), x1 = scale_for(m1);
+      zero(y);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        split_frag(u, ks, x0.mul, x1.mul, hi, lo);
+        step_rows<kC, 2>(y, hi, lo, st + St::kP, kC * kC * 2, ks, ks, lane);
+      }
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt) {
+        const float2 p = *reinterpret_cast<const float2 *>(vec + kRowP * kC + nt * 8 + 2 * c);
+        const float2 q = *reinterpret_cast<const float2 *>(vec + kRowO * kC + nt * 8 + 2 * c);
+        y[nt][0] = p.x * (x0.inv * y[nt][0]) + q.x * (s0.inv * qs[nt][0]);
+        y[nt][1] = p.y * (x0.inv * y[nt][1]) + q.y * (s0.inv * qs[nt][1]);
+        y[nt][2] = p.x * (x1.inv * y[nt][2]) + q.x * (s1.inv * qs[nt][2]);
+        y[nt][3] = p.y * (x1.inv * y[nt][3]) + q.y * (s1.inv * qs[nt][3]);
+      }
+      __syncwarp();
+      Tile::put(mine, lane, y);
+      __syncwarp();
+      Tile::store(mine, o + t0 * so, so, (int)min((long long)kC, a.time - t0), cols, lane);
+      __syncwarp();
+      if (n + 1 < chunks)
+        Tile::load(tile, v + (t0 + kC) * a.sv.t, a.sv.t, (int)min((long long)kC, len - t0 - kC),
+                   cols, lane);
+
+      const float gam = vec[kRowEG * kC + kC - 1];
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt) {
+        const float2 f = *reinterpret_cast<const float2 *>(vec + kRowU * kC + nt * 8 + 2 * c);
+        u[nt][0] *= f.x;
+        u[nt][1] *= f.y;
+        u[nt][2] *= f.x;
+        u[nt][3] *= f.y;
+      }
+      row_max(u, m0, m1);
+      x0 = scale_beside(m0, gam * big0), x1 = scale_beside(m1, gam * big1);
+#pragma unroll
+      for (int nt = 0; nt < KD / 8; ++nt) {
+        S[nt][0] *= gam * x0.mul;
+        S[nt][1] *= gam * x0.mul;
+        S[nt][2] *= gam * x1.mul;
+        S[nt][3] *= gam * x1.mul;
+      }
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        split_frag(u, ks, x0.mul, x1.mul, hi, lo);
+        step_cols<KD, 2, NP>(S, hi, lo, st + St::kK, kC * KD * 2, ks, KD, lane);
+      }
+#pragma unroll
+      for (int nt = 0; nt < KD / 8; ++nt) {
+        S[nt][0] *= x0.inv;
+        S[nt][1] *= x0.inv;
+        S[nt][2] *= x1.inv;
+        S[nt][3] *= x1.inv;
+      }
+    }
+    copy_commit();
+  }
+  copy_wait<0>();
+  if (!on) return;
+  if (a.sT != nullptr)
+    store_state<KD>(a.sT + bh * a.kdim * a.vdim, v0, a.kdim, a.vdim, lane, S);
+  // tokens past the row's end: zeros
+  constexpr int kPer = 16 / sizeof(E), kPieces = 16 / kPer;
+  for (long long t = (long long)chunks * kC + lane / kPieces; t < a.time; t += 32 / kPieces)
+    if ((lane % kPieces) * kPer < cols)
+      *reinterpret_cast<uint4 *>(o + t * so + (lane % kPieces) * kPer) = make_uint4(0, 0, 0, 0);
+}
+
+}  // namespace delta
+}  // namespace rqf

@@ -17,6 +17,8 @@
 #include "fbt_rank1.cuh"
 #include "fbt_scan.cuh"
 #include "coeffs.cuh"
+#include "delta_step.cuh"
+#include "grad_norm.cuh"
 #include "lowrank.cuh"
 #include "readout.cuh"
 #include "reduce.cuh"
@@ -2110,6 +2112,172 @@ int rqf_two_tap_coefficients_backward(const float *log_theta, const float *log_g
   return rqf_filter_two_tap_coefficients_backward(&L, &o, grad_c1, grad_tap0, grad_tap1,
                                                   grad_log_theta, grad_log_gamma, nullptr,
                                                   nullptr, n, stream);
+}
+
+}  // extern "C"
+
+// ------------------------------------------------ gated delta rule, one token
+extern "C" {
+
+int rqf_gated_delta_step(const rqf_delta_problem *problem, const void *q, const void *k,
+                         const void *v, const float *log_decay, const float *beta,
+                         const void *slots, int slots_64, int64_t pool, float *state, void *o,
+                         rqf_stream_t stream) {
+  const rqf_delta_problem *p = problem;
+  if (p == nullptr) return RQF_ERR_ARGUMENT;
+  if (p->batch < 0 || p->key_heads <= 0 || p->value_heads <= 0 || p->key_dim <= 0 ||
+      p->value_dim <= 0 || pool < 0 || p->value_heads % p->key_heads != 0 || p->key_dim % 8 != 0 ||
+      p->value_dim % 8 != 0 || p->key_dim > delta_step::kMaxK || p->value_heads > 0x7fffffffLL ||
+      p->value_dim > 0x7fffffffLL)
+    return RQF_ERR_SHAPE;
+  if (p->dtype != RQF_F32 && p->dtype != RQF_BF16 && p->dtype != RQF_F16) return RQF_ERR_ARGUMENT;
+  if (p->batch == 0) return RQF_OK;
+  if (!slots && p->batch > pool) return RQF_ERR_SHAPE;
+  if (!q || !k || !v || !log_decay || !beta || !o || (pool > 0 && !state)) return RQF_ERR_ARGUMENT;
+  if (!aligned(state, 16)) return RQF_ERR_ALIGN;
+  const double grid = (double)p->batch * (double)p->value_heads *
+                      (double)ceil_div(p->value_dim, delta_step::kCols);
+  if (grid > (double)0x7fffffffLL) return RQF_ERR_SHAPE;
+  delta_step::Args a;
+  a.q = q, a.k = k, a.v = v, a.g = log_decay, a.beta = beta;
+  a.qb = p->q_stride[0], a.qh = p->q_stride[2], a.kb = p->k_stride[0], a.kh = p->k_stride[2];
+  a.vb = p->v_stride[0], a.vh = p->v_stride[2], a.gb = p->g_stride[0], a.gh = p->g_stride[2];
+  a.bb = p->beta_stride[0], a.bh = p->beta_stride[2];
+  a.slots = slots, a.slots_64 = slots_64, a.state = state, a.o = o, a.scale = p->scale;
+  a.hv = (int)p->value_heads, a.rep = (int)(p->value_heads / p->key_heads);
+  a.kdim = (int)p->key_dim, a.vdim = (int)p->value_dim, a.pool = pool;
+  const unsigned blocks = (unsigned)grid;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (p->dtype == RQF_F32)
+    delta_step::step_kernel<float><<<blocks, delta_step::kThreads, 0, st>>>(a);
+  else if (p->dtype == RQF_BF16)
+    delta_step::step_kernel<__nv_bfloat16><<<blocks, delta_step::kThreads, 0, st>>>(a);
+  else
+    delta_step::step_kernel<__half><<<blocks, delta_step::kThreads, 0, st>>>(a);
+  return launch_status();
+}
+
+}  // extern "C"
+
+// ------------------------------------------------ gradient norm and clipping
+namespace {
+
+constexpr int64_t kGradTable = gradnorm::kTables[2];
+
+int64_t grad_launches(int64_t n) { return n <= 0 ? 0 : ceil_div(n, kGradTable); }
+
+template <int N>
+int grad_pass(const gradnorm::Entry *e, int count, int tiles, bool clip, double *partials,
+              int n_partials, float max_norm, float *norm, cudaStream_t st) {
+  gradnorm::Table<N> t;
+  t.count = count;
+  t.tiles = tiles;
+  for (int i = 0; i < count; ++i) t.e[i] = e[i];
+  const unsigned grid = (unsigned)(tiles < gradnorm::kMaxGrid ? tiles : gradnorm::kMaxGrid);
+  if (clip)
+    gradnorm::clip_kernel<N><<<grid, gradnorm::kThreads, 0, st>>>(t, partials, n_partials, max_norm,
+                                                                  norm);
+  else
+    gradnorm::squares_kernel<N><<<grid, gradnorm::kThreads, 0, st>>>(t, partials);
+  return launch_status();
+}
+
+// One pass over the tensors, in launches of up to kGradTable of them.  Returns
+// the number of partial sums in *n_partials.
+int grad_launch(const void *const *grads, void *const *outs, const int64_t *numel, const int *dtype,
+                int64_t n, bool clip, double *partials, int *n_partials, float max_norm, float *norm,
+                cudaStream_t st) {
+  static thread_local gradnorm::Entry entries[kGradTable];
+  int sums = 0;
+  for (int64_t i = 0; i < n;) {
+    int count = 0;
+    int64_t tiles = 0;
+    for (; i < n && count < kGradTable; ++i) {
+      if (numel[i] == 0) continue;
+      const int64_t per = dtype[i] == RQF_C64 ? 2 : 1, size = dtype[i] == RQF_F32 || per == 2 ? 4 : 2;
+      const int64_t each = ceil_div(numel[i] * per * size + 15, gradnorm::kTileBytes);
+      if (tiles + each > 0x7fffffffLL) {
+        if (count == 0) return RQF_ERR_SHAPE;
+        break;
+      }
+      gradnorm::Entry &e = entries[count++];
+      e.src = grads[i];
+      e.dst = outs ? outs[i] : nullptr;
+      e.n = numel[i] * per;
+      e.tile = (int)tiles;
+      e.type = dtype[i] == RQF_BF16 ? gradnorm::kBF16 : dtype[i] == RQF_F16 ? gradnorm::kF16 : gradnorm::kF32;
+      tiles += each;
+    }
+    if (count == 0) break;
+    int rc;
+    double *to = clip ? partials : partials + sums;
+    if (count <= gradnorm::kTables[0])
+      rc = grad_pass<gradnorm::kTables[0]>(entries, count, (int)tiles, clip, to, *n_partials, max_norm, norm, st);
+    else if (count <= gradnorm::kTables[1])
+      rc = grad_pass<gradnorm::kTables[1]>(entries, count, (int)tiles, clip, to, *n_partials, max_norm, norm, st);
+    else
+      rc = grad_pass<gradnorm::kTables[2]>(entries, count, (int)tiles, clip, to, *n_partials, max_norm, norm, st);
+    if (rc != RQF_OK) return rc;
+    sums += (int)(tiles < gradnorm::kMaxGrid ? tiles : gradnorm::kMaxGrid);
+  }
+  if (!clip) *n_partials = sums;
+  return RQF_OK;
+}
+
+int grad_check(const void *const *grads, void *const *outs, const int64_t *numel, const int *dtype,
+               int64_t n) {
+  if (n < 0 || n > 1000000) return RQF_ERR_SHAPE;
+  if (n > 0 && (!grads || !numel || !dtype)) return RQF_ERR_ARGUMENT;
+  for (int64_t i = 0; i < n; ++i) {
+    if (numel[i] < 0 || numel[i] > (1LL << 44)) return RQF_ERR_SHAPE;
+    if (dtype[i] < RQF_F32 || dtype[i] > RQF_C64) return RQF_ERR_ARGUMENT;
+    if (numel[i] == 0) continue;
+    if (!grads[i] || (outs && !outs[i])) return RQF_ERR_ARGUMENT;
+    const size_t size = dtype[i] == RQF_F32 || dtype[i] == RQF_C64 ? 4 : 2;
+    if (!aligned(grads[i], size) || (outs && !aligned(outs[i], size))) return RQF_ERR_ALIGN;
+  }
+  return RQF_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t rqf_grad_norm_scratch_bytes(int64_t n) {
+  return round256((size_t)(grad_launches(n) + 1) * gradnorm::kMaxGrid * sizeof(double));
+}
+
+int rqf_global_grad_norm(const void *const *grads, const int64_t *numel, const int *dtype, int64_t n,
+                         float *norm, void *scratch, rqf_stream_t stream) {
+  int rc = grad_check(grads, nullptr, numel, dtype, n);
+  if (rc != RQF_OK) return rc;
+  if (!norm || !scratch) return RQF_ERR_ARGUMENT;
+  if (!aligned(scratch, 8)) return RQF_ERR_ALIGN;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  int sums = 0;
+  rc = grad_launch(grads, nullptr, numel, dtype, n, false, static_cast<double *>(scratch), &sums, 0.f,
+                   norm, st);
+  if (rc != RQF_OK) return rc;
+  gradnorm::norm_kernel<<<1, gradnorm::kThreads, 0, st>>>(static_cast<const double *>(scratch), sums, norm);
+  return launch_status();
+}
+
+int rqf_clip_grads(const void *const *grads, void *const *outs, const int64_t *numel, const int *dtype,
+                   int64_t n, float max_norm, float *norm, void *scratch, rqf_stream_t stream) {
+  int rc = grad_check(grads, outs, numel, dtype, n);
+  if (rc != RQF_OK) return rc;
+  if ((n > 0 && !outs) || !norm || !scratch) return RQF_ERR_ARGUMENT;
+  if (!aligned(scratch, 8)) return RQF_ERR_ALIGN;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  int sums = 0;
+  double *partials = static_cast<double *>(scratch);
+  rc = grad_launch(grads, outs, numel, dtype, n, false, partials, &sums, 0.f, norm, st);
+  if (rc != RQF_OK) return rc;
+  if (sums == 0) {  // nothing to scale
+    gradnorm::norm_kernel<<<1, gradnorm::kThreads, 0, st>>>(partials, 0, norm);
+    return launch_status();
+  }
+  return grad_launch(grads, outs, numel, dtype, n, true, partials, &sums, max_norm, norm, st);
 }
 
 }  // extern "C"
