@@ -203,6 +203,26 @@ def load() -> ctypes.CDLL:
     return _LIB
 
 
+_NATIVE = None
+
+
+def native():
+    """The binding that calls the library without ctypes (csrc/binding.cpp); raises if it was not
+    built."""
+    global _NATIVE
+    if _NATIVE is None:
+        load()
+        try:
+            from . import _native
+        except ImportError as e:
+            raise ImportError(
+                f"{_PKG / '_native.so'} is missing or does not load ({e}): build it with "
+                "prospective_rqf_b200._build.build()") from e
+        _native.set_error(RQFError)
+        _NATIVE = _native
+    return _NATIVE
+
+
 def status_string(code: int) -> str:
     return load().rqf_status_string(int(code)).decode()
 

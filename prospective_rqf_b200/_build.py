@@ -1,16 +1,19 @@
-"""Build librqf_b200.so (the C-ABI CUDA library) in-tree for sm_100a."""
+"""Build librqf_b200.so (the C-ABI CUDA library, sm_100a) and _native.so (the Python binding of
+the operators where the host's share counts) in-tree."""
 
 from __future__ import annotations
 
 import os
 import shutil
 import subprocess
+import sysconfig
 import tempfile
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "librqf_b200.so"
+NATIVE = PKG / "_native.so"
 ROOT = PKG.parent
 
 NVCC_FLAGS = [
@@ -28,20 +31,37 @@ def _nvcc() -> str:
 
 
 def sources() -> list[Path]:
-    return sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + [ROOT / "include" / "rqf_b200.h"]
+    return sorted(CSRC.glob("*.cpp")) + sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + [ROOT / "include" / "rqf_b200.h"]
 
 
 def needs_build() -> bool:
-    if not LIB.exists():
+    if not LIB.exists() or not NATIVE.exists():
         return True
-    t = LIB.stat().st_mtime
+    t = min(LIB.stat().st_mtime, NATIVE.stat().st_mtime)
     return any(p.stat().st_mtime > t for p in sources())
+
+
+def _native_command(out: Path) -> list[str]:
+    """The compile and link of csrc/binding.cpp, which calls the C-ABI library next to it."""
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(_nvcc()).resolve().parents[1]
+    return [os.environ.get("CXX") or shutil.which("g++") or "g++", "-std=c++17", "-O2", "-fPIC",
+            "-shared", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            "-isystem", str(root / "include"),
+            "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
+            "-isystem", sysconfig.get_paths()["include"], "-isystem", str(cuda / "include"),
+            "-o", str(out), str(CSRC / "binding.cpp"), f"-L{PKG}", f"-l:{LIB.name}",
+            f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+            "-Wl,-rpath,$ORIGIN"]
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compile every csrc/*.cu (rqf_b200.cu and delta_rule.cu, which include the
     kernel headers) side by side and link them into
-    prospective_rqf_b200/librqf_b200.so."""
+    prospective_rqf_b200/librqf_b200.so, then csrc/binding.cpp into _native.so."""
     if not force and not needs_build():
         return LIB
     nvcc = _nvcc()
@@ -64,6 +84,11 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     os.replace(tmp, LIB)
     if verbose:
         print("".join(logs))
+    tmp = NATIVE.with_suffix(".so.tmp")
+    res = subprocess.run(_native_command(tmp), capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"the Python binding failed to build ({res.returncode}):\n{res.stderr}")
+    os.replace(tmp, NATIVE)
     return LIB
 
 

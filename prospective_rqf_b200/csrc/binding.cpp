@@ -1,0 +1,456 @@
+// Python binding of the operators that are called often on little work: the
+// gated delta rule and the gradients' norm.  A decode step's kernel takes 3 us
+// and a model has hundreds of gradients, so what a call costs on the host
+// counts: here it is checked, described to the C ABI and launched without
+// going through the interpreter (ctypes took 35 us for a step, and 3 us for
+// each tensor of a list).
+//
+// Refusals raise ValueError (shapes, types), RuntimeError (not CUDA tensors)
+// or RQFError (a status of the C ABI), as the ctypes callers do.
+#include <Python.h>
+
+#include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <string>
+#include <utility>
+#include <vector>
+
+#include "../../include/rqf_b200.h"
+
+namespace {
+
+using at::Tensor;
+
+PyObject *g_error = nullptr;  // RQFError
+
+struct StatusError {
+  int code;
+  const char *what;
+};
+void check(int code, const char *what) {
+  if (code != RQF_OK) throw StatusError{code, what};
+}
+
+rqf_stream_t stream_on(const Tensor &t) {
+  return reinterpret_cast<rqf_stream_t>(c10::cuda::getCurrentCUDAStream(t.get_device()).stream());
+}
+
+Tensor tensor_arg(PyObject *o, const char *name) {
+  if (!THPVariable_Check(o)) {
+    PyErr_Format(PyExc_TypeError, "%s must be a tensor, got %s", name, Py_TYPE(o)->tp_name);
+    throw python_error();
+  }
+  return THPVariable_Unpack(o);
+}
+Tensor optional_arg(PyObject *o, const char *name) { return o == Py_None ? Tensor() : tensor_arg(o, name); }
+
+void same_cuda(std::initializer_list<const Tensor *> ts) {
+  const Tensor *first = nullptr;
+  for (const Tensor *t : ts) {
+    if (!t->defined()) continue;
+    TORCH_CHECK(t->is_cuda(), "prospective_rqf_b200 runs on CUDA tensors only (no CPU fallback); got a tensor on ",
+                t->device());
+    if (!first) first = t;
+    TORCH_CHECK(t->device() == first->device(), "tensors on different devices: ", first->device(), " and ",
+                t->device());
+  }
+}
+
+// A shape for a message.  Numbers go into messages as strings: the streams of
+// this module's libstdc++ and of torch's do not share their number formatting.
+std::string text(at::IntArrayRef sizes) {
+  std::string out = "(";
+  for (size_t i = 0; i < sizes.size(); ++i) out += (i ? ", " : "") + std::to_string(sizes[i]);
+  return out + ")";
+}
+
+int dtype_of(const Tensor &t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return RQF_F32;
+    case at::kBFloat16: return RQF_BF16;
+    case at::kHalf: return RQF_F16;
+    case at::kComplexFloat: return RQF_C64;
+    default: return -1;
+  }
+}
+
+// A tensor whose last axis is dense; with `wide`, whose rows start on 16 bytes too.
+Tensor laid_out(const Tensor &t, bool wide) {
+  if (t.numel() == 0) return t;
+  bool ok = t.stride(-1) == 1;
+  if (wide) {
+    const int64_t per = 16 / t.element_size();
+    ok = ok && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+    for (int64_t i = 0; ok && i + 1 < t.dim(); ++i) ok = t.stride(i) % per == 0;
+  }
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+constexpr int64_t kMaxKey = 128;
+
+// Shapes and types of one call, `lead` axes (batch, or batch and time) before the heads.
+void check_delta(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, const Tensor &beta, int lead) {
+  const Tensor *ts[] = {&q, &k, &v, &g, &beta};
+  const char *names[] = {"q", "k", "v", "log_decay", "beta"};
+  for (int i = 0; i < 5; ++i)
+    TORCH_CHECK_VALUE(ts[i]->dim() == lead + (i < 3 ? 2 : 1), names[i], " must have ",
+                      std::to_string(lead + (i < 3 ? 2 : 1)), " axes, got shape ", text(ts[i]->sizes()));
+  const int type = dtype_of(v);
+  TORCH_CHECK_VALUE(type >= RQF_F32 && type <= RQF_F16 && q.scalar_type() == v.scalar_type() &&
+                        k.scalar_type() == v.scalar_type(),
+                    "q, k and v must all be float32, bfloat16 or float16, got ", q.scalar_type(), ", ",
+                    k.scalar_type(), ", ", v.scalar_type());
+  TORCH_CHECK_VALUE(q.sizes() == k.sizes(), "q and k must have one shape, got ", text(q.sizes()), " and ", text(k.sizes()));
+  for (int i = 0; i < lead; ++i)
+    TORCH_CHECK_VALUE(v.size(i) == q.size(i), "q and v do not match: ", text(q.sizes()), " and ", text(v.sizes()));
+  for (int i = 3; i < 5; ++i) {
+    TORCH_CHECK_VALUE(at::isFloatingType(ts[i]->scalar_type()), names[i], " must be floating point, got ",
+                      ts[i]->scalar_type());
+    TORCH_CHECK_VALUE(ts[i]->sizes() == v.sizes().slice(0, lead + 1), names[i], " must have shape ",
+                      text(v.sizes().slice(0, lead + 1)), ", got ", text(ts[i]->sizes()));
+  }
+  const int64_t hk = q.size(-2), dk = q.size(-1), hv = v.size(-2), dv = v.size(-1);
+  TORCH_CHECK_VALUE(hk > 0 && hv > 0 && hv % hk == 0, std::to_string(hv),
+                    " value heads cannot share ", std::to_string(hk), " key heads");
+  TORCH_CHECK_VALUE(dk > 0 && dv > 0 && dk % 8 == 0 && dv % 8 == 0 && dk <= kMaxKey,
+                    "head sizes must be multiples of 8 and the keys' at most ", std::to_string(kMaxKey), ", got ",
+                    std::to_string(dk), " and ", std::to_string(dv));
+}
+void check_state(const Tensor &s, at::IntArrayRef shape, const char *name) {
+  TORCH_CHECK_VALUE(s.scalar_type() == at::kFloat && s.sizes() == shape, name, " must be float32 ", text(shape),
+                    ", got ", s.scalar_type(), " ", text(s.sizes()));
+}
+Tensor index_arg(const Tensor &t, int64_t n, const char *name) {
+  TORCH_CHECK_VALUE((t.scalar_type() == at::kInt || t.scalar_type() == at::kLong) && t.dim() == 1 && t.size(0) == n,
+                    name, " must be ", std::to_string(n), " integers, got ", t.scalar_type(), " ", text(t.sizes()));
+  return t.contiguous();
+}
+
+rqf_delta_problem describe(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, const Tensor &beta,
+                           const Tensor &lengths, double scale) {
+  rqf_delta_problem p{};
+  const bool steps = v.dim() == 4;
+  p.batch = v.size(0);
+  p.time = steps ? v.size(1) : 1;
+  p.key_heads = q.size(-2), p.key_dim = q.size(-1);
+  p.value_heads = v.size(-2), p.value_dim = v.size(-1);
+  const auto put = [steps](int64_t (&to)[3], const Tensor &t) {
+    to[0] = t.stride(0);
+    to[1] = steps ? t.stride(1) : 0;
+    to[2] = t.stride(steps ? 2 : 1);
+  };
+  put(p.q_stride, q), put(p.k_stride, k), put(p.v_stride, v), put(p.g_stride, g), put(p.beta_stride, beta);
+  p.lengths = lengths.defined() ? lengths.const_data_ptr<int64_t>() : nullptr;
+  p.dtype = dtype_of(v);
+  p.scale = static_cast<float>(scale);
+  return p;
+}
+
+double scale_arg(PyObject *o, int64_t key_dim) {
+  if (o == Py_None) return 1.0 / std::sqrt(static_cast<double>(key_dim));
+  const double x = PyFloat_AsDouble(o);
+  if (PyErr_Occurred()) throw python_error();
+  return x;
+}
+
+void *data(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+const float *floats(const Tensor &t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; }
+
+// A write through a pointer, as autograd counts writes.
+void written(const Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+Tensor scratch_of(size_t bytes, const Tensor &like) {
+  return at::empty({static_cast<int64_t>(bytes < 256 ? 256 : bytes)}, like.options().dtype(at::kByte));
+}
+
+// What every entry does about errors.
+template <typename F>
+PyObject *guarded(F &&f) {
+  HANDLE_TH_ERRORS
+  const c10::NoGradGuard no_grad;
+  try {
+    return f();
+  } catch (const StatusError &e) {
+    PyErr_Format(g_error, "rqf_b200 %s failed: %s (status %d)", e.what, rqf_status_string(e.code), e.code);
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+bool arity(Py_ssize_t n, Py_ssize_t want, const char *name) {
+  if (n == want) return true;
+  PyErr_Format(PyExc_TypeError, "%s takes %zd arguments, got %zd", name, want, n);
+  return false;
+}
+PyObject *wrap(const Tensor &t) {
+  if (!t.defined()) Py_RETURN_NONE;
+  return THPVariable_Wrap(t);
+}
+PyObject *tuple_of(std::initializer_list<Tensor> ts) {
+  PyObject *out = PyTuple_New(static_cast<Py_ssize_t>(ts.size()));
+  Py_ssize_t i = 0;
+  for (const Tensor &t : ts) PyTuple_SET_ITEM(out, i++, wrap(t));
+  return out;
+}
+
+// delta_forward(q, k, v, log_decay, beta, initial_state, lengths, scale, save)
+//   -> o, final_state, context, q, k, v, log_decay, beta, lengths (as the call took them)
+PyObject *delta_forward(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (!arity(n, 9, "delta_forward")) return nullptr;
+  return guarded([&]() -> PyObject * {
+    Tensor q = tensor_arg(a[0], "q"), k = tensor_arg(a[1], "k"), v = tensor_arg(a[2], "v");
+    Tensor g = tensor_arg(a[3], "log_decay"), b = tensor_arg(a[4], "beta");
+    Tensor s0 = optional_arg(a[5], "initial_state"), lengths = optional_arg(a[6], "lengths");
+    check_delta(q, k, v, g, b, 2);
+    if (s0.defined()) check_state(s0, {v.size(0), v.size(2), q.size(3), v.size(3)}, "initial_state");
+    if (lengths.defined()) lengths = index_arg(lengths, v.size(0), "lengths");
+    same_cuda({&q, &k, &v, &g, &b, &s0, &lengths});
+    const double scale = scale_arg(a[7], q.size(3));
+    const int save = PyObject_IsTrue(a[8]);
+    const c10::cuda::CUDAGuard device(v.device());
+    q = laid_out(q, true), k = laid_out(k, true), v = laid_out(v, true);
+    g = g.to(at::kFloat), b = b.to(at::kFloat);
+    if (s0.defined()) s0 = s0.contiguous();
+    if (lengths.defined()) lengths = lengths.to(at::kLong);
+    Tensor o = at::empty(v.sizes(), v.options());
+    Tensor last = at::empty({v.size(0), v.size(2), q.size(3), v.size(3)}, v.options().dtype(at::kFloat));
+    const rqf_delta_problem p = describe(q, k, v, g, b, lengths, scale);
+    const size_t bytes = rqf_gated_delta_context_bytes(&p, save);
+    TORCH_CHECK_VALUE(bytes != SIZE_MAX, "gated_delta_scan does not take q ", text(q.sizes()), ", v ",
+                      text(v.sizes()));
+    Tensor context = scratch_of(bytes, v);
+    check(rqf_gated_delta_forward(&p, data(q), data(k), data(v), floats(g), floats(b), floats(s0), data(o),
+                                  last.data_ptr<float>(), data(context), save, stream_on(v)),
+          "rqf_gated_delta_forward");
+    if (!save) return tuple_of({o, last, Tensor()});
+    return tuple_of({o, last, context, q, k, v, g, b, lengths});
+  });
+}
+
+// delta_backward(q, k, v, log_decay, beta, lengths, context, scale, grad_o, grad_final_state,
+//   want_initial) -> grad_q, grad_k, grad_v, grad_log_decay, grad_beta, grad_initial_state
+PyObject *delta_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (!arity(n, 11, "delta_backward")) return nullptr;
+  return guarded([&]() -> PyObject * {
+    const Tensor q = tensor_arg(a[0], "q"), k = tensor_arg(a[1], "k"), v = tensor_arg(a[2], "v");
+    const Tensor g = tensor_arg(a[3], "log_decay"), b = tensor_arg(a[4], "beta");
+    const Tensor lengths = optional_arg(a[5], "lengths"), context = tensor_arg(a[6], "context");
+    const double scale = scale_arg(a[7], q.size(3));
+    Tensor go = optional_arg(a[8], "grad_o"), gl = optional_arg(a[9], "grad_final_state");
+    const int want = PyObject_IsTrue(a[10]);
+    const c10::cuda::CUDAGuard device(v.device());
+    go = go.defined() ? go.to(v.scalar_type()).contiguous() : at::zeros(v.sizes(), v.options());
+    go = laid_out(go, true);
+    if (gl.defined()) gl = gl.to(at::kFloat).contiguous();
+    Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(q.sizes(), q.options());
+    Tensor dv = at::empty(v.sizes(), v.options());
+    Tensor dg = at::empty(g.sizes(), g.options()), db = at::empty(g.sizes(), g.options());
+    Tensor ds0;
+    if (want) ds0 = at::empty({v.size(0), v.size(2), q.size(3), v.size(3)}, g.options());
+    const rqf_delta_problem p = describe(q, k, v, g, b, lengths, scale);
+    Tensor work = scratch_of(rqf_gated_delta_backward_workspace_bytes(&p), v);
+    check(rqf_gated_delta_backward(&p, data(v), data(context), data(go), floats(gl), data(dq), data(dk), data(dv),
+                                   dg.data_ptr<float>(), db.data_ptr<float>(),
+                                   want ? ds0.data_ptr<float>() : nullptr, data(work), stream_on(v)),
+          "rqf_gated_delta_backward");
+    return tuple_of({dq, dk, dv, dg, db, ds0});
+  });
+}
+
+// delta_step(q, k, v, log_decay, beta, state, slots, scale) -> o
+PyObject *delta_step(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (!arity(n, 8, "delta_step")) return nullptr;
+  return guarded([&]() -> PyObject * {
+    Tensor q = tensor_arg(a[0], "q"), k = tensor_arg(a[1], "k"), v = tensor_arg(a[2], "v");
+    Tensor g = tensor_arg(a[3], "log_decay"), b = tensor_arg(a[4], "beta");
+    Tensor state = tensor_arg(a[5], "state"), slots = optional_arg(a[6], "slots");
+    check_delta(q, k, v, g, b, 1);
+    check_state(state, {state.dim() ? state.size(0) : 0, v.size(1), q.size(2), v.size(2)}, "state");
+    TORCH_CHECK_VALUE(state.is_contiguous() && reinterpret_cast<uintptr_t>(state.const_data_ptr()) % 16 == 0,
+                      "state must be dense and start on 16 bytes: it is updated in place");
+    if (slots.defined())
+      slots = index_arg(slots, v.size(0), "slots");
+    else
+      TORCH_CHECK_VALUE(state.size(0) >= v.size(0), std::to_string(v.size(0)),
+                        " rows do not fit a pool of ", std::to_string(state.size(0)), " states");
+    same_cuda({&q, &k, &v, &g, &b, &state, &slots});
+    const double scale = scale_arg(a[7], q.size(2));
+    const c10::cuda::CUDAGuard device(v.device());
+    q = laid_out(q, false), k = laid_out(k, false), v = laid_out(v, false);
+    g = g.to(at::kFloat), b = b.to(at::kFloat);
+    Tensor o = at::empty(v.sizes(), v.options());
+    const rqf_delta_problem p = describe(q, k, v, g, b, Tensor(), scale);
+    check(rqf_gated_delta_step(&p, data(q), data(k), data(v), floats(g), floats(b), data(slots),
+                               slots.defined() && slots.scalar_type() == at::kLong, state.size(0),
+                               state.data_ptr<float>(), data(o), stream_on(v)),
+          "rqf_gated_delta_step");
+    written(state);
+    return wrap(o);
+  });
+}
+
+// ---------------------------------------------------------------- gradients
+// Whether the values fill one span of memory, in whatever order of the axes.
+bool filled(const Tensor &t) { return t.is_contiguous() || t.is_non_overlapping_and_dense(); }
+
+struct List {
+  std::vector<Tensor> t;
+  std::vector<void *> ptr;
+  std::vector<int64_t> numel;
+  std::vector<int> dtype;
+  void add(const Tensor &x) {
+    ptr.push_back(x.data_ptr());
+    numel.push_back(x.numel());
+    dtype.push_back(dtype_of(x));
+  }
+};
+
+List list_arg(PyObject *o, const char *name) {
+  List out;
+  if (THPVariable_Check(o)) {
+    out.t.push_back(THPVariable_Unpack(o));
+  } else {
+    PyObject *items = PySequence_Fast(o, "a tensor or a sequence of tensors is wanted");
+    if (!items) throw python_error();
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(items);
+    out.t.reserve(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      PyObject *x = PySequence_Fast_GET_ITEM(items, i);
+      if (!THPVariable_Check(x)) {
+        PyErr_Format(PyExc_TypeError, "%s must hold tensors, got %s", name, Py_TYPE(x)->tp_name);
+        Py_DECREF(items);
+        throw python_error();
+      }
+      out.t.push_back(THPVariable_Unpack(x));
+    }
+    Py_DECREF(items);
+  }
+  out.ptr.reserve(out.t.size());
+  out.numel.reserve(out.t.size());
+  out.dtype.reserve(out.t.size());
+  for (const Tensor &t : out.t) {
+    TORCH_CHECK_VALUE(dtype_of(t) >= 0, name, " must be float32, bfloat16, float16 or complex64, got ",
+                      t.scalar_type());
+    TORCH_CHECK_VALUE(!t.is_conj() && !t.is_neg(), name, " must not be lazy conjugates or negatives: resolve them first");
+    TORCH_CHECK(t.is_cuda(), "prospective_rqf_b200 runs on CUDA tensors only (no CPU fallback); got a tensor on ",
+                t.device());
+    TORCH_CHECK(t.get_device() == out.t[0].get_device(), "tensors on different devices: ", out.t[0].device(), " and ",
+                t.device());
+  }
+  return out;
+}
+
+// grad_norm(grads) -> norm
+PyObject *grad_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (!arity(n, 1, "grad_norm")) return nullptr;
+  return guarded([&]() -> PyObject * {
+    List g = list_arg(a[0], "grads");
+    if (g.t.empty()) return wrap(at::zeros({}));
+    const c10::cuda::CUDAGuard device(g.t[0].device());
+    std::vector<Tensor> copies;
+    for (const Tensor &t : g.t) {
+      if (filled(t)) {
+        g.add(t);
+      } else {
+        copies.push_back(t.contiguous());
+        g.add(copies.back());
+      }
+    }
+    const int64_t count = static_cast<int64_t>(g.t.size());
+    Tensor norm = at::empty({}, g.t[0].options().dtype(at::kFloat));
+    Tensor scratch = scratch_of(rqf_grad_norm_scratch_bytes(count), norm);
+    check(rqf_global_grad_norm(g.ptr.data(), g.numel.data(), g.dtype.data(), count, norm.data_ptr<float>(),
+                               data(scratch), stream_on(norm)),
+          "rqf_global_grad_norm");
+    return wrap(norm);
+  });
+}
+
+// clip_grads(grads, max_norm, out) -> norm
+PyObject *clip_grads(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (!arity(n, 3, "clip_grads")) return nullptr;
+  return guarded([&]() -> PyObject * {
+    const double max_norm = PyFloat_AsDouble(a[1]);
+    if (PyErr_Occurred()) throw python_error();
+    TORCH_CHECK_VALUE(max_norm >= 0.0, "max_norm must not be negative, got ", std::to_string(max_norm));
+    List g = list_arg(a[0], "grads");
+    const bool in_place = a[2] == Py_None;
+    List out;
+    if (!in_place) {
+      out = list_arg(a[2], "out");
+      TORCH_CHECK_VALUE(out.t.size() == g.t.size(), std::to_string(g.t.size()), " gradients and ",
+                        std::to_string(out.t.size()), " outputs");
+    }
+    if (g.t.empty()) return wrap(at::zeros({}));
+    const c10::cuda::CUDAGuard device(g.t[0].device());
+    std::vector<Tensor> copies;
+    std::vector<std::pair<Tensor, Tensor>> back;
+    std::vector<void *> to;
+    to.reserve(g.t.size());
+    for (size_t i = 0; i < g.t.size(); ++i) {
+      const Tensor &t = g.t[i];
+      const Tensor &o = in_place ? t : out.t[i];
+      TORCH_CHECK_VALUE(in_place || (o.sizes() == t.sizes() && o.scalar_type() == t.scalar_type()), "out ",
+                        o.scalar_type(), " ", text(o.sizes()), " does not match ", t.scalar_type(), " ",
+                        text(t.sizes()));
+      TORCH_CHECK(in_place || o.get_device() == t.get_device(), "tensors on different devices: ", t.device(), " and ",
+                  o.device());
+      if (filled(o) && (in_place || (t.is_contiguous() && o.is_contiguous()) || t.strides() == o.strides())) {
+        g.add(t);
+        to.push_back(o.data_ptr());
+        continue;
+      }
+      // what does not lie in memory as its output does goes through a dense copy
+      copies.push_back(t.clone(at::MemoryFormat::Contiguous));
+      g.add(copies.back());
+      to.push_back(copies.back().data_ptr());
+      back.emplace_back(o, copies.back());
+    }
+    if (in_place) {
+      std::vector<void *> seen;
+      for (size_t i = 0; i < g.ptr.size(); ++i)
+        if (g.numel[i]) seen.push_back(g.ptr[i]);
+      std::sort(seen.begin(), seen.end());
+      TORCH_CHECK_VALUE(std::adjacent_find(seen.begin(), seen.end()) == seen.end(),
+                        "a tensor stands in grads twice: it would be scaled twice");
+    }
+    const int64_t count = static_cast<int64_t>(g.t.size());
+    Tensor norm = at::empty({}, g.t[0].options().dtype(at::kFloat));
+    Tensor scratch = scratch_of(rqf_grad_norm_scratch_bytes(count), norm);
+    check(rqf_clip_grads(g.ptr.data(), to.data(), g.numel.data(), g.dtype.data(), count,
+                         static_cast<float>(max_norm), norm.data_ptr<float>(), data(scratch), stream_on(norm)),
+          "rqf_clip_grads");
+    for (const Tensor &o : in_place ? g.t : out.t) written(o);
+    for (auto &[o, c] : back) o.copy_(c);
+    return wrap(norm);
+  });
+}
+
+PyObject *set_error(PyObject *, PyObject *type) {
+  Py_INCREF(type);
+  Py_XSETREF(g_error, type);
+  Py_RETURN_NONE;
+}
+
+#define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
+PyMethodDef g_methods[] = {
+    FAST(delta_forward), FAST(delta_backward), FAST(delta_step), FAST(grad_norm), FAST(clip_grads),
+    {"set_error", set_error, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
+PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__native() {
+  g_error = PyExc_RuntimeError;
+  Py_INCREF(g_error);
+  return PyModule_Create(&g_module);
+}
