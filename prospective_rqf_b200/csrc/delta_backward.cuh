@@ -14,11 +14,13 @@
 //   dq = scale e^G X1 + E k
 //   dk = e^{G_C-G} X2 - beta e^G X3 + F k + E^T q + F^T k
 //   dbeta_i = dr_i.v_i - e^{G_i} k_i.X3_i + sum_j D_ij dA_ij k_i.k_j
-//   dg_t = sum_{i>=t} (in_i - out_i) + sum out + e^{G_C} <S, dS'>
+//   dg_t = sum_{i>=t>j} M_ij + sum_{i>=t} in_i + sum_{j<t} out_j + e^{G_C} <S, dS'>
 //
-// with in_i what token i takes of its past, out_i what it leaves for later:
-// in = q.(scale e^G X1) - k.(beta e^G X3) + rows of (E qk + F kk), out =
-// k.(e^{G_C-G} X2) + the same's columns.
+// a sum over all that crosses the gate between t - 1 and t: M = E (q k^T) + F (k k^T)
+// inside the chunk, in = q.(scale e^G X1) - k.(beta e^G X3) from before it to a token,
+// out = k.(e^{G_C-G} X2) from a token past its end.  (Differences of row and column sums
+// give the same with cancellation: 4e-7 from 64 bits in a CPU model against 1.3e-7, and not
+// 0 where a gate is closed.)
 #pragma once
 
 #include "delta_scan.cuh"
@@ -90,8 +92,7 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
       copy_wait<1>();
       __syncwarp();
       Tile::get(tile, mine, lane, x);
-      row_max(x, m0, m1);
-      save_max(a.maxes, first + n, kMaxDO, a.vp / 16, w, m0, m1, lane);
+      save_token_max(a.token_maxes, first + n, kTokenDO, a.vp / 16, w, x, lane);
       Scale x0, x1;
       {
         float y[8][4];
@@ -115,7 +116,7 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
       }
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt) {
-        const float2 f = *reinterpret_cast<const float2 *>(vec + kRowU * kC + nt * 8 + 2 * c);
+        const float2 f = *reinterpret_cast<const float2 *>(vec + kRowEC * kC + nt * 8 + 2 * c);
         const float2 t = *reinterpret_cast<const float2 *>(vec + kRowT * kC + nt * 8 + 2 * c);
         du[nt][0] = t.x * (x0.inv * du[nt][0] + f.x * (s0.inv * dr[nt][0]));
         du[nt][1] = t.y * (x0.inv * du[nt][1] + f.y * (s0.inv * dr[nt][1]));
@@ -132,19 +133,28 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
       }
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt) {
-        const float2 be = *reinterpret_cast<const float2 *>(vec + kRowBeta * kC + nt * 8 + 2 * c);
-        dr[nt][0] *= x0.inv;
-        dr[nt][1] *= x0.inv;
-        dr[nt][2] *= x1.inv;
-        dr[nt][3] *= x1.inv;
-        du[nt][0] = be.x * dr[nt][0];
-        du[nt][1] = be.y * dr[nt][1];
-        du[nt][2] = be.x * dr[nt][2];
-        du[nt][3] = be.y * dr[nt][3];
+        const float2 t = *reinterpret_cast<const float2 *>(vec + kRowT * kC + nt * 8 + 2 * c);
+        const float2 f = *reinterpret_cast<const float2 *>(vec + kRowK * kC + nt * 8 + 2 * c);
+        const float tx = inverse_pow2(t.x), ty = inverse_pow2(t.y);
+        dr[nt][0] = fmaf(x0.inv, dr[nt][0], tx * du[nt][0]);
+        dr[nt][1] = fmaf(x0.inv, dr[nt][1], ty * du[nt][1]);
+        dr[nt][2] = fmaf(x1.inv, dr[nt][2], tx * du[nt][2]);
+        dr[nt][3] = fmaf(x1.inv, dr[nt][3], ty * du[nt][3]);
+        du[nt][0] = f.x * dr[nt][0];
+        du[nt][1] = f.y * dr[nt][1];
+        du[nt][2] = f.x * dr[nt][2];
+        du[nt][3] = f.y * dr[nt][3];
       }
-      row_max(dr, m0, m1);
-      save_rows(a.drs + ((first + n) * a.vp + v0) * kC, lane, dr);
-      save_max(a.maxes, first + n, kMaxDR, a.vp / 16, w, m0, m1, lane);
+      save_rows(a.drs + ((first + n) * a.vp + v0) * kC, lane, du);  // dr with the keys' factors
+      save_token_max(a.token_maxes, first + n, kTokenDR, a.vp / 16, w, du, lane);
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt) {
+        const float2 be = *reinterpret_cast<const float2 *>(vec + kRowBeta * kC + nt * 8 + 2 * c);
+        du[nt][0] *= be.x;
+        du[nt][1] *= be.y;
+        du[nt][2] *= be.x;
+        du[nt][3] *= be.y;
+      }
       __syncwarp();
       Tile::put(mine, lane, du);
       __syncwarp();
@@ -218,13 +228,36 @@ struct Grad {
   static constexpr int kS = kDO + NP * kC * kVB * 2;               // [v][KD] hi, lo
   static constexpr int kDS = kS + 2 * kVB * KD * 2;
   static constexpr int kFloats = kDS + 2 * kVB * KD * 2;
-  static constexpr int kBytes = kFloats + 16 * kC * 4 + kC * 8;
+  static constexpr int kBytes = kFloats + 16 * kC * 4 + kC * 8 + kTokenMaxes * kC * 4;
   // after the products over V: E and F as halves in the place of u and dr, the second half of
   // dk in the place of S and dS'
   static constexpr int kE = kU, kF = kDR, kDK = kS;
 };
 
-// A 32-bit tile [rows][LD] from global memory as scaled halves hi, lo.
+// A 32-bit tile [v][token] as halves hi, lo, each token's column under its own scale.
+__device__ __forceinline__ void split_tokens(unsigned char *hi_tile, unsigned char *lo_tile, const float *src,
+                                             int rows, const float *inv, int tid) {
+  const int p = tid & 7;
+  float mul[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) mul[j] = inverse_pow2(inv[p * 8 + j]);
+#pragma unroll 2
+  for (int row = tid >> 3; row < kVB; row += kGradThreads / 8) {
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = 0.f;
+    if (row < rows) load8<float>(src + row * kC + p * 8, x);
+    uint4 hi, lo;
+    split2(x[0] * mul[0], x[1] * mul[1], hi.x, lo.x);
+    split2(x[2] * mul[2], x[3] * mul[3], hi.y, lo.y);
+    split2(x[4] * mul[4], x[5] * mul[5], hi.z, lo.z);
+    split2(x[6] * mul[6], x[7] * mul[7], hi.w, lo.w);
+    *reinterpret_cast<uint4 *>(hi_tile + 2 * tile_at<kC>(row, p)) = hi;
+    *reinterpret_cast<uint4 *>(lo_tile + 2 * tile_at<kC>(row, p)) = lo;
+  }
+}
+
+// A 32-bit tile [rows][LD] from global memory as halves hi, lo under one scale.
 template <int LD>
 __device__ __forceinline__ void split_tile(unsigned char *hi_tile, unsigned char *lo_tile,
                                            const float *src, int rows, int live, float mul, int tid) {
@@ -322,6 +355,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) gradient_kernel(const Args a)
   const uint32_t base = smem_u32(smem);
   float *sums = reinterpret_cast<float *>(smem + L::kFloats);  // [16][64]
   double *G = reinterpret_cast<double *>(sums + 16 * kC);
+  float *u_inv = reinterpret_cast<float *>(G + kC), *dr_inv = u_inv + kC, *do_inv = dr_inv + kC;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const bool first_half = warp < 4;
   const int row = (warp & 3) * 16;
@@ -364,6 +398,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) gradient_kernel(const Args a)
     sc[i] = scale_for(x);
   }
 
+  if (tid < kTokenMaxes * kC) {
+    const float *m = a.token_maxes + (chunk * kTokenMaxes + tid / kC) * (a.vp / 16) * kC + tid % kC;
+    float x = 0.f;
+    for (int j = 0; j < a.vp / 16; ++j) x = fmaxf(x, m[j * kC]);
+    u_inv[tid] = scale_for(x).inv;
+  }
+  __syncthreads();
+
   float xa[KD / 8][4], xb[KD / 8][4], d[8][4];  // X1 or X3; X2; dP or dA
   zero(xa);
   zero(xb);
@@ -373,10 +415,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) gradient_kernel(const Args a)
   for (int v0 = 0; v0 < a.vp; v0 += kVB) {
     const int rows = min(kVB, a.vp - v0);
     if (v0 > 0) __syncthreads();
-    split_tile<kC>(smem + L::kU, smem + L::kU + kVB * kC * 2, a.us + (chunk * a.vp + v0) * kC, kVB, rows,
-                   sc[kMaxU].mul, tid);
-    split_tile<kC>(smem + L::kDR, smem + L::kDR + kVB * kC * 2, a.drs + (chunk * a.vp + v0) * kC, kVB,
-                   rows, sc[kMaxDR].mul, tid);
+    split_tokens(smem + L::kU, smem + L::kU + kVB * kC * 2, a.us + (chunk * a.vp + v0) * kC, rows, u_inv, tid);
+    split_tokens(smem + L::kDR, smem + L::kDR + kVB * kC * 2, a.drs + (chunk * a.vp + v0) * kC, rows, dr_inv,
+                 tid);
     const float *S = a.states + (chunk * a.vp + v0) * KD, *dS = a.dstates + (chunk * a.vp + v0) * KD;
     split_tile<KD>(smem + L::kS, smem + L::kS + kVB * KD * 2, S, kVB, rows, sc[kMaxS].mul, tid);
     split_tile<KD>(smem + L::kDS, smem + L::kDS + kVB * KD * 2, dS, kVB, rows, sc[kMaxDS].mul, tid);
@@ -394,7 +435,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) gradient_kernel(const Args a)
         for (int j = 0; j < 8; ++j) x[j] = 0.f;
         if (t < live && v0 + p * 8 < a.vdim)
           load8<E>(dout + (long long)t * a.hv * a.vdim + p * 8, x);
-        const float mul = sc[kMaxDO].mul;
+        const float mul = inverse_pow2(do_inv[t]);
         uint4 hi, lo;
         split2(x[0] * mul, x[1] * mul, hi.x, lo.x);
         split2(x[2] * mul, x[3] * mul, hi.y, lo.y);
@@ -445,7 +486,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) gradient_kernel(const Args a)
     }
   }
   // E, F, their products with the keys' and queries' grams, and the sums of those
-  const float scale_x = first_half ? sc[kMaxDO].inv : sc[kMaxDR].inv;
+  const float *left_inv = first_half ? do_inv : dr_inv;
+  const float x_inv0 = left_inv[row + g], x_inv1 = left_inv[row + g + 8];
   float gram[8][4];
   zero(gram);
   {
@@ -472,37 +514,53 @@ __global__ void __launch_bounds__(kGradThreads, 1) gradient_kernel(const Args a)
   }
   const float *kfac = a.kfac + kv_chunk * kC, *qfac = a.qfac + kv_chunk * kC;
   const float *lfac = first_half ? qfac : kfac;
-  float row_sum[2] = {0.f, 0.f}, beta_sum[2] = {0.f, 0.f}, emax = 0.f;
-  const float mul_d = first_half ? sc[kMaxDO].inv * sc[kMaxU].inv : -sc[kMaxDR].inv * sc[kMaxU].inv;
+  float before[2] = {0.f, 0.f}, beta_sum[2] = {0.f, 0.f}, emax = 0.f;
+  const float mul_d0 = first_half ? x_inv0 : -x_inv0, mul_d1 = first_half ? x_inv1 : -x_inv1;
 #pragma unroll
   for (int nt = 0; nt < 8; ++nt) {
-    float col[2] = {0.f, 0.f};
+    float m[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int i = row + g + (e >> 1) * 8, j = nt * 8 + 2 * c + (e & 1);
       const bool in = first_half ? i >= j : i > j;
       const float dec = in ? expf((float)(G[i] - G[j])) : 0.f;
-      const float x = in ? mul_d * d[nt][e] * dec : 0.f;       // D dP or D dA
+      const float x = in ? u_inv[j] * ((e >> 1 ? mul_d1 : mul_d0) * d[nt][e]) * dec : 0.f;  // D dP or D dA
       const float gr = kfac[j] * (lfac[i] * gram[nt][e]);
       const float lead = first_half ? a.scale : vec[kRowBeta * kC + i];
       d[nt][e] = lead * x;                                     // E or F
-      const float m = in ? d[nt][e] * gr : 0.f;
+      m[e] = in ? d[nt][e] * gr : 0.f;
       if (!first_half && in) beta_sum[e >> 1] = fmaf(x, gr, beta_sum[e >> 1]);
-      row_sum[e >> 1] += m;
-      col[e & 1] += m;
       emax = fmaxf(emax, fabsf(lfac[i] * d[nt][e]));
+    }
+    // for both rows the sum of M over the columns before each of this thread's
+    float cross[2] = {0.f, 0.f};
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const float pair = m[2 * half] + m[2 * half + 1];
+      float run = pair;
+#pragma unroll
+      for (int s = 1; s < 4; s <<= 1) {
+        const float up = __shfl_up_sync(0xffffffffu, run, s, 4);
+        if (c >= s) run += up;
+      }
+      const float lead = before[half] + (run - pair);
+      const int t = nt * 8 + 2 * c;
+      before[half] += __shfl_sync(0xffffffffu, run, 3, 4);
+      const int i = row + g + 8 * half;
+      if (i >= t) cross[0] += lead;
+      if (i >= t + 1) cross[1] += lead + m[2 * half];
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float x = col[e];
+      float x = cross[e];
       x += __shfl_xor_sync(0xffffffffu, x, 4);
       x += __shfl_xor_sync(0xffffffffu, x, 8);
       x += __shfl_xor_sync(0xffffffffu, x, 16);
-      if (g == 0) sums[warp * kC + nt * 8 + 2 * c + e] = x;  // columns: [warp][64]
+      if (g == 0) sums[warp * kC + nt * 8 + 2 * c + e] = x;  // [warp][64]
     }
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i) row_sum[i] = quad_sum(row_sum[i]), beta_sum[i] = quad_sum(beta_sum[i]);
+  for (int i = 0; i < 2; ++i) beta_sum[i] = quad_sum(beta_sum[i]);
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) emax = fmaxf(emax, __shfl_xor_sync(0xffffffffu, emax, s));
   float *per_warp = sums + 15 * kC;  // scalars
@@ -532,22 +590,22 @@ __global__ void __launch_bounds__(kGradThreads, 1) gradient_kernel(const Args a)
   }
   // X's true values and what they give for the decays
   {
-    const float mul_x = scale_x * sc[kMaxS].inv;
+    const float s_inv = sc[kMaxS].inv;
     const float e0 = vec[kRowEG * kC + row + g], e1 = vec[kRowEG * kC + row + g + 8];
     const float b0 = vec[kRowBeta * kC + row + g], b1 = vec[kRowBeta * kC + row + g + 8];
-    const float f0 = mul_x * (first_half ? a.scale * e0 : -e0), f1 = mul_x * (first_half ? a.scale * e1 : -e1);
+    const float f0 = x_inv0 * (first_half ? a.scale * e0 : -e0), f1 = x_inv1 * (first_half ? a.scale * e1 : -e1);
 #pragma unroll
     for (int nt = 0; nt < KD / 8; ++nt) {
-      xa[nt][0] *= f0;
-      xa[nt][1] *= f0;
-      xa[nt][2] *= f1;
-      xa[nt][3] *= f1;
+      xa[nt][0] = f0 * (s_inv * xa[nt][0]);
+      xa[nt][1] = f0 * (s_inv * xa[nt][1]);
+      xa[nt][2] = f1 * (s_inv * xa[nt][2]);
+      xa[nt][3] = f1 * (s_inv * xa[nt][3]);
     }
     float d0, d1;
     dot_rows<KD, NP>(xa, smem + (first_half ? L::kQ : L::kK), row, lane, d0, d1);
     d0 *= lfac[row + g], d1 *= lfac[row + g + 8];
     if (!first_half) {
-      rv0 = quad_sum(rv0) * sc[kMaxDR].inv, rv1 = quad_sum(rv1) * sc[kMaxDR].inv;
+      rv0 = quad_sum(rv0) * x_inv0, rv1 = quad_sum(rv1) * x_inv1;
       if (c == 0) {
         const long long at = gb + (long long)(row + g) * a.hv;
         if (row + g < here) a.dbeta[at] = row + g < live ? rv0 + d0 + beta_sum[0] : 0.f;
@@ -564,16 +622,17 @@ __global__ void __launch_bounds__(kGradThreads, 1) gradient_kernel(const Args a)
       }
     }
     float *in = sums + (first_half ? 8 : 9) * kC;
-    if (c == 0) in[row + g] = d0 + row_sum[0], in[row + g + 8] = d1 + row_sum[1];
+    if (c == 0) in[row + g] = d0, in[row + g + 8] = d1;
     if (first_half) {
-      const float mul_u = sc[kMaxU].inv * sc[kMaxDS].inv;
-      const float u0 = mul_u * vec[kRowEC * kC + row + g], u1 = mul_u * vec[kRowEC * kC + row + g + 8];
+      const float ds_inv = sc[kMaxDS].inv;
+      const float u0 = u_inv[row + g] * vec[kRowEC * kC + row + g];
+      const float u1 = u_inv[row + g + 8] * vec[kRowEC * kC + row + g + 8];
 #pragma unroll
       for (int nt = 0; nt < KD / 8; ++nt) {
-        xb[nt][0] *= u0;
-        xb[nt][1] *= u0;
-        xb[nt][2] *= u1;
-        xb[nt][3] *= u1;
+        xb[nt][0] = u0 * (ds_inv * xb[nt][0]);
+        xb[nt][1] = u0 * (ds_inv * xb[nt][1]);
+        xb[nt][2] = u1 * (ds_inv * xb[nt][2]);
+        xb[nt][3] = u1 * (ds_inv * xb[nt][3]);
       }
       dot_rows<KD, NP>(xb, smem + L::kK, row, lane, d0, d1);
       if (c == 0) {
@@ -669,38 +728,39 @@ __global__ void __launch_bounds__(kGradThreads, 1) gradient_kernel(const Args a)
     }
     store_grad_rows<E, KD>(a, a.dk, dk_part, b, h, t0, row, here, lane, xb);
   } else if (warp == 4) {
-    // dg: suffix sums over the chunk
-    double diff[2], out = 0.0;
+    // dg: a suffix sum of what comes in, a prefix sum of what goes out
+    double in[2], out[2], here_[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int t = 2 * lane + i;
-      float cs = 0.f;
+      float cross = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        // warps above a column's block hold nothing of it but zeros
-        cs += sums[j * kC + t];
-      }
-      diff[i] = (double)sums[8 * kC + t] + sums[9 * kC + t] - sums[10 * kC + t] - cs;
-      out += sums[10 * kC + t];
+      for (int j = 0; j < 8; ++j) cross += sums[j * kC + t];
+      here_[i] = cross;
+      in[i] = (double)sums[8 * kC + t] + sums[9 * kC + t];
+      out[i] = sums[10 * kC + t];
     }
-    double run = diff[0] + diff[1];
+    double after = in[0] + in[1], upto = out[0] + out[1];
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
-      const double up = __shfl_down_sync(0xffffffffu, run, s);
-      if (lane + s < 32) run += up;
+      const double down = __shfl_down_sync(0xffffffffu, after, s);
+      const double up = __shfl_up_sync(0xffffffffu, upto, s);
+      if (lane + s < 32) after += down;
+      if (lane >= s) upto += up;
     }
+    // after: in of this lane's tokens and all later ones; upto: out of all tokens before the lane's
+    upto = __shfl_up_sync(0xffffffffu, upto, 1);
+    if (lane == 0) upto = 0.0;
+    const double later = __shfl_down_sync(0xffffffffu, after, 1);
+    double through = 0.0;
 #pragma unroll
-    for (int s = 16; s > 0; s >>= 1) out += __shfl_xor_sync(0xffffffffu, out, s);
-    double bs = 0.0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) bs += per_warp[8 + i];
-    out += (double)vec[kRowEG * kC + kC - 1] * bs;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int t = 2 * lane + i;
-      if (t < here)
-        a.dg[gb + (long long)t * a.hv] = t < live ? (float)(run - (i ? diff[0] : 0.0) + out) : 0.f;
-    }
+    for (int i = 0; i < 8; ++i) through += per_warp[8 + i];
+    through *= (double)vec[kRowEG * kC + kC - 1];
+    const double first = here_[0] + after + upto + through;
+    const double second = here_[1] + (in[1] + (lane < 31 ? later : 0.0)) + (upto + out[0]) + through;
+    const int t = 2 * lane;
+    if (t < here) a.dg[gb + (long long)t * a.hv] = t < live ? (float)first : 0.f;
+    if (t + 1 < here) a.dg[gb + (long long)(t + 1) * a.hv] = t + 1 < live ? (float)second : 0.f;
   }
 }
 

@@ -23,6 +23,13 @@
 // 32-bit input two more.  Splitting into bf16 parts instead keeps 16 bits of
 // the 22 and measured 4e-6 to 8e-6 from 64 bits in a CPU model of these
 // formulas, against 2e-7 for this split.
+//
+// Sizes of keys.  k_i = kfac_i k^_i, kfac_i the power of two of its row's scale.
+// What token i puts into the state is k^_i (kfac_i u_i), so the kernels carry
+// kfac u and kfac r, in which tokens of small and large keys stand as they
+// count, with A^_ij = beta_i kfac_i^2 e^{G_i-G_j} k^_i.k^_j in A's place.  And
+// T = I + T': r itself is added in 32 bits, so that a token whose key is tiny
+// still has its own u to 32 bits for the gradient of that key.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -34,19 +41,20 @@ namespace rqf {
 namespace delta {
 
 constexpr int kC = 64;       // tokens of a chunk
-constexpr int kVec = 8;      // coefficient rows kept for a chunk (enum Row)
+constexpr int kVec = 9;      // coefficient rows kept for a chunk (enum Row)
 constexpr float kMinDecay = -200.f;  // e^-200 is 0 in 32 bits: -inf gates are taken as this
 
 // Coefficient rows of a chunk, 64 floats each.
 enum Row {
-  kRowKS = 0,    // beta e^G kfac: the factor of k S in r
-  kRowBeta = 1,  // beta
+  kRowKS = 0,    // beta kfac^2 e^G: the factor of k S in r
+  kRowV = 1,     // beta kfac: the factor of v in r
   kRowT = 2,     // 2^t, the scale of T's row
   kRowP = 3,     // 2^p, the scale of P's row
   kRowO = 4,     // scale e^G qfac: the factor of q S in o
-  kRowU = 5,     // e^{G_C-G} kfac: the factor of u in the state
-  kRowEG = 6,    // e^G
-  kRowEC = 7     // e^{G_C-G}
+  kRowEG = 5,    // e^G
+  kRowEC = 6,    // e^{G_C-G}
+  kRowBeta = 7,  // beta
+  kRowK = 8      // kfac
 };
 
 template <typename E>
@@ -115,6 +123,11 @@ __device__ __forceinline__ Scale scale_for(float m) {
 // operand so far below its sums loses nothing that they could hold.
 __device__ __forceinline__ Scale scale_beside(float m, float sums) {
   return scale_for(fmaxf(m, sums * 0x1p-16f));
+}
+
+// 1 / x of a power of two.
+__device__ __forceinline__ float inverse_pow2(float x) {
+  return __uint_as_float((254u << 23) - __float_as_uint(x));
 }
 
 // Two scaled values as halves, and what the halves leave out as halves again.
@@ -280,7 +293,7 @@ struct Args {
   __half *khat, *qhat, *tmat, *pmat;
   float *kfac, *qfac, *vec;
   double *gsum;
-  float *states, *us, *dstates, *drs, *maxes;
+  float *states, *us, *dstates, *drs, *maxes, *token_maxes;
   float *dq_part, *dk_part;  // (B, T, Hv, K) when key heads are shared
 };
 

@@ -1,5 +1,5 @@
 // The part of a chunk that needs no state: the scaled halves of q and k, the
-// decays, T = (I + A)^{-1} and P.  One CTA for a chunk of a value head, all
+// decays, T' = (I + A)^{-1} - I and P, both for the scaled keys.  One CTA for a chunk of a value head, all
 // chunks at once.
 //
 // A and P are one 64 x 64 x K product each on the tensor cores, from exact
@@ -211,8 +211,8 @@ __global__ void __launch_bounds__(kPrepThreads) prep_kernel(const Args a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int i = warp * 16 + g + (e >> 1) * 8, j = nt * 8 + 2 * c + (e & 1);
-      const float d = i >= j ? expf((float)(G[i] - G[j])) * kfac[j] : 0.f;
-      A[i * kLdA + j] = i > j ? beta[i] * d * kfac[i] * kk[nt][e] : 0.f;
+      const float d = i >= j ? expf((float)(G[i] - G[j])) : 0.f;
+      A[i * kLdA + j] = i > j ? beta[i] * (kfac[i] * (kfac[i] * (d * kk[nt][e]))) : 0.f;
       qk[nt][e] = i >= j ? a.scale * d * qfac[i] * qk[nt][e] : 0.f;
       m[e >> 1] = fmaxf(m[e >> 1], fabsf(qk[nt][e]));
     }
@@ -268,7 +268,10 @@ __global__ void __launch_bounds__(kPrepThreads) prep_kernel(const Args a) {
     const int row = tid >> 1, from = (tid & 1) * 32;
     float mx = 0.f;
 #pragma unroll 8
-    for (int j = 0; j < 32; ++j) mx = fmaxf(mx, fabsf(T[row * kLdA + from + j]));
+    for (int j = 0; j < 32; ++j) {
+      if (from + j == row) T[row * kLdA + row] = 0.f;  // I apart
+      mx = fmaxf(mx, fabsf(T[row * kLdA + from + j]));
+    }
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     const Scale s = scale_for(mx);
     __half *out = a.tmat + chunk * 2 * kC * kC + row * kC;
@@ -278,10 +281,11 @@ __global__ void __launch_bounds__(kPrepThreads) prep_kernel(const Args a) {
   if (tid < kC) {
     const double last = G[kC - 1];
     const float eg = expf((float)G[tid]), ec = expf((float)(last - G[tid]));
-    vec[kRowKS * kC + tid] = beta[tid] * eg * kfac[tid];
+    vec[kRowKS * kC + tid] = beta[tid] * (kfac[tid] * (kfac[tid] * eg));
+    vec[kRowV * kC + tid] = beta[tid] * kfac[tid];
     vec[kRowBeta * kC + tid] = beta[tid];
+    vec[kRowK * kC + tid] = kfac[tid];
     vec[kRowO * kC + tid] = a.scale * eg * qfac[tid];
-    vec[kRowU * kC + tid] = ec * kfac[tid];
     vec[kRowEG * kC + tid] = eg;
     vec[kRowEC * kC + tid] = ec;
     if (a.gsum != nullptr) a.gsum[chunk * kC + tid] = G[tid];

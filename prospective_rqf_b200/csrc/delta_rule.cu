@@ -80,6 +80,7 @@ size_t carve_context(void *buffer, const Sizes &s, bool save, Args *a) {
     c.take(a->states, (size_t)s.bhn * s.vp * s.kd);
     c.take(a->us, (size_t)s.bhn * s.vp * kC);
     c.take(a->maxes, (size_t)s.bhn * kMaxes * (s.vp / 16));
+    c.take(a->token_maxes, (size_t)s.bhn * kTokenMaxes * (s.vp / 16) * kC);
   }
   return c.used;
 }

@@ -4,7 +4,7 @@
 // never meet, so warps share only the chunk's tiles (k, q, T, P), and each
 // product's sums are laid out as the next one's left operand needs them:
 //
-//   (kS)^T = S^T k^T  ->  r^T  ->  u^T = r^T T^T  ->  o^T, S'^T += u^T k
+//   (kS)^T = S^T k^T  ->  r^T  ->  u^T = r^T + r^T T'^T  ->  o^T, S'^T += u^T k
 //
 // runs with no trip through shared memory.  That is why these products use
 // m16n8k16 and not tcgen05: the chain from one chunk to the next is three
@@ -208,8 +208,10 @@ __device__ __forceinline__ void save_rows(float *dst, int lane, const float (&x)
   }
 }
 
-// Where the backward's last pass finds the largest magnitudes, for its scales.
-enum Max { kMaxS = 0, kMaxU, kMaxDS, kMaxDR, kMaxDO, kMaxes };
+// Where the backward's last pass finds the largest magnitudes, for its scales: of S and dS'
+// one for each warp's columns of V, of u, dr and do one for each of them and each token.
+enum Max { kMaxS = 0, kMaxDS, kMaxes };
+enum TokenMax { kTokenU = 0, kTokenDR, kTokenDO, kTokenMaxes };
 __device__ __forceinline__ void save_max(float *maxes, long long chunk, int which, int warps, int w,
                                          float m0, float m1, int lane) {
   float m = fmaxf(m0, m1);
@@ -217,6 +219,29 @@ __device__ __forceinline__ void save_max(float *maxes, long long chunk, int whic
   m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
   m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
   if (lane == 0) maxes[(chunk * kMaxes + which) * warps + w] = m;
+}
+
+__device__ __forceinline__ void save_token_max(float *maxes, long long chunk, int which, int warps, int w,
+                                               const float (&x)[8][4], int lane) {
+  // over the 16 rows: each exchange halves the tokens that a lane still has
+  float m[8][2];
+#pragma unroll
+  for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) m[nt][e] = fmaxf(fabsf(x[nt][e]), fabsf(x[nt][e + 2]));
+#pragma unroll
+  for (int half = 4; half > 0; half >>= 1) {
+    const bool up = lane & (half * 4);
+#pragma unroll
+    for (int nt = 0; nt < half; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float give = up ? m[nt][e] : m[nt + half][e], keep = up ? m[nt + half][e] : m[nt][e];
+        m[nt][e] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, give, half * 4));
+      }
+  }
+  float *to = maxes + ((chunk * kTokenMaxes + which) * warps + w) * kC;
+  *reinterpret_cast<float2 *>(to + 2 * lane) = make_float2(m[0][0], m[0][1]);
 }
 
 template <typename E, int KD, int W, bool SAVE>
@@ -290,7 +315,7 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt) {
           const float2 f = *reinterpret_cast<const float2 *>(vec + kRowKS * kC + nt * 8 + 2 * c);
-          const float2 be = *reinterpret_cast<const float2 *>(vec + kRowBeta * kC + nt * 8 + 2 * c);
+          const float2 be = *reinterpret_cast<const float2 *>(vec + kRowV * kC + nt * 8 + 2 * c);
           r[nt][0] = be.x * x[nt][0] - f.x * (s0.inv * r[nt][0]);
           r[nt][1] = be.y * x[nt][1] - f.y * (s0.inv * r[nt][1]);
           r[nt][2] = be.x * x[nt][2] - f.x * (s1.inv * r[nt][2]);
@@ -310,16 +335,25 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt) {
         const float2 f = *reinterpret_cast<const float2 *>(vec + kRowT * kC + nt * 8 + 2 * c);
-        u[nt][0] *= f.x * x0.inv;
-        u[nt][1] *= f.y * x0.inv;
-        u[nt][2] *= f.x * x1.inv;
-        u[nt][3] *= f.y * x1.inv;
+        u[nt][0] = fmaf(f.x * x0.inv, u[nt][0], r[nt][0]);
+        u[nt][1] = fmaf(f.y * x0.inv, u[nt][1], r[nt][1]);
+        u[nt][2] = fmaf(f.x * x1.inv, u[nt][2], r[nt][2]);
+        u[nt][3] = fmaf(f.y * x1.inv, u[nt][3], r[nt][3]);
+      }
+      if (SAVE) {  // u without the keys' factors
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt) {
+          const float2 f = *reinterpret_cast<const float2 *>(vec + kRowK * kC + nt * 8 + 2 * c);
+          const float fx = inverse_pow2(f.x), fy = inverse_pow2(f.y);
+          r[nt][0] = fx * u[nt][0];
+          r[nt][1] = fy * u[nt][1];
+          r[nt][2] = fx * u[nt][2];
+          r[nt][3] = fy * u[nt][3];
+        }
+        save_rows(a.us + ((first + n) * a.vp + v0) * kC, lane, r);
+        save_token_max(a.token_maxes, first + n, kTokenU, a.vp / 16, w, r, lane);
       }
       row_max(u, m0, m1);
-      if (SAVE) {
-        save_rows(a.us + ((first + n) * a.vp + v0) * kC, lane, u);
-        save_max(a.maxes, first + n, kMaxU, a.vp / 16, w, m0, m1, lane);
-      }
       x0 = scale_for(m0), x1 = scale_for(m1);
       zero(y);
 #pragma unroll
@@ -348,7 +382,7 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
       const float gam = vec[kRowEG * kC + kC - 1];
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt) {
-        const float2 f = *reinterpret_cast<const float2 *>(vec + kRowU * kC + nt * 8 + 2 * c);
+        const float2 f = *reinterpret_cast<const float2 *>(vec + kRowEC * kC + nt * 8 + 2 * c);
         u[nt][0] *= f.x;
         u[nt][1] *= f.y;
         u[nt][2] *= f.x;
