@@ -278,24 +278,11 @@ __device__ __forceinline__ void split_tile(unsigned char *hi_tile, unsigned char
   }
 }
 
-// acc += A (AP parts, fragments given) times columns of a tile in BP parts.
+// acc += A (AP parts, fragments given) times columns of a tile in BP parts, ordered as step_cols.
 template <int LD, int AP, int BP, int NT>
 __device__ __forceinline__ void cols_step(float (&acc)[NT][4], const uint32_t (&a)[AP][4],
-                                          uint32_t tile, uint32_t part, int k0, int n0, int lane) {
-#pragma unroll
-  for (int np = 0; np < NT / 2; ++np) {
-#pragma unroll
-    for (int p = 0; p < BP; ++p) {
-      uint32_t f[4];
-      ldsm4t(b_cols<LD>(tile + p * part, k0, n0 + np * 16, lane), f);
-      mma(acc[2 * np], a[0], f[0], f[1]);
-      mma(acc[2 * np + 1], a[0], f[2], f[3]);
-      if (AP == 2 && p == 0) {
-        mma(acc[2 * np], a[AP - 1], f[0], f[1]);
-        mma(acc[2 * np + 1], a[AP - 1], f[2], f[3]);
-      }
-    }
-  }
+                                          uint32_t tile, uint32_t part, int ks, int lane) {
+  step_cols<LD, AP, BP>(acc, a[0], a[AP - 1], tile, part, ks, NT, lane);
 }
 
 // Two rows' dot products of a 16 x KD accumulator with rows of a half tile in NP parts.
@@ -458,9 +445,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) gradient_kernel(const Args a)
           ldsm4(a_rows<kVB>(base + L::kDO + p * kC * kVB * 2, row, ks * 16, lane), fo[p]);
 #pragma unroll
         for (int p = 0; p < 2; ++p) ldsm4t(a_cols<kC>(base + L::kU + p * kSquare, ks * 16, row, lane), fu[p]);
-        cols_step<KD, NP, 2>(xa, fo, base + L::kS, kWide, ks * 16, 0, lane);
-        cols_step<KD, 2, 2>(xb, fu, base + L::kDS, kWide, ks * 16, 0, lane);
-        cols_step<kC, NP, 2>(d, fo, base + L::kU, kSquare, ks * 16, 0, lane);
+        cols_step<KD, NP, 2>(xa, fo, base + L::kS, kWide, ks, lane);
+        cols_step<KD, 2, 2>(xb, fu, base + L::kDS, kWide, ks, lane);
+        cols_step<kC, NP, 2>(d, fo, base + L::kU, kSquare, ks, lane);
       }
     } else {
       const E *v = static_cast<const E *>(a.v) + b * a.sv.b + t0 * a.sv.t + h * a.sv.h + v0;
@@ -470,8 +457,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) gradient_kernel(const Args a)
 #pragma unroll
         for (int p = 0; p < 2; ++p)
           ldsm4t(a_cols<kC>(base + L::kDR + p * kSquare, ks * 16, row, lane), fr[p]);
-        cols_step<KD, 2, 2>(xa, fr, base + L::kS, kWide, ks * 16, 0, lane);
-        cols_step<kC, 2, 2>(d, fr, base + L::kU, kSquare, ks * 16, 0, lane);
+        cols_step<KD, 2, 2>(xa, fr, base + L::kS, kWide, ks, lane);
+        cols_step<kC, 2, 2>(d, fr, base + L::kU, kSquare, ks, lane);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int t = row + g + (i & 1) * 8, col = ks * 16 + 2 * c + (i >> 1) * 8;
@@ -667,7 +654,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) gradient_kernel(const Args a)
       if (ks * 16 > row) continue;
       uint32_t fd[2][4];
       split_frag(d, ks, s0.mul, s1.mul, fd[0], fd[1]);
-      cols_step<KD, 2, NP>(xa, fd, base + L::kK, kC * KD * 2, ks * 16, 0, lane);
+      cols_step<KD, 2, NP>(xa, fd, base + L::kK, kC * KD * 2, ks, lane);
     }
 #pragma unroll
     for (int nt = 0; nt < KD / 8; ++nt) {
@@ -691,7 +678,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) gradient_kernel(const Args a)
       uint32_t fd[2][4];
 #pragma unroll
       for (int p = 0; p < 2; ++p) ldsm4t(a_cols<kC>(base + L::kE + p * kC * kC * 2, ks * 16, row, lane), fd[p]);
-      cols_step<KD, 2, NP>(y, fd, base + L::kQ, kC * KD * 2, ks * 16, 0, lane);
+      cols_step<KD, 2, NP>(y, fd, base + L::kQ, kC * KD * 2, ks, lane);
     }
 #pragma unroll
     for (int nt = 0; nt < KD / 8; ++nt)
@@ -704,7 +691,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) gradient_kernel(const Args a)
       uint32_t fd[2][4];
 #pragma unroll
       for (int p = 0; p < 2; ++p) ldsm4t(a_cols<kC>(base + L::kF + p * kC * kC * 2, ks * 16, row, lane), fd[p]);
-      cols_step<KD, 2, NP>(y, fd, base + L::kK, kC * KD * 2, ks * 16, 0, lane);
+      cols_step<KD, 2, NP>(y, fd, base + L::kK, kC * KD * 2, ks, lane);
     }
     float2 *to = reinterpret_cast<float2 *>(smem + L::kDK) + (warp - 4) * (KD / 8) * 2 * 32 + lane;
 #pragma unroll

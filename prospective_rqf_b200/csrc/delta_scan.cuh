@@ -118,47 +118,78 @@ struct WarpTile {
   }
 };
 
-// acc (16 x 64) += A (hi + lo, 16 x 16 of the contraction at ks) times a tile stored [n][k].
+// acc (16 x 8 NT) += A (hi + lo, 16 x 16 of the contraction at ks) times a tile stored [n][k]
+// in NP parts, from pair `from` of 8-column tiles on.  All products of one part come before the
+// next part's, so that no two in a row sum into the same registers: with one warp to a scheduler
+// a product that waits for the one before it costs its whole latency.
 template <int LD, int NP, int NT>
 __device__ __forceinline__ void step_rows(float (&acc)[NT][4], const uint32_t (&hi)[4],
                                           const uint32_t (&lo)[4], uint32_t tile, uint32_t part,
                                           int ks, int from, int lane) {
+  uint32_t b[NT / 2][4];
 #pragma unroll
-  for (int np = 0; np < NT / 2; ++np) {
-    if (np < from) continue;
-    uint32_t b[4];
-    ldsm4(b_rows<LD>(tile, np * 16, ks * 16, lane), b);
-    mma(acc[2 * np], hi, b[0], b[1]);
-    mma(acc[2 * np + 1], hi, b[2], b[3]);
-    mma(acc[2 * np], lo, b[0], b[1]);
-    mma(acc[2 * np + 1], lo, b[2], b[3]);
-    if (NP == 2) {
-      ldsm4(b_rows<LD>(tile + part, np * 16, ks * 16, lane), b);
-      mma(acc[2 * np], hi, b[0], b[1]);
-      mma(acc[2 * np + 1], hi, b[2], b[3]);
+  for (int np = 0; np < NT / 2; ++np)
+    if (np >= from) ldsm4(b_rows<LD>(tile, np * 16, ks * 16, lane), b[np]);
+#pragma unroll
+  for (int np = 0; np < NT / 2; ++np)
+    if (np >= from) {
+      mma(acc[2 * np], hi, b[np][0], b[np][1]);
+      mma(acc[2 * np + 1], hi, b[np][2], b[np][3]);
     }
+#pragma unroll
+  for (int np = 0; np < NT / 2; ++np)
+    if (np >= from) {
+      mma(acc[2 * np], lo, b[np][0], b[np][1]);
+      mma(acc[2 * np + 1], lo, b[np][2], b[np][3]);
+    }
+  if (NP == 2) {
+#pragma unroll
+    for (int np = 0; np < NT / 2; ++np)
+      if (np >= from) ldsm4(b_rows<LD>(tile + part, np * 16, ks * 16, lane), b[np]);
+#pragma unroll
+    for (int np = 0; np < NT / 2; ++np)
+      if (np >= from) {
+        mma(acc[2 * np], hi, b[np][0], b[np][1]);
+        mma(acc[2 * np + 1], hi, b[np][2], b[np][3]);
+      }
   }
 }
-// The same with a tile stored [k][n], and columns up to `to` pairs.
+// The same with a tile stored [k][n], A in AP parts, and pairs up to `to`.
 template <int LD, int AP, int NP, int NT>
 __device__ __forceinline__ void step_cols(float (&acc)[NT][4], const uint32_t (&hi)[4],
                                           const uint32_t (&lo)[4], uint32_t tile, uint32_t part,
                                           int ks, int to, int lane) {
+  constexpr int kAt = NT / 2 < 4 ? NT / 2 : 4;  // pairs at a time
 #pragma unroll
-  for (int np = 0; np < NT / 2; ++np) {
-    if (np > to) continue;
-    uint32_t b[4];
-    ldsm4t(b_cols<LD>(tile, ks * 16, np * 16, lane), b);
-    mma(acc[2 * np], hi, b[0], b[1]);
-    mma(acc[2 * np + 1], hi, b[2], b[3]);
+  for (int n0 = 0; n0 < NT / 2; n0 += kAt) {
+    uint32_t b[kAt][4];
+#pragma unroll
+    for (int i = 0; i < kAt; ++i)
+      if (n0 + i <= to) ldsm4t(b_cols<LD>(tile, ks * 16, (n0 + i) * 16, lane), b[i]);
+#pragma unroll
+    for (int i = 0; i < kAt; ++i)
+      if (n0 + i <= to) {
+        mma(acc[2 * (n0 + i)], hi, b[i][0], b[i][1]);
+        mma(acc[2 * (n0 + i) + 1], hi, b[i][2], b[i][3]);
+      }
     if (AP == 2) {
-      mma(acc[2 * np], lo, b[0], b[1]);
-      mma(acc[2 * np + 1], lo, b[2], b[3]);
+#pragma unroll
+      for (int i = 0; i < kAt; ++i)
+        if (n0 + i <= to) {
+          mma(acc[2 * (n0 + i)], lo, b[i][0], b[i][1]);
+          mma(acc[2 * (n0 + i) + 1], lo, b[i][2], b[i][3]);
+        }
     }
     if (NP == 2) {
-      ldsm4t(b_cols<LD>(tile + part, ks * 16, np * 16, lane), b);
-      mma(acc[2 * np], hi, b[0], b[1]);
-      mma(acc[2 * np + 1], hi, b[2], b[3]);
+#pragma unroll
+      for (int i = 0; i < kAt; ++i)
+        if (n0 + i <= to) ldsm4t(b_cols<LD>(tile + part, ks * 16, (n0 + i) * 16, lane), b[i]);
+#pragma unroll
+      for (int i = 0; i < kAt; ++i)
+        if (n0 + i <= to) {
+          mma(acc[2 * (n0 + i)], hi, b[i][0], b[i][1]);
+          mma(acc[2 * (n0 + i) + 1], hi, b[i][2], b[i][3]);
+        }
     }
   }
 }

@@ -7,9 +7,9 @@
 // from eight at a time on, into one partial sum for each CTA; the second adds
 // those up in their order (every CTA the same) and scales.  No atomics: the
 // same gradients give the same norm bit for bit.  Both are bound by memory:
-// one read for the norm, one read and one write for the clipping, which goes
-// through the tiles from the last to the first, so that it finds what the
-// first launch read last in L2.
+// one read for the norm, one read and one write for the clipping.  A CTA has a
+// run of tiles; the second launch goes through it from the last to the first,
+// so that it finds what the first read last in L2.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -81,8 +81,9 @@ __device__ __forceinline__ void load_vec(const E *p, long long i0, long long n, 
 
 // Squares of one vector.  In 32 bits; where those leave their range, in 64.
 template <typename E>
-__device__ __forceinline__ double squares(const E (&x)[16 / sizeof(E)]) {
+__device__ __forceinline__ double squares(const uint4 &v) {
   constexpr int kPer = 16 / sizeof(E);
+  const E *x = reinterpret_cast<const E *>(&v);
   float s = 0.f;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
@@ -98,23 +99,41 @@ __device__ __forceinline__ double squares(const E (&x)[16 / sizeof(E)]) {
   }
   return d;
 }
+__device__ __forceinline__ double squares(const uint4 &v, int type) {
+  return type == kF32 ? squares<float>(v) : type == kBF16 ? squares<__nv_bfloat16>(v) : squares<__half>(v);
+}
 
-template <typename E>
-__device__ __forceinline__ double tile_squares(const Entry &e, int tile) {
-  constexpr int kPer = 16 / sizeof(E);
-  const E *p = static_cast<const E *>(e.src);
-  const int off = (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(E));  // elements past a boundary
-  const long long first = (long long)(tile - e.tile) * (kTileBytes / sizeof(E)) - off;
-  E x[kVecs][kPer];
+// This thread's vectors of one tile, as the bytes stand from the 16-byte
+// boundary at or before the tensor's start; zeros before it and past its end.
+__device__ __forceinline__ void load_tile(const Entry &e, int tile, uint4 (&x)[kVecs]) {
+  const int size = e.type == kF32 ? 4 : 2;
+  const char *p = static_cast<const char *>(e.src);
+  const int off = (int)(reinterpret_cast<uintptr_t>(p) & 15);
+  const long long first = (long long)(tile - e.tile) * kTileBytes - off, bytes = e.n * size;
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
-    const long long i0 = first + (threadIdx.x + i * kThreads) * kPer;
-    load_vec<E>(p, i0, e.n, i0 >= 0 && i0 + kPer <= e.n, x[i]);
-  }
-  double s = 0.0;
+    const long long at = first + (threadIdx.x + i * kThreads) * 16;
+    if (at >= 0 && at + 16 <= bytes) {
+      x[i] = *reinterpret_cast<const uint4 *>(p + at);
+    } else {
+      uint32_t w[4] = {0, 0, 0, 0};
+      if (size == 4) {
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i) s += squares<E>(x[i]);
-  return s;
+        for (int j = 0; j < 4; ++j) {
+          const long long b = at + 4 * j;
+          if (b >= 0 && b < bytes) w[j] = *reinterpret_cast<const uint32_t *>(p + b);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const long long b = at + 2 * j;
+          if (b >= 0 && b < bytes)
+            w[j >> 1] |= (uint32_t)*reinterpret_cast<const unsigned short *>(p + b) << (16 * (j & 1));
+        }
+      }
+      x[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
 }
 
 // dst = c src on one tile, in vectors that are aligned at the destination.
@@ -147,6 +166,14 @@ __device__ __forceinline__ void tile_scale(const Entry &e, int tile, float c) {
   }
 }
 
+// The tiles of this CTA: a run of them, so that the table is searched once.
+struct Range {
+  int from, to;
+};
+__device__ __forceinline__ Range my_tiles(int tiles) {
+  return {(int)((long long)tiles * blockIdx.x / gridDim.x), (int)((long long)tiles * (blockIdx.x + 1) / gridDim.x)};
+}
+
 __device__ __forceinline__ double block_sum(double s) {
   __shared__ double red[kThreads / 32];
 #pragma unroll
@@ -162,12 +189,22 @@ __device__ __forceinline__ double block_sum(double s) {
 template <int N>
 __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant__ Table<N> t,
                                                            double *partials) {
+  const Range r = my_tiles(t.tiles);
+  int at = find(t, r.from);
   double s = 0.0;
-  for (int tile = blockIdx.x; tile < t.tiles; tile += gridDim.x) {
-    const Entry &e = t.e[find(t, tile)];
-    s += e.type == kF32    ? tile_squares<float>(e, tile)
-         : e.type == kBF16 ? tile_squares<__nv_bfloat16>(e, tile)
-                           : tile_squares<__half>(e, tile);
+  uint4 x[kVecs], y[kVecs];
+  load_tile(t.e[at], r.from, x);
+  for (int tile = r.from; tile < r.to; ++tile) {
+    const int type = t.e[at].type;
+    if (tile + 1 < r.to) {  // the next tile's loads before this one's sums
+      if (at + 1 < t.count && t.e[at + 1].tile <= tile + 1) ++at;
+      load_tile(t.e[at], tile + 1, y);
+    }
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      s += squares(x[i], type);
+      x[i] = y[i];
+    }
   }
   s = block_sum(s);
   if (threadIdx.x == 0) partials[blockIdx.x] = s;
@@ -192,9 +229,11 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ 
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm = total;
   float c = max_norm / (total + 1e-6f);
   c = c > 1.f ? 1.f : c;  // NaN stays
-  for (int i = blockIdx.x; i < t.tiles; i += gridDim.x) {
-    const int tile = t.tiles - 1 - i;
-    const Entry &e = t.e[find(t, tile)];
+  const Range r = my_tiles(t.tiles);
+  int at = find(t, r.to - 1);
+  for (int tile = r.to - 1; tile >= r.from; --tile) {
+    if (t.e[at].tile > tile) --at;
+    const Entry &e = t.e[at];
     if (c == 1.f && e.src == e.dst) continue;
     if (e.type == kF32) tile_scale<float>(e, tile, c);
     else if (e.type == kBF16) tile_scale<__nv_bfloat16>(e, tile, c);

@@ -2117,6 +2117,20 @@ int rqf_two_tap_coefficients_backward(const float *log_theta, const float *log_g
 }  // extern "C"
 
 // ------------------------------------------------ gated delta rule, one token
+namespace {
+template <typename E>
+int delta_step_launch(const delta_step::Args &a, int64_t heads, cudaStream_t st) {
+  const unsigned grid = (unsigned)(heads * ceil_div(a.vdim, delta_step::kCols));
+  if (a.kdim <= 32)
+    delta_step::step_kernel<E, 2><<<grid, delta_step::kThreads, 0, st>>>(a);
+  else if (a.kdim <= 64)
+    delta_step::step_kernel<E, 4><<<grid, delta_step::kThreads, 0, st>>>(a);
+  else
+    delta_step::step_kernel<E, 8><<<grid, delta_step::kThreads, 0, st>>>(a);
+  return launch_status();
+}
+}  // namespace
+
 extern "C" {
 
 int rqf_gated_delta_step(const rqf_delta_problem *problem, const void *q, const void *k,
@@ -2135,9 +2149,8 @@ int rqf_gated_delta_step(const rqf_delta_problem *problem, const void *q, const 
   if (!slots && p->batch > pool) return RQF_ERR_SHAPE;
   if (!q || !k || !v || !log_decay || !beta || !o || (pool > 0 && !state)) return RQF_ERR_ARGUMENT;
   if (!aligned(state, 16)) return RQF_ERR_ALIGN;
-  const double grid = (double)p->batch * (double)p->value_heads *
-                      (double)ceil_div(p->value_dim, delta_step::kCols);
-  if (grid > (double)0x7fffffffLL) return RQF_ERR_SHAPE;
+  const double heads = (double)p->batch * (double)p->value_heads;
+  if (heads * (double)ceil_div(p->value_dim, delta_step::kCols) > (double)0x7fffffffLL) return RQF_ERR_SHAPE;
   delta_step::Args a;
   a.q = q, a.k = k, a.v = v, a.g = log_decay, a.beta = beta;
   a.qb = p->q_stride[0], a.qh = p->q_stride[2], a.kb = p->k_stride[0], a.kh = p->k_stride[2];
@@ -2146,15 +2159,10 @@ int rqf_gated_delta_step(const rqf_delta_problem *problem, const void *q, const 
   a.slots = slots, a.slots_64 = slots_64, a.state = state, a.o = o, a.scale = p->scale;
   a.hv = (int)p->value_heads, a.rep = (int)(p->value_heads / p->key_heads);
   a.kdim = (int)p->key_dim, a.vdim = (int)p->value_dim, a.pool = pool;
-  const unsigned blocks = (unsigned)grid;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (p->dtype == RQF_F32)
-    delta_step::step_kernel<float><<<blocks, delta_step::kThreads, 0, st>>>(a);
-  else if (p->dtype == RQF_BF16)
-    delta_step::step_kernel<__nv_bfloat16><<<blocks, delta_step::kThreads, 0, st>>>(a);
-  else
-    delta_step::step_kernel<__half><<<blocks, delta_step::kThreads, 0, st>>>(a);
-  return launch_status();
+  if (p->dtype == RQF_F32) return delta_step_launch<float>(a, p->batch * p->value_heads, st);
+  if (p->dtype == RQF_BF16) return delta_step_launch<__nv_bfloat16>(a, p->batch * p->value_heads, st);
+  return delta_step_launch<__half>(a, p->batch * p->value_heads, st);
 }
 
 }  // extern "C"
