@@ -274,8 +274,8 @@ struct Strides {
 };
 
 // One call's tensors and sizes.  n_chunks covers `time`; a row's own length
-// ends it earlier.  State-like buffers are [row][chunk][v][KD] and
-// [row][chunk][v][64], v padded to VP, a multiple of 16.
+// ends it earlier.  u and dr are [row][chunk][v][64], v padded to VP, a multiple
+// of 16.
 struct Args {
   const void *q, *k, *v, *dout;
   const float *g, *beta;
@@ -293,7 +293,8 @@ struct Args {
   __half *khat, *qhat, *tmat, *pmat;
   float *kfac, *qfac, *vec;
   double *gsum;
-  float *states, *us, *dstates, *drs, *maxes, *token_maxes;
+  __half *states, *dstates;  // [chunk][hi, lo][v][KD], rows scaled
+  float *scales, *us, *drs, *token_maxes;
   float *dq_part, *dk_part;  // (B, T, Hv, K) when key heads are shared
 };
 

@@ -239,18 +239,29 @@ __device__ __forceinline__ void save_rows(float *dst, int lane, const float (&x)
   }
 }
 
-// Where the backward's last pass finds the largest magnitudes, for its scales: of S and dS'
-// one for each warp's columns of V, of u, dr and do one for each of them and each token.
-enum Max { kMaxS = 0, kMaxDS, kMaxes };
-enum TokenMax { kTokenU = 0, kTokenDR, kTokenDO, kTokenMaxes };
-__device__ __forceinline__ void save_max(float *maxes, long long chunk, int which, int warps, int w,
-                                         float m0, float m1, int lane) {
-  float m = fmaxf(m0, m1);
-  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-  if (lane == 0) maxes[(chunk * kMaxes + which) * warps + w] = m;
+// What the backward's last pass finds of S and dS': the halves that the products took, and each
+// row's 1 / scale (next to nothing for a row of zeros, which so stands below all others).
+enum RowScale { kScaleS = 0, kScaleDS, kScales };
+__device__ __forceinline__ void save_scales(float *scales, long long chunk, int which, int vp, int v0,
+                                            float m0, float m1, int lane) {
+  float *to = scales + (chunk * kScales + which) * vp + v0 + (lane >> 2);
+  if ((lane & 3) == 0) {
+    to[0] = m0 == 0.f ? 0x1p-118f : scale_for(m0).inv;
+    to[8] = m1 == 0.f ? 0x1p-118f : scale_for(m1).inv;
+  }
 }
+template <int KD>
+__device__ __forceinline__ void save_frag(__half *hi_rows, long long plane, int ks, int lane,
+                                          const uint32_t (&hi)[4], const uint32_t (&lo)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    __half *to = hi_rows + ((lane >> 2) + (i & 1) * 8) * KD + ks * 16 + (i >> 1) * 8 + 2 * (lane & 3);
+    *reinterpret_cast<uint32_t *>(to) = hi[i];
+    *reinterpret_cast<uint32_t *>(to + plane) = lo[i];
+  }
+}
+// And of u, dr and do the largest magnitude of each token in each warp's columns.
+enum TokenMax { kTokenU = 0, kTokenDR, kTokenDO, kTokenMaxes };
 
 __device__ __forceinline__ void save_token_max(float *maxes, long long chunk, int which, int warps, int w,
                                                const float (&x)[8][4], int lane) {
@@ -324,10 +335,8 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
       row_max(S, m0, m1);
       const float big0 = m0, big1 = m1;
       const Scale s0 = scale_for(m0), s1 = scale_for(m1);
-      if (SAVE) {
-        save_rows(a.states + ((first + n) * a.vp + v0) * KD, lane, S);
-        save_max(a.maxes, first + n, kMaxS, a.vp / 16, w, m0, m1, lane);
-      }
+      if (SAVE) save_scales(a.scales, first + n, kScaleS, a.vp, v0, m0, m1, lane);
+      __half *keep = SAVE ? a.states + ((first + n) * 2 * a.vp + v0) * KD : nullptr;
       float r[8][4], qs[8][4];
       zero(r);
       zero(qs);
@@ -335,6 +344,7 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
       for (int ks = 0; ks < KD / 16; ++ks) {
         uint32_t hi[4], lo[4];
         split_frag(S, ks, s0.mul, s1.mul, hi, lo);
+        if (SAVE) save_frag<KD>(keep, (long long)a.vp * KD, ks, lane, hi, lo);
         step_rows<KD, NP>(r, hi, lo, st + St::kK, kC * KD * 2, ks, 0, lane);
         step_rows<KD, NP>(qs, hi, lo, st + St::kQ, kC * KD * 2, ks, 0, lane);
       }
