@@ -3,28 +3,25 @@
 // The first runs from the last chunk to the first with the state's cotangent
 // dS' (16 columns of V to a warp, as the forward holds the state):
 //
-//   du = P^T do + e^{G_C-G} k dS',   dr = T^T du,   dv = beta dr
+//   du = P^T do + e^{G_C-G} k dS',   dr = du + T'^T diag(beta) du,   dv = beta dr
 //   dS = e^{G_C} dS' + (scale e^G q)^T do - (beta e^G k)^T dr
 //
-// and keeps dS' and dr.  The second takes all chunks at once, with S, u from
-// the forward and dS', dr from the first:
+// and keeps dS', dr and v.dv.  The second takes all chunks at once, with S, w
+// from the forward and dS', dr from the first (u = beta w):
 //
 //   dP = do u^T,  dA = -dr u^T,  X1 = do S^T,  X2 = u dS'^T,  X3 = dr S^T,
 //   E = scale D dP,  F = beta D dA  (D_ij = e^{G_i-G_j}, lower triangles)
 //   dq = scale e^G X1 + E k
 //   dk = e^{G_C-G} X2 - beta e^G X3 + F k + E^T q + F^T k
-//   dbeta_i = dr_i.u_i / beta_i
-//   dg_t = sum_{i>=t>j} M_ij + sum_{i>=t} in_i + sum_{j<t} out_j + e^{G_C} <S, dS'>
+//   dbeta = dr.w
+//   dg_t = <S, dS> - sum_{i<t} (q_i.dq_i - v_i.dv_i)
 //
-// a sum over all that crosses the gate between t - 1 and t: M = E (q k^T) + F (k k^T)
-// inside the chunk, in = q.(scale e^G X1) - k.(beta e^G X3) from before it to a token,
-// out = k.(e^{G_C-G} X2) from a token past its end.  (Differences of row and column sums
-// give the same with cancellation: 4e-7 from 64 bits in a CPU model against 1.3e-7, and not
-// 0 where a gate is closed.)
-//
-// dbeta: r = beta (v - e^G k S) and (I + A) u = r, so that dr_i.(v_i - e^{G_i} k_i S) and
-// sum_j dA_ij A_ij / beta_i add up to dr_i.u_i / beta_i.  Where beta is (next to) 0 the two
-// are taken as they stand.
+// dS the cotangent of the state that enters the chunk.  The last line: with D_t
+// = a_t S_{t-1}, dg_t = <D_t, dD_t>; dD_t = dS_t - k_t dr_t^T and S_t = D_t +
+// k_t u_t^T give <D_t, dD_t> = <S_t, dS_t> - v_t.dv_t, and dS_t has scale q_t
+// do_t^T besides a_{t+1} dD_{t+1}, so that <S_t, dS_t> = dg_{t+1} + o_t.do_t,
+// where o_t.do_t = q_t.dq_t.  No product of chunk by chunk is needed for it, and
+// the sum runs over one chunk at most.
 #pragma once
 
 #include "delta_scan.cuh"
@@ -49,9 +46,11 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
   const long long len = row_length(a, b);
   const int chunks = (int)((len + kC - 1) / kC);
   const long long kv_first = ((long long)b * a.hk + hk) * a.n_chunks, first = bh * a.n_chunks;
+  const long long slot = bh * (a.n_chunks + 1);
   const uint32_t base = smem_u32(smem);
   unsigned char *mine = smem + 2 * St::kBytes + warp * kC * 16 * sizeof(E);
   const uint32_t tile = smem_u32(mine);
+  const E *v = static_cast<const E *>(a.v) + b * a.sv.b + h * a.sv.h + v0;
   const long long so = (long long)a.hv * a.vdim;  // do and dv are dense
   const long long at = ((long long)b * a.time * a.hv + h) * a.vdim + v0;
   const E *dout = static_cast<const E *>(a.dout) + at;
@@ -84,8 +83,8 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
       row_max(S, m0, m1);
       const float big0 = m0, big1 = m1;
       const Scale s0 = scale_for(m0), s1 = scale_for(m1);
-      save_scales(a.scales, first + n, kScaleDS, a.vp, v0, m0, m1, lane);
-      __half *keep = a.dstates + ((first + n) * 2 * a.vp + v0) * KD;
+      save_scales(a.dscales + (slot + n + 1) * a.vp + v0, m0, m1, lane);
+      __half *keep = a.dstates + ((slot + n + 1) * 2 * a.vp + v0) * KD;
       float du[8][4], dr[8][4], x[8][4];
       zero(dr);  // k dS' first
 #pragma unroll
@@ -97,6 +96,9 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
       copy_wait<1>();
       __syncwarp();
       Tile::get(tile, mine, lane, x);
+      __syncwarp();  // v takes the place of do
+      Tile::load(tile, v + t0 * a.sv.t, a.sv.t, (int)min((long long)kC, len - t0), cols, lane);
+      copy_commit();
       save_token_max(a.token_maxes, first + n, kTokenDO, a.vp / 16, w, x, lane);
       Scale x0, x1;
       {
@@ -122,29 +124,39 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt) {
         const float2 f = *reinterpret_cast<const float2 *>(vec + kRowEC * kC + nt * 8 + 2 * c);
-        const float2 t = *reinterpret_cast<const float2 *>(vec + kRowT * kC + nt * 8 + 2 * c);
-        du[nt][0] = t.x * (x0.inv * du[nt][0] + f.x * (s0.inv * dr[nt][0]));
-        du[nt][1] = t.y * (x0.inv * du[nt][1] + f.y * (s0.inv * dr[nt][1]));
-        du[nt][2] = t.x * (x1.inv * du[nt][2] + f.x * (s1.inv * dr[nt][2]));
-        du[nt][3] = t.y * (x1.inv * du[nt][3] + f.y * (s1.inv * dr[nt][3]));
+        du[nt][0] = x0.inv * du[nt][0] + f.x * (s0.inv * dr[nt][0]);
+        du[nt][1] = x0.inv * du[nt][1] + f.y * (s0.inv * dr[nt][1]);
+        du[nt][2] = x1.inv * du[nt][2] + f.x * (s1.inv * dr[nt][2]);
+        du[nt][3] = x1.inv * du[nt][3] + f.y * (s1.inv * dr[nt][3]);
       }
-      row_max(du, m0, m1);
-      x0 = scale_for(m0), x1 = scale_for(m1);
-      zero(dr);
+      {
+        float y[8][4];
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        split_frag(du, ks, x0.mul, x1.mul, hi, lo);
-        step_cols<kC, 2, 2>(dr, hi, lo, st + St::kT, kC * kC * 2, ks, ks, lane);
+        for (int nt = 0; nt < 8; ++nt) {
+          const float2 t = *reinterpret_cast<const float2 *>(vec + kRowT * kC + nt * 8 + 2 * c);
+          const float2 be = *reinterpret_cast<const float2 *>(vec + kRowBeta * kC + nt * 8 + 2 * c);
+          const float fx = t.x * be.x, fy = t.y * be.y;
+          y[nt][0] = fx * du[nt][0];
+          y[nt][1] = fy * du[nt][1];
+          y[nt][2] = fx * du[nt][2];
+          y[nt][3] = fy * du[nt][3];
+        }
+        row_max(y, m0, m1);
+        x0 = scale_for(m0), x1 = scale_for(m1);
+        zero(dr);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          split_frag(y, ks, x0.mul, x1.mul, hi, lo);
+          step_cols<kC, 2, 2>(dr, hi, lo, st + St::kT, kC * kC * 2, ks, ks, lane);
+        }
       }
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt) {
-        const float2 t = *reinterpret_cast<const float2 *>(vec + kRowT * kC + nt * 8 + 2 * c);
         const float2 f = *reinterpret_cast<const float2 *>(vec + kRowK * kC + nt * 8 + 2 * c);
-        const float tx = inverse_pow2(t.x), ty = inverse_pow2(t.y);
-        dr[nt][0] = fmaf(x0.inv, dr[nt][0], tx * du[nt][0]);
-        dr[nt][1] = fmaf(x0.inv, dr[nt][1], ty * du[nt][1]);
-        dr[nt][2] = fmaf(x1.inv, dr[nt][2], tx * du[nt][2]);
-        dr[nt][3] = fmaf(x1.inv, dr[nt][3], ty * du[nt][3]);
+        dr[nt][0] = fmaf(x0.inv, dr[nt][0], du[nt][0]);
+        dr[nt][1] = fmaf(x0.inv, dr[nt][1], du[nt][1]);
+        dr[nt][2] = fmaf(x1.inv, dr[nt][2], du[nt][2]);
+        dr[nt][3] = fmaf(x1.inv, dr[nt][3], du[nt][3]);
         du[nt][0] = f.x * dr[nt][0];
         du[nt][1] = f.y * dr[nt][1];
         du[nt][2] = f.x * dr[nt][2];
@@ -160,6 +172,17 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
         du[nt][2] *= be.x;
         du[nt][3] *= be.y;
       }
+      copy_wait<0>();
+      __syncwarp();
+      {
+        float y[8][4], m[8][2];
+        Tile::get(tile, mine, lane, y);
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) m[nt][e] = fmaf(y[nt][e], du[nt][e], y[nt][e + 2] * du[nt][e + 2]);
+        save_tokens<true>(a.vdv + ((first + n) * (a.vp / 16) + w) * kC, m, lane);
+      }
       __syncwarp();
       Tile::put(mine, lane, du);
       __syncwarp();
@@ -173,14 +196,16 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
       for (int nt = 0; nt < 8; ++nt) {
         const float2 p = *reinterpret_cast<const float2 *>(vec + kRowO * kC + nt * 8 + 2 * c);
         const float2 k = *reinterpret_cast<const float2 *>(vec + kRowKS * kC + nt * 8 + 2 * c);
+        const float2 be = *reinterpret_cast<const float2 *>(vec + kRowBeta * kC + nt * 8 + 2 * c);
+        const float kx = -be.x * k.x, ky = -be.y * k.y;
         x[nt][0] *= p.x;
         x[nt][1] *= p.y;
         x[nt][2] *= p.x;
         x[nt][3] *= p.y;
-        dr[nt][0] *= -k.x;
-        dr[nt][1] *= -k.y;
-        dr[nt][2] *= -k.x;
-        dr[nt][3] *= -k.y;
+        dr[nt][0] *= kx;
+        dr[nt][1] *= ky;
+        dr[nt][2] *= kx;
+        dr[nt][3] *= ky;
       }
       float d0, d1;
       row_max(x, m0, m1);
@@ -212,6 +237,18 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
   }
   copy_wait<0>();
   if (!on) return;
+  if (chunks > 0) {  // the cotangent of the state that enters the first chunk
+    float m0, m1;
+    row_max(S, m0, m1);
+    const Scale s0 = scale_for(m0), s1 = scale_for(m1);
+    save_scales(a.dscales + slot * a.vp + v0, m0, m1, lane);
+#pragma unroll
+    for (int ks = 0; ks < KD / 16; ++ks) {
+      uint32_t hi[4], lo[4];
+      split_frag(S, ks, s0.mul, s1.mul, hi, lo);
+      save_frag<KD>(a.dstates + (slot * 2 * a.vp + v0) * KD, (long long)a.vp * KD, ks, lane, hi, lo);
+    }
+  }
   if (a.ds0 != nullptr)
     store_state<KD>(a.ds0 + bh * a.kdim * a.vdim, v0, a.kdim, a.vdim, lane, S);
   constexpr int kPer = 16 / sizeof(E), kPieces = 16 / kPer;
@@ -222,41 +259,33 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
 
 // ------------------------------------------------------------ all chunks at once
 
-constexpr float kTinyBeta = 1e-20f;
-
-template <int KD, int NP>
+template <typename E, int KD>
 struct Grad {
-  // At K = 128 sixteen warps of 128 registers, each with half the columns; else eight, and two
-  // CTAs to an SM.  With eight warps of 255 at K = 128 the kernel took 3.5 ms for 16000 chunks
-  // (two warps to a scheduler, waiting on shared memory most of the time).
+  static constexpr int NP = Elem<E>::kParts;
+  // Sixteen warps, each with half the columns of K, keep their sums in 128 registers: with eight
+  // of 255 registers two warps share a scheduler and wait on shared memory most of the time.
   static constexpr int kHalves = KD >= 64 ? 2 : 1;
   static constexpr int kThreads = 256 * kHalves;
-  static constexpr int kVB = KD == 128 ? 128 : 64;  // columns of V whose u, dr, do are there at a time
+  static constexpr int kVB = KD == 128 ? 128 : 64;  // columns of V whose w, dr, do are there at a time
   static constexpr int kKq = NP * kC * KD * 2;
   static constexpr int kK = 0, kQ = kKq;
-  static constexpr int kU = 2 * kKq, kDR = kU + 2 * kVB * kC * 2;  // [v][t] hi, lo
+  static constexpr int kW = 2 * kKq, kDR = kW + 2 * kVB * kC * 2;  // [v][t] hi, lo
   static constexpr int kDO = kDR + 2 * kVB * kC * 2;               // [t][v] parts
-  // a ring of 16 columns of V of S and dS': [v][KD] S hi, lo, dS' hi, lo
+  // a ring of 16 columns of V: S, dS and dS', hi and lo
   static constexpr int kRing = kDO + NP * kC * kVB * 2;
-  static constexpr int kTile = 16 * KD * 2, kStage = 4 * kTile;
-  static constexpr int kStages = NP == 2 && KD == 128 ? 3 : 4;
-  // after the products over V, from u's place on: E and F, each with the keys' factors (for the
-  // products along rows) and with their rows' factors (down the columns), as hi and lo; and F's
-  // part of dk
-  static constexpr int kEF = kU, kSquare = kC * kC * 2, kDK = kEF + 8 * kSquare;
+  static constexpr int kTile = 16 * KD * 2, kTiles = 6, kStage = kTiles * kTile;
+  static constexpr int kStages = NP == 2 && KD == 128 ? 2 : 4;
+  // after the products over V, from w's place on, hi and lo: E with the keys' factors, E with the
+  // queries', F with the keys' of its columns and of its rows; then F's part of dk
+  static constexpr int kSquare = kC * kC * 2;
+  static constexpr int kE = kW, kEq = kE + 2 * kSquare, kF = kEq + 2 * kSquare,
+                       kFk = kF + 2 * kSquare, kDK = kFk + 2 * kSquare;
   static constexpr int kEnd = kRing + kStages * kStage, kNeed = kDK + kC * KD * 4;
-  static constexpr int kFloats = kEnd > kNeed ? kEnd : kNeed;
-  static constexpr int kSums = 29;  // rows of 64 floats
-  static constexpr int kBytes = kFloats + kSums * kC * 4 + 2 * kVB * 2;
-};
-// Rows of sums: cross sums of each warp, then
-enum Sum {
-  kSumIn = 16,     // what tokens take of S, by role and half of the columns
-  kSumOut = 20,    // what they leave in S'
-  kSumRows = 22,   // M's row sums over the first half of the columns, by role
-  kSumG = 24,      // the gates' sums, hi and lo
-  kSumDiag = 26,   // dr_i.u_i
-  kSumSlow = 27    // the explicit form of dbeta without dr.v, by half of the columns
+  static constexpr int kCoef = kEnd > kNeed ? kEnd : kNeed;  // vec's rows, qfac
+  static constexpr int kFloats = kCoef + (kVec + 1) * kC * 4;
+  // rows of 64: q.dq by half, v.dv, w's scale with beta, gates' sums hi and lo; then the rows'
+  // scales of S, dS, dS'
+  static constexpr int kBytes = kFloats + 6 * kC * 4 + 3 * kVB * 4;
 };
 
 // A 32-bit tile [v][token] as halves hi, lo, each token's column under its own scale.
@@ -307,20 +336,25 @@ __device__ __forceinline__ void split_dout(unsigned char *tile, const E *src, lo
   }
 }
 
-// 16 columns of V of S and dS' into one stage of the ring.
-template <int KD, int NP>
-__device__ __forceinline__ void load_states(uint32_t stage, const Args &a, long long chunk, int v0, int tid) {
-  using L = Grad<KD, NP>;
-  const long long plane = (long long)a.vp * KD, at = chunk * 2 * plane + (long long)v0 * KD;
-  copy_tile<KD>(stage, a.states + at, 16, tid, L::kThreads);
-  copy_tile<KD>(stage + L::kTile, a.states + at + plane, 16, tid, L::kThreads);
-  copy_tile<KD>(stage + 2 * L::kTile, a.dstates + at, 16, tid, L::kThreads);
-  copy_tile<KD>(stage + 3 * L::kTile, a.dstates + at + plane, 16, tid, L::kThreads);
+// 16 columns of V of S, dS and dS' into one stage of the ring.
+template <typename E, int KD>
+__device__ __forceinline__ void load_states(uint32_t stage, const Args &a, long long chunk, long long slot, int v0,
+                                            int tid) {
+  using L = Grad<E, KD>;
+  const long long plane = (long long)a.vp * KD, at = (long long)v0 * KD;
+  const __half *S = a.states + chunk * 2 * plane + at, *dS = a.dstates + slot * 2 * plane + at;
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    copy_tile<KD>(stage + p * L::kTile, S + p * plane, 16, tid, L::kThreads);
+    copy_tile<KD>(stage + (2 + p) * L::kTile, dS + p * plane, 16, tid, L::kThreads);
+    copy_tile<KD>(stage + (4 + p) * L::kTile, dS + (2 + p) * plane, 16, tid, L::kThreads);
+  }
 }
 
 // A fragment with its contraction's columns times powers of two: f0 for 2c, 2c + 1, f1 for
 // eight on.  Exact, but for what a half's range drops of the smallest.
-__device__ __forceinline__ void scale_frag(const uint32_t (&a)[4], __half2 f0, __half2 f1, uint32_t (&to)[4]) {
+__device__ __forceinline__ void scale_frag(const uint32_t (&a)[4], float2 x0, float2 x1, uint32_t (&to)[4]) {
+  const __half2 f0 = __floats2half2_rn(x0.x, x0.y), f1 = __floats2half2_rn(x1.x, x1.y);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const __half2 x = __hmul2(*reinterpret_cast<const __half2 *>(&a[i]), i < 2 ? f0 : f1);
@@ -403,27 +437,26 @@ __device__ __forceinline__ void store_grad_rows(const Args &a, void *out, float 
   }
 }
 
-// Half the warps ("rows of do") have 16 rows each of X1, X2 and dP, and so dq and a part of dk;
-// the others 16 rows each of X3 and dA, and so the rest of dk.
+// Half the warps ("of do") have 16 rows each of X1, X2 and dP, and so dq and a part of dk; the
+// others 16 rows each of X3 and dA, and so the rest of dk.
 template <typename E, int KD>
-__global__ void __launch_bounds__(Grad<KD, Elem<E>::kParts>::kThreads, KD >= 64 ? 1 : 2)
-gradient_kernel(const Args a) {
-  constexpr int NP = Elem<E>::kParts;
-  using L = Grad<KD, NP>;
-  constexpr int H = L::kHalves, VB = L::kVB, kThreads = L::kThreads;
+__global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradient_kernel(const Args a) {
+  using L = Grad<E, KD>;
+  constexpr int NP = L::NP, H = L::kHalves, VB = L::kVB, kThreads = L::kThreads;
   constexpr int NX = KD / 8 / H, ND = 8 / H;  // accumulator tiles of X and of dP, dA
   extern __shared__ __align__(128) unsigned char smem[];
   const uint32_t base = smem_u32(smem);
-  float *sums = reinterpret_cast<float *>(smem + L::kFloats);
-  float *g_hi = sums + kSumG * kC, *g_lo = g_hi + kC;
-  __half *rho = reinterpret_cast<__half *>(sums + L::kSums * kC);  // [S, dS'][v]: each row's scale
-  __shared__ float u_inv[kTokenMaxes * kC], per_warp[2][kThreads / 32], both_sums[kThreads / 32];
-  float *dr_inv = u_inv + kTokenDR * kC, *do_inv = u_inv + kTokenDO * kC;
+  const float *vec = reinterpret_cast<const float *>(smem + L::kCoef), *qfac = vec + kVec * kC;
+  const float *kfac = vec + kRowK * kC, *beta = vec + kRowBeta * kC;
+  float *qdq = reinterpret_cast<float *>(smem + L::kFloats), *vdv = qdq + 2 * kC, *wb = vdv + kC;
+  float *g_hi = wb + kC, *g_lo = g_hi + kC, *rho = g_lo + kC;  // rho: [S, dS, dS'][v]
+  __shared__ float w_inv[kTokenMaxes * kC], per_warp[2][kThreads / 32], both_sums[kThreads / 32];
+  float *dr_inv = w_inv + kTokenDR * kC, *do_inv = w_inv + kTokenDO * kC;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const bool is_do = warp < 4 * H;
   const int rb = warp & 3, row = rb * 16, half = (warp >> 2) % H;
   const int xcol = half * (KD / H), dcol = half * (kC / H);  // this warp's first columns
-  const int dto = rb - half * (ND / 2);                      // its last pair of dP's or dA's, if any
+  const int dto = rb - half * (ND / 2);  // its last pair of columns of dP or dA: the diagonal's
   const int n = blockIdx.x % a.n_chunks;
   const long long bh = blockIdx.x / a.n_chunks;
   const int b = (int)(bh / a.hv), h = (int)(bh % a.hv), hk = h / a.rep;
@@ -446,79 +479,85 @@ gradient_kernel(const Args a) {
     return;
   }
   const long long chunk = bh * a.n_chunks + n, kv_chunk = ((long long)b * a.hk + hk) * a.n_chunks + n;
-  const float *vec = a.vec + chunk * kVec * kC;
+  const long long slot = bh * (a.n_chunks + 1) + n;
   copy_tile<KD>(base + L::kK, a.khat + kv_chunk * NP * kC * KD, NP * kC, tid, kThreads);
   copy_tile<KD>(base + L::kQ, a.qhat + kv_chunk * NP * kC * KD, NP * kC, tid, kThreads);
+  for (int i = tid; i < (kVec + 1) * kC / 4; i += kThreads)
+    copy16(base + L::kCoef + i * 16,
+           i < kVec * kC / 4 ? a.vec + chunk * kVec * kC + i * 4 : a.qfac + kv_chunk * kC + (i - kVec * kC / 4) * 4);
   copy_commit();
   const int steps = a.vp / 16;
 #pragma unroll
   for (int i = 0; i < L::kStages - 1; ++i) {
-    if (i < steps) load_states<KD, NP>(base + L::kRing + i * L::kStage, a, chunk, i * 16, tid);
+    if (i < steps) load_states<E, KD>(base + L::kRing + i * L::kStage, a, chunk, slot, i * 16, tid);
     copy_commit();
   }
-  if (tid < kC) {
-    const double x = a.gsum[chunk * kC + tid];
-    const float hi = (float)x;
-    g_hi[tid] = hi;
-    g_lo[tid] = (float)(x - hi);
-  }
-  // the largest row scales of S and dS', to which all rows' are taken
-  float big[kScales];
+  // the largest row scales of S, dS and dS', to which all rows' are taken
+  const float *row_scales[3] = {a.scales + chunk * a.vp, a.dscales + slot * a.vp, a.dscales + (slot + 1) * a.vp};
+  float big[3];
 #pragma unroll
-  for (int i = 0; i < kScales; ++i) {
-    const float *m = a.scales + (chunk * kScales + i) * a.vp;
+  for (int i = 0; i < 3; ++i) {
     float x = 0.f;
-    for (int j = lane; j < a.vp; j += 32) x = fmaxf(x, m[j]);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+    for (int j = lane; j < a.vp; j += 32) x = fmaxf(x, row_scales[i][j]);
     big[i] = x;
   }
   if (tid < kTokenMaxes * kC) {
     const float *m = a.token_maxes + (chunk * kTokenMaxes + tid / kC) * steps * kC + tid % kC;
     float x = 0.f;
+#pragma unroll 4
     for (int j = 0; j < steps; ++j) x = fmaxf(x, m[j * kC]);
-    u_inv[tid] = scale_for(x).inv;
+    w_inv[tid] = scale_for(x).inv;
+  } else if (tid < kTokenMaxes * kC + kC) {
+    const int t = tid - kTokenMaxes * kC;
+    const float2 x = a.gsum[chunk * kC + t];
+    g_hi[t] = x.x;
+    g_lo[t] = x.y;
+    const float *m = a.vdv + chunk * steps * kC + t;
+    float s = 0.f;
+#pragma unroll 4
+    for (int j = 0; j < steps; ++j) s += m[j * kC];
+    vdv[t] = s;
   }
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) big[i] = fmaxf(big[i], __shfl_xor_sync(0xffffffffu, big[i], d));
   __syncthreads();
 
   float xa[NX][4], xb[NX][4], d[ND][4];  // X1 or X3; X2; dP or dA
   zero(xa);
   zero(xb);
   zero(d);
-  float both = 0.f;  // <S, dS'>, this thread's part
+  float both = 0.f;  // <S, dS>, this thread's part
   for (int step = 0; step < steps; ++step) {
     const int v0 = step * 16, local = v0 % VB;
     if (local == 0) {
       if (v0 > 0) __syncthreads();
       const int rows = min(VB, a.vp - v0);
-      split_tokens<VB, kThreads>(smem + L::kU, smem + L::kU + VB * kC * 2, a.us + (chunk * a.vp + v0) * kC, rows,
-                                 u_inv, tid);
+      split_tokens<VB, kThreads>(smem + L::kW, smem + L::kW + VB * kC * 2, a.ws + (chunk * a.vp + v0) * kC, rows,
+                                 w_inv, tid);
       split_tokens<VB, kThreads>(smem + L::kDR, smem + L::kDR + VB * kC * 2, a.drs + (chunk * a.vp + v0) * kC,
                                  rows, dr_inv, tid);
       split_dout<E, VB, NP, kThreads>(smem + L::kDO, static_cast<const E *>(a.dout) + (gb * a.vdim + v0),
                                       (long long)a.hv * a.vdim, live, a.vdim - v0, do_inv, tid);
-      for (int i = tid; i < 2 * rows; i += kThreads) {
-        const int which = i / rows, r = i % rows;
-        rho[which * VB + r] = __float2half_rn(a.scales[(chunk * kScales + which) * a.vp + v0 + r] *
-                                              inverse_pow2(big[which]));
-      }
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (tid < rows) rho[i * VB + tid] = row_scales[i][v0 + tid] * inverse_pow2(big[i]);
     }
     copy_wait<L::kStages - 2>();
     __syncthreads();
     {
       const int next = step + L::kStages - 1;
       if (next < steps)
-        load_states<KD, NP>(base + L::kRing + next % L::kStages * L::kStage, a, chunk, next * 16, tid);
+        load_states<E, KD>(base + L::kRing + next % L::kStages * L::kStage, a, chunk, slot, next * 16, tid);
       copy_commit();
     }
-    const int slot = L::kRing + step % L::kStages * L::kStage;
-    const uint32_t st = base + slot;
-    constexpr uint32_t kSquare = VB * kC * 2;
-    const __half2 s0 = *reinterpret_cast<const __half2 *>(rho + local + 2 * c);
-    const __half2 s1 = *reinterpret_cast<const __half2 *>(rho + local + 2 * c + 8);
-    if (tid < 16 * KD / 8) {  // a piece of eight of <S, dS'>
+    const int stage = L::kRing + step % L::kStages * L::kStage;
+    const uint32_t st = base + stage;
+    constexpr uint32_t kWide = VB * kC * 2;
+    if (tid < 16 * KD / 8) {  // a piece of eight of <S, dS>
       const int r = tid / (KD / 8);
-      const unsigned char *p = smem + slot + 2 * tile_at<KD>(r, tid % (KD / 8));
+      const unsigned char *p = smem + stage + 2 * tile_at<KD>(r, tid % (KD / 8));
       uint4 w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint4 *>(p + j * L::kTile);
@@ -529,12 +568,14 @@ gradient_kernel(const Args a) {
         const float2 z = half2_float2((&w[2].x)[j]), q = half2_float2((&w[3].x)[j]);
         sum = fmaf(x.x + y.x, z.x + q.x, fmaf(x.y + y.y, z.y + q.y, sum));
       }
-      both = fmaf(sum, __half2float(rho[local + r]) * __half2float(rho[VB + local + r]), both);
+      both = fmaf(sum, rho[local + r] * rho[VB + local + r], both);
     }
+    const float2 s0 = *reinterpret_cast<const float2 *>(rho + local + 2 * c);
+    const float2 s1 = *reinterpret_cast<const float2 *>(rho + local + 2 * c + 8);
     if (is_do) {
-      const __half2 d0 = *reinterpret_cast<const __half2 *>(rho + VB + local + 2 * c);
-      const __half2 d1 = *reinterpret_cast<const __half2 *>(rho + VB + local + 2 * c + 8);
-      uint32_t fo[NP][4], fx[NP][4], fu[2][4];
+      const float2 d0 = *reinterpret_cast<const float2 *>(rho + 2 * VB + local + 2 * c);
+      const float2 d1 = *reinterpret_cast<const float2 *>(rho + 2 * VB + local + 2 * c + 8);
+      uint32_t fo[NP][4], fx[NP][4], fw[2][4];
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
         ldsm4(a_rows<VB>(base + L::kDO + p * kC * VB * 2, row, local, lane), fo[p]);
@@ -542,124 +583,58 @@ gradient_kernel(const Args a) {
       }
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        ldsm4t(a_cols<kC>(base + L::kU + p * kSquare, local, row, lane), fu[p]);
-        scale_frag(fu[p], d0, d1, fu[p]);
+        ldsm4t(a_cols<kC>(base + L::kW + p * kWide, local, row, lane), fw[p]);
+        scale_frag(fw[p], d0, d1, fw[p]);
       }
       cols_step<KD, NP, 2>(xa, fx, st, L::kTile, 0, xcol, NX, lane);
-      cols_step<KD, 2, 2>(xb, fu, st + 2 * L::kTile, L::kTile, 0, xcol, NX, lane);
-      cols_step<kC, NP, 2>(d, fo, base + L::kU, kSquare, local, dcol, dto, lane);
+      cols_step<KD, 2, 2>(xb, fw, st + 4 * L::kTile, L::kTile, 0, xcol, NX, lane);
+      cols_step<kC, NP, 2>(d, fo, base + L::kW, kWide, local, dcol, dto, lane);
     } else {
       uint32_t fr[2][4], fx[2][4];
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        ldsm4t(a_cols<kC>(base + L::kDR + p * kSquare, local, row, lane), fr[p]);
-        scale_frag(fr[p], s0, s1, fx[p]);
-      }
+      for (int p = 0; p < 2; ++p) ldsm4t(a_cols<kC>(base + L::kDR + p * kWide, local, row, lane), fr[p]);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) scale_frag(fr[p], s0, s1, fx[p]);
       cols_step<KD, 2, 2>(xa, fx, st, L::kTile, 0, xcol, NX, lane);
-      cols_step<kC, 2, 2>(d, fr, base + L::kU, kSquare, local, dcol, dto, lane);
+      cols_step<kC, 2, 2>(d, fr, base + L::kW, kWide, local, dcol, dto, lane);
     }
   }
-  both *= big[kScaleS] * big[kScaleDS];
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) both += __shfl_xor_sync(0xffffffffu, both, s);
   if (lane == 0) both_sums[warp] = both;
 
-  // E and F from dP and dA, and M from their products with the grams q k^T and k k^T
-  const float *kfac = vec + kRowK * kC, *lfac = is_do ? a.qfac + kv_chunk * kC : kfac;
-  const float *left_inv = is_do ? do_inv : dr_inv;
+  // E and F from dP and dA
+  const float *lfac = is_do ? qfac : kfac, *left_inv = is_do ? do_inv : dr_inv;
   const float x_inv0 = left_inv[row + g], x_inv1 = left_inv[row + g + 8];
   const float l0 = lfac[row + g], l1 = lfac[row + g + 8];
-  const float b0 = vec[kRowBeta * kC + row + g], b1 = vec[kRowBeta * kC + row + g + 8];
-  const float d_lead0 = is_do ? a.scale * x_inv0 : -x_inv0 * b0, d_lead1 = is_do ? a.scale * x_inv1 : -x_inv1 * b1;
-  const bool tiny = !is_do && __any_sync(0xffffffffu, fabsf(b0) < kTinyBeta || fabsf(b1) < kTinyBeta);
-  float before[2] = {0.f, 0.f}, slow[2] = {0.f, 0.f}, max_k = 0.f, max_l = 0.f;
+  const float b0 = beta[row + g], b1 = beta[row + g + 8];
+  float max_k = 0.f, max_l = 0.f;
   {
-    const uint32_t left = base + (is_do ? L::kQ : L::kK);
+    const float lead0 = is_do ? a.scale * x_inv0 : -x_inv0 * b0, lead1 = is_do ? a.scale * x_inv1 : -x_inv1 * b1;
     const float gh0 = g_hi[row + g], gl0 = g_lo[row + g], gh1 = g_hi[row + g + 8], gl1 = g_lo[row + g + 8];
 #pragma unroll
-    for (int np = 0; np < ND / 2; ++np) {
-      float cross[4] = {0.f, 0.f, 0.f, 0.f};
-      if (np <= dto) {
-        float gram[2][4];
-        zero(gram);
-#pragma unroll
-        for (int ks = 0; ks < KD / 16; ++ks) {
-          uint32_t fa[NP][4], f[4];
-#pragma unroll
-          for (int p = 0; p < NP; ++p) ldsm4(a_rows<KD>(left + p * kC * KD * 2, row, ks * 16, lane), fa[p]);
-#pragma unroll
-          for (int p = 0; p < NP; ++p) {
-            ldsm4(b_rows<KD>(base + L::kK + p * kC * KD * 2, dcol + np * 16, ks * 16, lane), f);
-            mma(gram[0], fa[0], f[0], f[1]);
-            mma(gram[1], fa[0], f[2], f[3]);
-            if (NP == 2 && p == 0) {
-              mma(gram[0], fa[NP - 1], f[0], f[1]);
-              mma(gram[1], fa[NP - 1], f[2], f[3]);
-            }
-          }
-        }
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int nt = 2 * np + q, j = dcol + nt * 8 + 2 * c;
-          const float2 ui = *reinterpret_cast<const float2 *>(u_inv + j);
-          const float2 kf = *reinterpret_cast<const float2 *>(kfac + j);
-          const float2 gh = *reinterpret_cast<const float2 *>(g_hi + j);
-          const float2 gl = *reinterpret_cast<const float2 *>(g_lo + j);
-          float m[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int i = row + g + (e >> 1) * 8, jj = j + (e & 1);
-            const float ghi = (e >> 1 ? gh1 : gh0) - (e & 1 ? gh.y : gh.x);
-            const float glo = (e >> 1 ? gl1 : gl0) - (e & 1 ? gl.y : gl.x);
-            const float x = (e & 1 ? ui.y : ui.x) * d[nt][e];
-            if (!is_do && i == jj) sums[kSumDiag * kC + i] = x * (e >> 1 ? x_inv1 : x_inv0);
-            const bool in = is_do ? i >= jj : i > jj;
-            const float dec = in ? __expf(ghi + glo) : 0.f;
-            const float gr = (e & 1 ? kf.y : kf.x) * ((e >> 1 ? l1 : l0) * gram[q][e]);
-            if (tiny && in)  // without beta, which may be 0
-              slow[e >> 1] = fmaf(dec * gr, -(e >> 1 ? x_inv1 : x_inv0) * x, slow[e >> 1]);
-            const float ef = in ? (e >> 1 ? d_lead1 : d_lead0) * x * dec : 0.f;
-            m[e] = in ? ef * gr : 0.f;
-            d[nt][e] = ef;
-            max_k = fmaxf(max_k, fabsf(ef * (e & 1 ? kf.y : kf.x)));
-            max_l = fmaxf(max_l, fabsf(ef * (e >> 1 ? l1 : l0)));
-          }
-          // for both rows the sum of M over the columns before each of this thread's
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const float pair = m[2 * r] + m[2 * r + 1];
-            float run = pair;
-#pragma unroll
-            for (int s = 1; s < 4; s <<= 1) {
-              const float up = __shfl_up_sync(0xffffffffu, run, s, 4);
-              if (c >= s) run += up;
-            }
-            const float lead = before[r] + (run - pair);
-            before[r] += __shfl_sync(0xffffffffu, run, 3, 4);
-            const int i = row + g + 8 * r;
-            if (i >= j) cross[2 * q] += lead;
-            if (i >= j + 1) cross[2 * q + 1] += lead + m[2 * r];
-          }
-        }
-      } else {  // columns past this warp's rows: nothing crosses there
-#pragma unroll
-        for (int q = 0; q < 2; ++q)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) d[2 * np + q][e] = 0.f;
-      }
+    for (int nt = 0; nt < ND; ++nt) {
+      if (nt / 2 > dto) continue;
+      const int j = dcol + nt * 8 + 2 * c;
+      const float2 wi = *reinterpret_cast<const float2 *>(w_inv + j);
+      const float2 be = *reinterpret_cast<const float2 *>(beta + j);
+      const float2 kf = *reinterpret_cast<const float2 *>(kfac + j);
+      const float2 gh = *reinterpret_cast<const float2 *>(g_hi + j);
+      const float2 gl = *reinterpret_cast<const float2 *>(g_lo + j);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float x = cross[e];
-        x += __shfl_xor_sync(0xffffffffu, x, 4);
-        x += __shfl_xor_sync(0xffffffffu, x, 8);
-        x += __shfl_xor_sync(0xffffffffu, x, 16);
-        if (g == 0) sums[warp * kC + np * 16 + (e >> 1) * 8 + 2 * c + (e & 1)] = x;
+        const int i = row + g + (e >> 1) * 8, jj = j + (e & 1);
+        const float x = (e & 1 ? wi.y : wi.x) * d[nt][e];
+        if (!is_do && i == jj && i < here)
+          a.dbeta[gb + (long long)i * a.hv] = i < live ? x * (e >> 1 ? x_inv1 : x_inv0) : 0.f;
+        const float diff = ((e >> 1 ? gh1 : gh0) - (e & 1 ? gh.y : gh.x)) + ((e >> 1 ? gl1 : gl0) - (e & 1 ? gl.y : gl.x));
+        const bool in = is_do ? i >= jj : i > jj;
+        const float ef = in ? ((e >> 1 ? lead1 : lead0) * x) * ((e & 1 ? be.y : be.x) * __expf(diff)) : 0.f;
+        d[nt][e] = ef;
+        max_k = fmaxf(max_k, fabsf(ef * (e & 1 ? kf.y : kf.x)));
+        max_l = fmaxf(max_l, fabsf(ef * (e >> 1 ? l1 : l0)));
       }
     }
-  }
-  if (H == 2 && half == 0 && c == 0) {
-    float *to = sums + (kSumRows + (is_do ? 0 : 1)) * kC;
-    to[row + g] = before[0], to[row + g + 8] = before[1];
   }
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) {
@@ -667,58 +642,31 @@ gradient_kernel(const Args a) {
     max_l = fmaxf(max_l, __shfl_xor_sync(0xffffffffu, max_l, s));
   }
   if (lane == 0) per_warp[0][warp] = max_k, per_warp[1][warp] = max_l;
-
-  // X's true values and what they give for the decays
-  const float e0 = vec[kRowEG * kC + row + g], e1 = vec[kRowEG * kC + row + g + 8];
+  // X's true values
   {
-    const float f0 = x_inv0 * (is_do ? a.scale * e0 : -e0), f1 = x_inv1 * (is_do ? a.scale * e1 : -e1);
-    const float s_inv = big[kScaleS];
-    float d0, d1;
+    const float e0 = vec[kRowEG * kC + row + g], e1 = vec[kRowEG * kC + row + g + 8];
+    const float f0 = x_inv0 * (is_do ? a.scale * e0 : -b0 * e0), f1 = x_inv1 * (is_do ? a.scale * e1 : -b1 * e1);
 #pragma unroll
     for (int nt = 0; nt < NX; ++nt) {
-      xa[nt][0] = f0 * (s_inv * xa[nt][0]);
-      xa[nt][1] = f0 * (s_inv * xa[nt][1]);
-      xa[nt][2] = f1 * (s_inv * xa[nt][2]);
-      xa[nt][3] = f1 * (s_inv * xa[nt][3]);
+      xa[nt][0] = f0 * (big[0] * xa[nt][0]);
+      xa[nt][1] = f0 * (big[0] * xa[nt][1]);
+      xa[nt][2] = f1 * (big[0] * xa[nt][2]);
+      xa[nt][3] = f1 * (big[0] * xa[nt][3]);
     }
-    dot_rows<KD, NP>(xa, smem + (is_do ? L::kQ : L::kK), row, xcol, lane, d0, d1);
-    d0 *= l0, d1 *= l1;
-    if (!is_do) {
-      slow[0] = quad_sum(slow[0]) + d0, slow[1] = quad_sum(slow[1]) + d1;
-      if (c == 0) {
-        float *to = sums + (kSumSlow + half) * kC;
-        to[row + g] = slow[0], to[row + g + 8] = slow[1];
-      }
+    if (is_do) {
+      const float u0 = (w_inv[row + g] * b0) * vec[kRowEC * kC + row + g];
+      const float u1 = (w_inv[row + g + 8] * b1) * vec[kRowEC * kC + row + g + 8];
 #pragma unroll
       for (int nt = 0; nt < NX; ++nt) {
-        xa[nt][0] *= b0;
-        xa[nt][1] *= b0;
-        xa[nt][2] *= b1;
-        xa[nt][3] *= b1;
+        xb[nt][0] = u0 * (big[2] * xb[nt][0]);
+        xb[nt][1] = u0 * (big[2] * xb[nt][1]);
+        xb[nt][2] = u1 * (big[2] * xb[nt][2]);
+        xb[nt][3] = u1 * (big[2] * xb[nt][3]);
       }
-      d0 *= b0, d1 *= b1;
     }
-    float *in = sums + (kSumIn + (is_do ? 0 : 2) + half) * kC;
-    if (c == 0) in[row + g] = d0, in[row + g + 8] = d1;
   }
-  if (is_do) {
-    const float ds_inv = big[kScaleDS];
-    const float u0 = u_inv[row + g] * vec[kRowEC * kC + row + g];
-    const float u1 = u_inv[row + g + 8] * vec[kRowEC * kC + row + g + 8];
-    float d0, d1;
-#pragma unroll
-    for (int nt = 0; nt < NX; ++nt) {
-      xb[nt][0] = u0 * (ds_inv * xb[nt][0]);
-      xb[nt][1] = u0 * (ds_inv * xb[nt][1]);
-      xb[nt][2] = u1 * (ds_inv * xb[nt][2]);
-      xb[nt][3] = u1 * (ds_inv * xb[nt][3]);
-    }
-    dot_rows<KD, NP>(xb, smem + L::kK, row, xcol, lane, d0, d1);
-    float *out = sums + (kSumOut + half) * kC;
-    if (c == 0) out[row + g] = d0 * kfac[row + g], out[row + g + 8] = d1 * kfac[row + g + 8];
-  }
-  __syncthreads();  // u, dr, do and the ring are read; maxima and sums are there
-  Scale sk, sl, sle;  // of E or F along rows, down columns, and of E down columns
+  __syncthreads();  // w, dr, do and the ring are read; the maxima are there
+  Scale sk, sl, sle;  // of E or F with column factors, with row factors, and of E with row factors
   {
     float m[3] = {0.f, 0.f, 0.f};
 #pragma unroll
@@ -728,7 +676,7 @@ gradient_kernel(const Args a) {
       m[2] = fmaxf(m[2], per_warp[1][w]);
     }
     sk = scale_for(m[0]), sl = scale_for(m[1]), sle = scale_for(m[2]);
-    unsigned char *to = smem + L::kEF + (is_do ? 0 : 4) * L::kSquare;
+    unsigned char *cols = smem + (is_do ? L::kE : L::kF), *rows = smem + (is_do ? L::kEq : L::kFk);
     const float r0 = l0 * sl.mul, r1 = l1 * sl.mul;
 #pragma unroll
     for (int nt = 0; nt < ND; ++nt) {
@@ -739,50 +687,48 @@ gradient_kernel(const Args a) {
       const int at1 = 2 * (tile_at<kC>(row + g + 8, dcol / 8 + nt) + 2 * c);
       uint32_t hi, lo;
       split2(d[nt][0] * kx, d[nt][1] * ky, hi, lo);
-      *reinterpret_cast<uint32_t *>(to + at0) = hi;
-      *reinterpret_cast<uint32_t *>(to + L::kSquare + at0) = lo;
+      *reinterpret_cast<uint32_t *>(cols + at0) = hi;
+      *reinterpret_cast<uint32_t *>(cols + L::kSquare + at0) = lo;
       split2(d[nt][2] * kx, d[nt][3] * ky, hi, lo);
-      *reinterpret_cast<uint32_t *>(to + at1) = hi;
-      *reinterpret_cast<uint32_t *>(to + L::kSquare + at1) = lo;
+      *reinterpret_cast<uint32_t *>(cols + at1) = hi;
+      *reinterpret_cast<uint32_t *>(cols + L::kSquare + at1) = lo;
       split2(d[nt][0] * r0, d[nt][1] * r0, hi, lo);
-      *reinterpret_cast<uint32_t *>(to + 2 * L::kSquare + at0) = hi;
-      *reinterpret_cast<uint32_t *>(to + 3 * L::kSquare + at0) = lo;
+      *reinterpret_cast<uint32_t *>(rows + at0) = hi;
+      *reinterpret_cast<uint32_t *>(rows + L::kSquare + at0) = lo;
       split2(d[nt][2] * r1, d[nt][3] * r1, hi, lo);
-      *reinterpret_cast<uint32_t *>(to + 2 * L::kSquare + at1) = hi;
-      *reinterpret_cast<uint32_t *>(to + 3 * L::kSquare + at1) = lo;
+      *reinterpret_cast<uint32_t *>(rows + at1) = hi;
+      *reinterpret_cast<uint32_t *>(rows + L::kSquare + at1) = lo;
     }
   }
   __syncthreads();  // E and F are in shared memory
-  {  // dq = X1 + E k, and X3 + F k: along rows
-    const uint32_t ef = base + L::kEF + (is_do ? 0 : 4) * L::kSquare;
-    float y[NX][4];
-    zero(y);
+  constexpr int kExchange = NX * 2 * 32;  // pairs of a warp
+  float2 *exchange = reinterpret_cast<float2 *>(smem + L::kDK) + (warp % (4 * H)) * kExchange + lane;
+  float y[NX][4];
+  zero(y);
+  if (is_do) {
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
+    for (int ks = 0; ks < 4; ++ks) {  // dq = X1 + E k
       if (ks > rb) continue;
       uint32_t f[2][4];
 #pragma unroll
-      for (int p = 0; p < 2; ++p) ldsm4(a_rows<kC>(ef + p * L::kSquare, row, ks * 16, lane), f[p]);
+      for (int p = 0; p < 2; ++p) ldsm4(a_rows<kC>(base + L::kE + p * L::kSquare, row, ks * 16, lane), f[p]);
       cols_step<KD, 2, NP>(y, f, base + L::kK, kC * KD * 2, ks * 16, xcol, NX, lane);
     }
 #pragma unroll
     for (int nt = 0; nt < NX; ++nt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) xa[nt][e] = fmaf(y[nt][e], sk.inv, xa[nt][e]);
-  }
-  constexpr int kExchange = NX * 2 * 32;  // pairs of a warp
-  float2 *exchange = reinterpret_cast<float2 *>(smem + L::kDK) + (warp % (4 * H)) * kExchange + lane;
-  if (is_do) {
+    float d0, d1;
+    dot_rows<KD, NP>(xa, smem + L::kQ, row, xcol, lane, d0, d1);
+    if (c == 0) qdq[half * kC + row + g] = l0 * d0, qdq[half * kC + row + g + 8] = l1 * d1;
     store_grad_rows<E>(a, a.dq, dq_part, gb, row, here, xcol, lane, xa);
-    // E^T q, down the columns
-    float y[NX][4];
     zero(y);
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
+    for (int ks = 0; ks < 4; ++ks) {  // E^T q
       if (ks < rb) continue;
       uint32_t f[2][4];
 #pragma unroll
-      for (int p = 0; p < 2; ++p) ldsm4t(a_cols<kC>(base + L::kEF + (2 + p) * L::kSquare, ks * 16, row, lane), f[p]);
+      for (int p = 0; p < 2; ++p) ldsm4t(a_cols<kC>(base + L::kEq + p * L::kSquare, ks * 16, row, lane), f[p]);
       cols_step<KD, 2, NP>(y, f, base + L::kQ, kC * KD * 2, ks * 16, xcol, NX, lane);
     }
 #pragma unroll
@@ -790,14 +736,25 @@ gradient_kernel(const Args a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) xb[nt][e] = fmaf(y[nt][e], sle.inv, xb[nt][e]);
   } else {
-    float y[NX][4];
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {  // F k
+      if (ks > rb) continue;
+      uint32_t f[2][4];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) ldsm4(a_rows<kC>(base + L::kF + p * L::kSquare, row, ks * 16, lane), f[p]);
+      cols_step<KD, 2, NP>(y, f, base + L::kK, kC * KD * 2, ks * 16, xcol, NX, lane);
+    }
+#pragma unroll
+    for (int nt = 0; nt < NX; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) xa[nt][e] = fmaf(y[nt][e], sk.inv, xa[nt][e]);
     zero(y);
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
+    for (int ks = 0; ks < 4; ++ks) {  // F^T k
       if (ks < rb) continue;
       uint32_t f[2][4];
 #pragma unroll
-      for (int p = 0; p < 2; ++p) ldsm4t(a_cols<kC>(base + L::kEF + (6 + p) * L::kSquare, ks * 16, row, lane), f[p]);
+      for (int p = 0; p < 2; ++p) ldsm4t(a_cols<kC>(base + L::kFk + p * L::kSquare, ks * 16, row, lane), f[p]);
       cols_step<KD, 2, NP>(y, f, base + L::kK, kC * KD * 2, ks * 16, xcol, NX, lane);
     }
 #pragma unroll
@@ -812,75 +769,41 @@ gradient_kernel(const Args a) {
   if (is_do) {
 #pragma unroll
     for (int nt = 0; nt < NX; ++nt) {
-      const float2 x = exchange[(2 * nt) * 32], y = exchange[(2 * nt + 1) * 32];
+      const float2 x = exchange[(2 * nt) * 32], z = exchange[(2 * nt + 1) * 32];
       xb[nt][0] += x.x;
       xb[nt][1] += x.y;
-      xb[nt][2] += y.x;
-      xb[nt][3] += y.y;
+      xb[nt][2] += z.x;
+      xb[nt][3] += z.y;
     }
     store_grad_rows<E>(a, a.dk, dk_part, gb, row, here, xcol, lane, xb);
-    return;
-  }
-  if (warp == 4 * H) {
-    // dg: suffix sums of what comes in, prefix sums of what goes out
-    float in[2], out[2], rows[2], at[2];
+  } else if (warp == 4 * H) {
+    // dg: <S, dS> less what the tokens before each gate have had
+    float x[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int t = 2 * lane + i;
-      at[i] = in[i] = out[i] = rows[i] = 0.f;
-#pragma unroll
-      for (int j = 0; j < 2 * H; ++j) {
-        // warps of one half of the columns hold the cross sums there
-        const int hf = t / (kC / H);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (j % H == 0) at[i] += sums[((j / H) * 4 * H + hf * 4 + r) * kC + t % (kC / H)];
-      }
-#pragma unroll
-      for (int j = 0; j < H; ++j) {
-        in[i] += sums[(kSumIn + j) * kC + t] + sums[(kSumIn + 2 + j) * kC + t];
-        out[i] += sums[(kSumOut + j) * kC + t];
-      }
-      if (H == 2) rows[i] = sums[kSumRows * kC + t] + sums[(kSumRows + 1) * kC + t];
+      x[i] = qdq[t] + (H == 2 ? qdq[kC + t] : 0.f) - vdv[t];
     }
-    float after = in[0] + in[1], upto = out[0] + out[1], below = rows[0] + rows[1];
+    float upto = x[0] + x[1];
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
-      const float x = __shfl_down_sync(0xffffffffu, after, s), y = __shfl_down_sync(0xffffffffu, below, s);
       const float up = __shfl_up_sync(0xffffffffu, upto, s);
-      if (lane + s < 32) after += x, below += y;
       if (lane >= s) upto += up;
     }
     upto = __shfl_up_sync(0xffffffffu, upto, 1);
     if (lane == 0) upto = 0.f;
-    float later = __shfl_down_sync(0xffffffffu, after, 1), lower = __shfl_down_sync(0xffffffffu, below, 1);
-    if (lane == 31) later = lower = 0.f;
-    float through = 0.f;
+    float all = 0.f;
 #pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) through += both_sums[w];
-    through *= vec[kRowEG * kC + kC - 1];
-    const int t = 2 * lane;
-    const bool second_half = H == 2 && t >= kC / 2;  // the first half's columns lie before t there
-    const float x = at[0] + (second_half ? below : 0.f) + after + upto + through;
-    const float y = at[1] + (second_half ? rows[1] + lower : 0.f) + (in[1] + later) + (upto + out[0]) + through;
-    if (t < here) a.dg[gb + (long long)t * a.hv] = t < live ? x : 0.f;
-    if (t + 1 < here) a.dg[gb + (long long)(t + 1) * a.hv] = t + 1 < live ? y : 0.f;
-  } else if (warp == 4 * H + 1) {
-    for (int t = lane; t < here; t += 32) {
-      const float beta = vec[kRowBeta * kC + t];
-      if (fabsf(beta) >= kTinyBeta || t >= live)
-        a.dbeta[gb + (long long)t * a.hv] = t < live ? sums[kSumDiag * kC + t] / beta : 0.f;
-    }
-    for (int t = 0; t < live; ++t) {
-      if (!(fabsf(vec[kRowBeta * kC + t]) < kTinyBeta)) continue;
-      const E *v = static_cast<const E *>(a.v) + b * a.sv.b + (t0 + t) * a.sv.t + h * a.sv.h;
-      float x = 0.f;
-      for (int i = lane; i < a.vdim; i += 32) x = fmaf(a.drs[(chunk * a.vp + i) * kC + t], Elem<E>::get(v[i]), x);
+    for (int w = 0; w < kThreads / 32; ++w) all += both_sums[w];
+    all *= big[0] * big[1];
 #pragma unroll
-      for (int s = 16; s > 0; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
-#pragma unroll
-      for (int j = 0; j < H; ++j) x += sums[(kSumSlow + j) * kC + t];
-      if (lane == 0) a.dbeta[gb + (long long)t * a.hv] = x;
+    for (int i = 0; i < 2; ++i) {
+      const int t = 2 * lane + i;
+      // a gate at the least decay is closed: nothing passes, and its gradient is 0
+      const float gate = t == 0 ? g_hi[0] : (g_hi[t] - g_hi[t - 1]) + (g_lo[t] - g_lo[t - 1]);
+      if (t < here)
+        a.dg[gb + (long long)t * a.hv] =
+            t < live && gate > 0.999f * kMinDecay ? all - (upto + (i ? x[0] : 0.f)) : 0.f;
     }
   }
 }

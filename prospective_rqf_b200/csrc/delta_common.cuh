@@ -13,6 +13,10 @@
 //   r = beta (v - e^G k S),   u = T r,   o = scale e^G q S + P u,
 //   S' = e^{G_C} S + (e^{G_C-G} k)^T u.
 //
+// A's rows have the factor beta_i, and so have those of T - I = diag(beta) T'.  The kernels take
+// w = u / beta = (v - e^G k S) + T' r, which is what each token finds missing at its key: with it
+// a beta of 0 needs no division anywhere, and dbeta = dr.w.
+//
 // Operands.  The products run on the tensor cores (m16n8k16, half inputs,
 // 32-bit sums), yet states, cotangents of the 32-bit inputs and the chain from
 // chunk to chunk have to keep 32-bit accuracy.  So a 32-bit operand enters as
@@ -28,8 +32,8 @@
 // What token i puts into the state is k^_i (kfac_i u_i), so the kernels carry
 // kfac u and kfac r, in which tokens of small and large keys stand as they
 // count, with A^_ij = beta_i kfac_i^2 e^{G_i-G_j} k^_i.k^_j in A's place.  And
-// T = I + T': r itself is added in 32 bits, so that a token whose key is tiny
-// still has its own u to 32 bits for the gradient of that key.
+// T' r is added in 32 bits to what a token has by itself, so that one whose key
+// is tiny still has its own w to 32 bits for the gradient of that key.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -41,20 +45,19 @@ namespace rqf {
 namespace delta {
 
 constexpr int kC = 64;       // tokens of a chunk
-constexpr int kVec = 9;      // coefficient rows kept for a chunk (enum Row)
+constexpr int kVec = 8;      // coefficient rows kept for a chunk (enum Row)
 constexpr float kMinDecay = -200.f;  // e^-200 is 0 in 32 bits: -inf gates are taken as this
 
 // Coefficient rows of a chunk, 64 floats each.
 enum Row {
-  kRowKS = 0,    // beta kfac^2 e^G: the factor of k S in r
-  kRowV = 1,     // beta kfac: the factor of v in r
-  kRowT = 2,     // 2^t, the scale of T's row
+  kRowKS = 0,    // kfac^2 e^G: the factor of k S in w
+  kRowK = 1,     // kfac: that of v
+  kRowT = 2,     // 2^t, the scale of the row of T'
   kRowP = 3,     // 2^p, the scale of P's row
   kRowO = 4,     // scale e^G qfac: the factor of q S in o
   kRowEG = 5,    // e^G
   kRowEC = 6,    // e^{G_C-G}
-  kRowBeta = 7,  // beta
-  kRowK = 8      // kfac
+  kRowBeta = 7   // beta
 };
 
 template <typename E>
@@ -274,8 +277,9 @@ struct Strides {
 };
 
 // One call's tensors and sizes.  n_chunks covers `time`; a row's own length
-// ends it earlier.  u and dr are [row][chunk][v][64], v padded to VP, a multiple
-// of 16.
+// ends it earlier.  w and dr are [row][chunk][v][64], v padded to VP, a multiple
+// of 16; dstates has one slot more for each row than it has chunks, slot n for
+// the cotangent of the state that enters chunk n.
 struct Args {
   const void *q, *k, *v, *dout;
   const float *g, *beta;
@@ -292,9 +296,9 @@ struct Args {
   // workspace and saved context
   __half *khat, *qhat, *tmat, *pmat;
   float *kfac, *qfac, *vec;
-  double *gsum;
+  float2 *gsum;  // running sums of g inside a chunk, hi and lo
   __half *states, *dstates;  // [chunk][hi, lo][v][KD], rows scaled
-  float *scales, *us, *drs, *token_maxes;
+  float *scales, *dscales, *ws, *drs, *token_maxes, *vdv;
   float *dq_part, *dk_part;  // (B, T, Hv, K) when key heads are shared
 };
 

@@ -1,13 +1,16 @@
 // The part of a chunk that needs no state: the scaled halves of q and k, the
-// decays, T' = (I + A)^{-1} - I and P, both for the scaled keys.  One CTA for a chunk of a value head, all
+// decays, T' with (I + A)^{-1} = I + diag(beta) T', and P, both for the scaled keys.  One CTA for a chunk of a value head, all
 // chunks at once.
 //
 // A and P are one 64 x 64 x K product each on the tensor cores, from exact
-// halves.  T solves (I + A) T = I in 32 bits: the four 16 x 16 blocks on the
-// diagonal by substitution (a thread for each column), then the blocks below
-// them from -T22 A21 T11, at 16 and at 32, which stays accurate where the keys
-// of a chunk are nearly parallel (powers of A, the other usual form, do not:
-// their entries grow like binomials and cancel).
+// halves.  With A = diag(beta) B, T' solves T' = -B (I + diag(beta) T') in 32
+// bits: the four 16 x 16 blocks on the diagonal by substitution (a thread for
+// each column), then the blocks below them, at 16 and at 32, as
+//
+//   X = B21 + B21 diag(beta1) T'11,   T'21 = -(X + T'22 diag(beta2) X),
+//
+// which stays accurate where the keys of a chunk are nearly parallel (powers of
+// A, the other usual form, do not: their entries grow like binomials and cancel).
 #pragma once
 
 #include "delta_common.cuh"
@@ -105,10 +108,10 @@ __device__ __forceinline__ void store_square_row(const float *row, int from, flo
   }
 }
 
-// Blocks of N below the diagonal blocks of T: T21 = -T22 (A21 T11) for every
-// pair of neighbouring N x N blocks; A21 T11 stands in T21's place meanwhile.
+// Blocks of N below the diagonal blocks of T', for every pair of neighbouring N x N blocks; X
+// stands in T'21's place meanwhile.
 template <int N>
-__device__ __forceinline__ void merge_blocks(const float *A, float *T, int tid) {
+__device__ __forceinline__ void merge_blocks(const float *A, float *T, const float *beta, int tid) {
   constexpr int kPairs = kC / (2 * N);
   constexpr int kEach = kPairs * N * N / kPrepThreads;  // elements of a thread: 4 or 8
   // a thread has one column and kEach rows of a pair's block
@@ -116,19 +119,17 @@ __device__ __forceinline__ void merge_blocks(const float *A, float *T, int tid) 
   const int base = pair * 2 * N;
   float x[kEach];
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) x[i] = 0.f;
+  for (int i = 0; i < kEach; ++i) x[i] = A[(base + N + r0 + i) * kLdA + base + col];
   for (int l = 0; l < N; ++l) {
-    const float t = T[(base + l) * kLdA + base + col];
+    const float t = beta[base + l] * T[(base + l) * kLdA + base + col];
 #pragma unroll
     for (int i = 0; i < kEach; ++i) x[i] = fmaf(A[(base + N + r0 + i) * kLdA + base + l], t, x[i]);
   }
 #pragma unroll
   for (int i = 0; i < kEach; ++i) T[(base + N + r0 + i) * kLdA + base + col] = x[i];
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) x[i] = 0.f;
   for (int l = 0; l < N; ++l) {
-    const float t = T[(base + N + l) * kLdA + base + col];
+    const float t = beta[base + N + l] * T[(base + N + l) * kLdA + base + col];
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
       x[i] = fmaf(T[(base + N + r0 + i) * kLdA + base + N + l], t, x[i]);
@@ -212,7 +213,7 @@ __global__ void __launch_bounds__(kPrepThreads) prep_kernel(const Args a) {
     for (int e = 0; e < 4; ++e) {
       const int i = warp * 16 + g + (e >> 1) * 8, j = nt * 8 + 2 * c + (e & 1);
       const float d = i >= j ? expf((float)(G[i] - G[j])) : 0.f;
-      A[i * kLdA + j] = i > j ? beta[i] * (kfac[i] * (kfac[i] * (d * kk[nt][e]))) : 0.f;
+      A[i * kLdA + j] = i > j ? kfac[i] * (kfac[i] * (d * kk[nt][e])) : 0.f;
       qk[nt][e] = i >= j ? a.scale * d * qfac[i] * qk[nt][e] : 0.f;
       m[e >> 1] = fmaxf(m[e >> 1], fabsf(qk[nt][e]));
     }
@@ -242,36 +243,33 @@ __global__ void __launch_bounds__(kPrepThreads) prep_kernel(const Args a) {
   }
   __syncthreads();
 
-  // T: diagonal blocks of 16 by substitution, then 32 and 64
+  // T': diagonal blocks of 16 by substitution, then 32 and 64
   if (tid < kC) {
     const int base = tid & ~15, col = tid & 15;
     float t[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      float x = i == col ? 1.f : 0.f, y = 0.f;
+      float x = 0.f, y = 0.f;
 #pragma unroll
       for (int l = 0; l < i; ++l) {
         const float e = A[(base + i) * kLdA + base + l];
-        if (l & 1) y = fmaf(-e, t[l], y);
-        else x = fmaf(-e, t[l], x);
+        if (l & 1) y = fmaf(e, t[l], y);
+        else x = fmaf(e, t[l], x);
       }
-      t[i] = x + y;
+      // t: the column of I + diag(beta) T'
+      t[i] = i < col ? 0.f : i == col ? 1.f : -beta[base + i] * (x + y);
+      if (i > col) T[(base + i) * kLdA + base + col] = -(x + y);
     }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) T[(base + i) * kLdA + base + col] = t[i];
   }
   __syncthreads();
-  merge_blocks<16>(A, T, tid);
-  merge_blocks<32>(A, T, tid);
+  merge_blocks<16>(A, T, beta, tid);
+  merge_blocks<32>(A, T, beta, tid);
 
   {
     const int row = tid >> 1, from = (tid & 1) * 32;
     float mx = 0.f;
 #pragma unroll 8
-    for (int j = 0; j < 32; ++j) {
-      if (from + j == row) T[row * kLdA + row] = 0.f;  // I apart
-      mx = fmaxf(mx, fabsf(T[row * kLdA + from + j]));
-    }
+    for (int j = 0; j < 32; ++j) mx = fmaxf(mx, fabsf(T[row * kLdA + from + j]));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     const Scale s = scale_for(mx);
     __half *out = a.tmat + chunk * 2 * kC * kC + row * kC;
@@ -281,14 +279,16 @@ __global__ void __launch_bounds__(kPrepThreads) prep_kernel(const Args a) {
   if (tid < kC) {
     const double last = G[kC - 1];
     const float eg = expf((float)G[tid]), ec = expf((float)(last - G[tid]));
-    vec[kRowKS * kC + tid] = beta[tid] * (kfac[tid] * (kfac[tid] * eg));
-    vec[kRowV * kC + tid] = beta[tid] * kfac[tid];
+    vec[kRowKS * kC + tid] = kfac[tid] * (kfac[tid] * eg);
     vec[kRowBeta * kC + tid] = beta[tid];
     vec[kRowK * kC + tid] = kfac[tid];
     vec[kRowO * kC + tid] = a.scale * eg * qfac[tid];
     vec[kRowEG * kC + tid] = eg;
     vec[kRowEC * kC + tid] = ec;
-    if (a.gsum != nullptr) a.gsum[chunk * kC + tid] = G[tid];
+    if (a.gsum != nullptr) {
+      const float hi = (float)G[tid];
+      a.gsum[chunk * kC + tid] = make_float2(hi, (float)(G[tid] - hi));
+    }
   }
 }
 

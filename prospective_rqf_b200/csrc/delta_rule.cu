@@ -78,15 +78,18 @@ size_t carve_context(void *buffer, const Sizes &s, bool save, Args *a) {
   if (save) {
     c.take(a->gsum, (size_t)s.bhn * kC);
     c.take(a->states, (size_t)s.bhn * 2 * s.vp * s.kd);
-    c.take(a->us, (size_t)s.bhn * s.vp * kC);
-    c.take(a->scales, (size_t)s.bhn * kScales * s.vp);
+    c.take(a->ws, (size_t)s.bhn * s.vp * kC);
+    c.take(a->scales, (size_t)s.bhn * s.vp);
     c.take(a->token_maxes, (size_t)s.bhn * kTokenMaxes * (s.vp / 16) * kC);
   }
   return c.used;
 }
 size_t carve_workspace(void *buffer, const rqf_delta_problem *p, const Sizes &s, Args *a) {
   Carver c{static_cast<unsigned char *>(buffer)};
-  c.take(a->dstates, (size_t)s.bhn * 2 * s.vp * s.kd);
+  const size_t slots = (size_t)s.bhn + (size_t)p->batch * p->value_heads;
+  c.take(a->dstates, slots * 2 * s.vp * s.kd);
+  c.take(a->dscales, slots * s.vp);
+  c.take(a->vdv, (size_t)s.bhn * (s.vp / 16) * kC);
   c.take(a->drs, (size_t)s.bhn * s.vp * kC);
   a->dq_part = a->dk_part = nullptr;
   if (p->value_heads != p->key_heads) {
@@ -173,7 +176,7 @@ int run_backward(const Args &a, cudaStream_t st) {
   }
   if (rc != RQF_OK || a.n_chunks == 0) return rc;
   rc = launch(gradient_kernel<E, KD>, (int64_t)a.batch * a.hv * a.n_chunks,
-              Grad<KD, Elem<E>::kParts>::kThreads, Grad<KD, Elem<E>::kParts>::kBytes, a, st);
+              Grad<E, KD>::kThreads, Grad<E, KD>::kBytes, a, st);
   if (rc != RQF_OK || a.dq_part == nullptr) return rc;
   const int64_t rows = a.batch * a.time, pairs = rows * a.hk * (a.kdim / 2);
   const int64_t blocks = ceil_div(pairs, 256);

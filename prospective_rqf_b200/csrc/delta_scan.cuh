@@ -4,7 +4,7 @@
 // never meet, so warps share only the chunk's tiles (k, q, T, P), and each
 // product's sums are laid out as the next one's left operand needs them:
 //
-//   (kS)^T = S^T k^T  ->  r^T  ->  u^T = r^T + r^T T'^T  ->  o^T, S'^T += u^T k
+//   (kS)^T = S^T k^T  ->  r^T  ->  w^T = (r / beta)^T + r^T T'^T, u = beta w  ->  o^T, S'^T += u^T k
 //
 // runs with no trip through shared memory.  That is why these products use
 // m16n8k16 and not tcgen05: the chain from one chunk to the next is three
@@ -241,10 +241,8 @@ __device__ __forceinline__ void save_rows(float *dst, int lane, const float (&x)
 
 // What the backward's last pass finds of S and dS': the halves that the products took, and each
 // row's 1 / scale (next to nothing for a row of zeros, which so stands below all others).
-enum RowScale { kScaleS = 0, kScaleDS, kScales };
-__device__ __forceinline__ void save_scales(float *scales, long long chunk, int which, int vp, int v0,
-                                            float m0, float m1, int lane) {
-  float *to = scales + (chunk * kScales + which) * vp + v0 + (lane >> 2);
+__device__ __forceinline__ void save_scales(float *scales, float m0, float m1, int lane) {
+  float *to = scales + (lane >> 2);
   if ((lane & 3) == 0) {
     to[0] = m0 == 0.f ? 0x1p-118f : scale_for(m0).inv;
     to[8] = m1 == 0.f ? 0x1p-118f : scale_for(m1).inv;
@@ -260,17 +258,13 @@ __device__ __forceinline__ void save_frag(__half *hi_rows, long long plane, int 
     *reinterpret_cast<uint32_t *>(to + plane) = lo[i];
   }
 }
-// And of u, dr and do the largest magnitude of each token in each warp's columns.
-enum TokenMax { kTokenU = 0, kTokenDR, kTokenDO, kTokenMaxes };
+// And of w, dr and do the largest magnitude of each token in each warp's columns.
+enum TokenMax { kTokenW = 0, kTokenDR, kTokenDO, kTokenMaxes };
 
-__device__ __forceinline__ void save_token_max(float *maxes, long long chunk, int which, int warps, int w,
-                                               const float (&x)[8][4], int lane) {
-  // over the 16 rows: each exchange halves the tokens that a lane still has
-  float m[8][2];
-#pragma unroll
-  for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) m[nt][e] = fmaxf(fabsf(x[nt][e]), fabsf(x[nt][e + 2]));
+// Over the 16 rows of a warp's tiles the largest magnitude, or the sum, of each token; lane l
+// stores those of tokens 2l and 2l + 1.  Each exchange halves the tokens that a lane still has.
+template <bool SUM>
+__device__ __forceinline__ void save_tokens(float *to, float (&m)[8][2], int lane) {
 #pragma unroll
   for (int half = 4; half > 0; half >>= 1) {
     const bool up = lane & (half * 4);
@@ -279,11 +273,20 @@ __device__ __forceinline__ void save_token_max(float *maxes, long long chunk, in
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float give = up ? m[nt][e] : m[nt + half][e], keep = up ? m[nt + half][e] : m[nt][e];
-        m[nt][e] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, give, half * 4));
+        const float got = __shfl_xor_sync(0xffffffffu, give, half * 4);
+        m[nt][e] = SUM ? keep + got : fmaxf(keep, got);
       }
   }
-  float *to = maxes + ((chunk * kTokenMaxes + which) * warps + w) * kC;
   *reinterpret_cast<float2 *>(to + 2 * lane) = make_float2(m[0][0], m[0][1]);
+}
+__device__ __forceinline__ void save_token_max(float *maxes, long long chunk, int which, int warps, int w,
+                                               const float (&x)[8][4], int lane) {
+  float m[8][2];
+#pragma unroll
+  for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) m[nt][e] = fmaxf(fabsf(x[nt][e]), fabsf(x[nt][e + 2]));
+  save_tokens<false>(maxes + ((chunk * kTokenMaxes + which) * warps + w) * kC, m, lane);
 }
 
 template <typename E, int KD, int W, bool SAVE>
@@ -335,9 +338,9 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
       row_max(S, m0, m1);
       const float big0 = m0, big1 = m1;
       const Scale s0 = scale_for(m0), s1 = scale_for(m1);
-      if (SAVE) save_scales(a.scales, first + n, kScaleS, a.vp, v0, m0, m1, lane);
+      if (SAVE) save_scales(a.scales + (first + n) * a.vp + v0, m0, m1, lane);
       __half *keep = SAVE ? a.states + ((first + n) * 2 * a.vp + v0) * KD : nullptr;
-      float r[8][4], qs[8][4];
+      float r[8][4], qs[8][4];  // r without beta, from here to w
       zero(r);
       zero(qs);
 #pragma unroll
@@ -356,7 +359,7 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt) {
           const float2 f = *reinterpret_cast<const float2 *>(vec + kRowKS * kC + nt * 8 + 2 * c);
-          const float2 be = *reinterpret_cast<const float2 *>(vec + kRowV * kC + nt * 8 + 2 * c);
+          const float2 be = *reinterpret_cast<const float2 *>(vec + kRowK * kC + nt * 8 + 2 * c);
           r[nt][0] = be.x * x[nt][0] - f.x * (s0.inv * r[nt][0]);
           r[nt][1] = be.y * x[nt][1] - f.y * (s0.inv * r[nt][1]);
           r[nt][2] = be.x * x[nt][2] - f.x * (s1.inv * r[nt][2]);
@@ -365,12 +368,20 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
       }
       float u[8][4], y[8][4];
       uint32_t hi[4], lo[4];
-      row_max(r, m0, m1);
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt) {
+        const float2 be = *reinterpret_cast<const float2 *>(vec + kRowBeta * kC + nt * 8 + 2 * c);
+        y[nt][0] = be.x * r[nt][0];
+        y[nt][1] = be.y * r[nt][1];
+        y[nt][2] = be.x * r[nt][2];
+        y[nt][3] = be.y * r[nt][3];
+      }
+      row_max(y, m0, m1);
       Scale x0 = scale_for(m0), x1 = scale_for(m1);
       zero(u);
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
-        split_frag(r, ks, x0.mul, x1.mul, hi, lo);
+        split_frag(y, ks, x0.mul, x1.mul, hi, lo);
         step_rows<kC, 2>(u, hi, lo, st + St::kT, kC * kC * 2, ks, ks, lane);
       }
 #pragma unroll
@@ -381,7 +392,7 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
         u[nt][2] = fmaf(f.x * x1.inv, u[nt][2], r[nt][2]);
         u[nt][3] = fmaf(f.y * x1.inv, u[nt][3], r[nt][3]);
       }
-      if (SAVE) {  // u without the keys' factors
+      if (SAVE) {  // w without the keys' factors
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt) {
           const float2 f = *reinterpret_cast<const float2 *>(vec + kRowK * kC + nt * 8 + 2 * c);
@@ -391,8 +402,16 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
           r[nt][2] = fx * u[nt][2];
           r[nt][3] = fy * u[nt][3];
         }
-        save_rows(a.us + ((first + n) * a.vp + v0) * kC, lane, r);
-        save_token_max(a.token_maxes, first + n, kTokenU, a.vp / 16, w, r, lane);
+        save_rows(a.ws + ((first + n) * a.vp + v0) * kC, lane, r);
+        save_token_max(a.token_maxes, first + n, kTokenW, a.vp / 16, w, r, lane);
+      }
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt) {
+        const float2 be = *reinterpret_cast<const float2 *>(vec + kRowBeta * kC + nt * 8 + 2 * c);
+        u[nt][0] *= be.x;
+        u[nt][1] *= be.y;
+        u[nt][2] *= be.x;
+        u[nt][3] *= be.y;
       }
       row_max(u, m0, m1);
       x0 = scale_for(m0), x1 = scale_for(m1);
