@@ -60,23 +60,31 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
   load_state<KD>(a.dsT ? a.dsT + bh * a.kdim * a.vdim : nullptr, on ? v0 : a.vdim, a.kdim, a.vdim, lane,
                  S);
 
-  if (chunks > 0) {
-    const int n = chunks - 1;
-    load_stage<KD, NP, W * 32>(base + (n & 1) * St::kBytes, a, kv_first + n, first + n, tid);
-    copy_commit();
-    if (on) Tile::load(tile, dout + (long long)n * kC * so, so, (int)(len - (long long)n * kC), cols, lane);
-    copy_commit();
+  __shared__ __align__(8) uint64_t bars[2];
+  const uint32_t bar = smem_u32(bars);
+  Waiter wait{a.error, false};
+  if (tid == 0) {
+    bar_init(bar);
+    bar_init(bar + 8);
+    bars_ready();
+    if (chunks > 0) load_stage<KD, NP>(base, a, kv_first + chunks - 1, first + chunks - 1, bar);
   }
+  if (chunks > 0 && on) {
+    const long long t0 = (long long)(chunks - 1) * kC;
+    Tile::load(tile, dout + t0 * so, so, (int)(len - t0), cols, lane);
+  }
+  copy_commit();
+  __syncthreads();
   for (int n = chunks - 1; n >= 0; --n) {
-    const uint32_t st = base + (n & 1) * St::kBytes;
-    const float *vec = reinterpret_cast<const float *>(smem + (n & 1) * St::kBytes + St::kV);
+    const int turn = chunks - 1 - n;
+    const uint32_t st = base + (turn & 1) * St::kBytes;
+    const float *vec = reinterpret_cast<const float *>(smem + (turn & 1) * St::kBytes + St::kV);
     const long long t0 = (long long)n * kC;
-    copy_wait<1>();
-    __syncthreads();
-    if (n > 0)
-      load_stage<KD, NP, W * 32>(base + ((n - 1) & 1) * St::kBytes, a, kv_first + n - 1,
-                                 first + n - 1, tid);
-    copy_commit();
+    wait(bar + (turn & 1) * 8, (turn >> 1) & 1);
+    __syncthreads();  // all are done with the other stage
+    if (tid == 0 && n > 0)
+      load_stage<KD, NP>(base + ((turn + 1) & 1) * St::kBytes, a, kv_first + n - 1, first + n - 1,
+                         bar + ((turn + 1) & 1) * 8);
     if (on) {
       float m0, m1;
       uint32_t hi[4], lo[4];
@@ -84,16 +92,16 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
       const float big0 = m0, big1 = m1;
       const Scale s0 = scale_for(m0), s1 = scale_for(m1);
       save_scales(a.dscales + (slot + n + 1) * a.vp + v0, m0, m1, lane);
-      __half *keep = a.dstates + ((slot + n + 1) * 2 * a.vp + v0) * KD;
+      __half *keep = a.dstates + ((slot + n + 1) * a.vp + v0) * 2 * KD;
       float du[8][4], dr[8][4], x[8][4];
       zero(dr);  // k dS' first
 #pragma unroll
       for (int ks = 0; ks < KD / 16; ++ks) {
         split_frag(S, ks, s0.mul, s1.mul, hi, lo);
-        save_frag<KD>(keep, (long long)a.vp * KD, ks, lane, hi, lo);
+        save_frag<KD>(keep, ks, lane, hi, lo);
         step_rows<KD, NP>(dr, hi, lo, st + St::kK, kC * KD * 2, ks, 0, lane);
       }
-      copy_wait<1>();
+      copy_wait<0>();
       __syncwarp();
       Tile::get(tile, mine, lane, x);
       __syncwarp();  // v takes the place of do
@@ -246,7 +254,7 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
     for (int ks = 0; ks < KD / 16; ++ks) {
       uint32_t hi[4], lo[4];
       split_frag(S, ks, s0.mul, s1.mul, hi, lo);
-      save_frag<KD>(a.dstates + (slot * 2 * a.vp + v0) * KD, (long long)a.vp * KD, ks, lane, hi, lo);
+      save_frag<KD>(a.dstates + (slot * a.vp + v0) * 2 * KD, ks, lane, hi, lo);
     }
   }
   if (a.ds0 != nullptr)
@@ -339,16 +347,13 @@ __device__ __forceinline__ void split_dout(unsigned char *tile, const E *src, lo
 // 16 columns of V of S, dS and dS' into one stage of the ring.
 template <typename E, int KD>
 __device__ __forceinline__ void load_states(uint32_t stage, const Args &a, long long chunk, long long slot, int v0,
-                                            int tid) {
+                                            uint32_t bar) {
   using L = Grad<E, KD>;
-  const long long plane = (long long)a.vp * KD, at = (long long)v0 * KD;
-  const __half *S = a.states + chunk * 2 * plane + at, *dS = a.dstates + slot * 2 * plane + at;
-#pragma unroll
-  for (int p = 0; p < 2; ++p) {
-    copy_tile<KD>(stage + p * L::kTile, S + p * plane, 16, tid, L::kThreads);
-    copy_tile<KD>(stage + (2 + p) * L::kTile, dS + p * plane, 16, tid, L::kThreads);
-    copy_tile<KD>(stage + (4 + p) * L::kTile, dS + (2 + p) * plane, 16, tid, L::kThreads);
-  }
+  const long long plane = 2LL * a.vp * KD, at = 2LL * v0 * KD;
+  bar_expect(bar, L::kStage);
+  bulk_load(stage, a.states + chunk * plane + at, 2 * L::kTile, bar);
+  bulk_load(stage + 2 * L::kTile, a.dstates + slot * plane + at, 2 * L::kTile, bar);
+  bulk_load(stage + 4 * L::kTile, a.dstates + (slot + 1) * plane + at, 2 * L::kTile, bar);
 }
 
 // A fragment with its contraction's columns times powers of two: f0 for 2c, 2c + 1, f1 for
@@ -480,17 +485,22 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
   }
   const long long chunk = bh * a.n_chunks + n, kv_chunk = ((long long)b * a.hk + hk) * a.n_chunks + n;
   const long long slot = bh * (a.n_chunks + 1) + n;
-  copy_tile<KD>(base + L::kK, a.khat + kv_chunk * NP * kC * KD, NP * kC, tid, kThreads);
-  copy_tile<KD>(base + L::kQ, a.qhat + kv_chunk * NP * kC * KD, NP * kC, tid, kThreads);
-  for (int i = tid; i < (kVec + 1) * kC / 4; i += kThreads)
-    copy16(base + L::kCoef + i * 16,
-           i < kVec * kC / 4 ? a.vec + chunk * kVec * kC + i * 4 : a.qfac + kv_chunk * kC + (i - kVec * kC / 4) * 4);
-  copy_commit();
   const int steps = a.vp / 16;
+  __shared__ __align__(8) uint64_t bars[L::kStages + 1];
+  const uint32_t bar = smem_u32(bars), first_bar = bar + L::kStages * 8;
+  Waiter wait{a.error, false};
+  if (tid == 0) {
 #pragma unroll
-  for (int i = 0; i < L::kStages - 1; ++i) {
-    if (i < steps) load_states<E, KD>(base + L::kRing + i * L::kStage, a, chunk, slot, i * 16, tid);
-    copy_commit();
+    for (int i = 0; i <= L::kStages; ++i) bar_init(bar + i * 8);
+    bars_ready();
+    bar_expect(first_bar, 2 * L::kKq + (kVec + 1) * kC * 4);
+    bulk_load(base + L::kCoef, a.vec + chunk * kVec * kC, kVec * kC * 4, first_bar);
+    bulk_load(base + L::kCoef + kVec * kC * 4, a.qfac + kv_chunk * kC, kC * 4, first_bar);
+    bulk_load(base + L::kK, a.khat + kv_chunk * NP * kC * KD, L::kKq, first_bar);
+    bulk_load(base + L::kQ, a.qhat + kv_chunk * NP * kC * KD, L::kKq, first_bar);
+#pragma unroll
+    for (int i = 0; i < L::kStages - 1; ++i)
+      if (i < steps) load_states<E, KD>(base + L::kRing + i * L::kStage, a, chunk, slot, i * 16, bar + i * 8);
   }
   // the largest row scales of S, dS and dS', to which all rows' are taken
   const float *row_scales[3] = {a.scales + chunk * a.vp, a.dscales + slot * a.vp, a.dscales + (slot + 1) * a.vp};
@@ -544,13 +554,13 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
       for (int i = 0; i < 3; ++i)
         if (tid < rows) rho[i * VB + tid] = row_scales[i][v0 + tid] * inverse_pow2(big[i]);
     }
-    copy_wait<L::kStages - 2>();
-    __syncthreads();
-    {
+    wait(bar + step % L::kStages * 8, step / L::kStages & 1);
+    __syncthreads();  // all are done with the stage before
+    if (tid == 0) {
       const int next = step + L::kStages - 1;
       if (next < steps)
-        load_states<E, KD>(base + L::kRing + next % L::kStages * L::kStage, a, chunk, slot, next * 16, tid);
-      copy_commit();
+        load_states<E, KD>(base + L::kRing + next % L::kStages * L::kStage, a, chunk, slot, next * 16,
+                           bar + next % L::kStages * 8);
     }
     const int stage = L::kRing + step % L::kStages * L::kStage;
     const uint32_t st = base + stage;
@@ -603,6 +613,7 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
   for (int s = 16; s > 0; s >>= 1) both += __shfl_xor_sync(0xffffffffu, both, s);
   if (lane == 0) both_sums[warp] = both;
 
+  wait(first_bar, 0);  // coefficients, k and q
   // E and F from dP and dA
   const float *lfac = is_do ? qfac : kfac, *left_inv = is_do ? do_inv : dr_inv;
   const float x_inv0 = left_inv[row + g], x_inv1 = left_inv[row + g + 8];

@@ -260,16 +260,44 @@ __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// A whole tile of `rows` rows of LD halves, stored without gaps, by all threads.
-template <int LD>
-__device__ __forceinline__ void copy_tile(uint32_t dst, const __half *src, int rows, int tid,
-                                          int threads) {
-  constexpr int kPieces = LD / 8;
-  for (int i = tid; i < rows * kPieces; i += threads) {
-    const int row = i / kPieces, p = i % kPieces;
-    copy16(dst + 2 * tile_at<LD>(row, p), src + (size_t)i * 8);
-  }
+// Tiles that stand in global memory as they will stand in shared memory (tile_at's order) come
+// whole, by one thread's bulk copies, which an mbarrier counts in.
+__device__ __forceinline__ void bar_init(uint32_t bar) {
+  asm volatile("mbarrier.init.shared.b64 [%0], 1;" ::"r"(bar) : "memory");
 }
+__device__ __forceinline__ void bars_ready() {
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+// Waits for the phase of this parity.  A copy takes microseconds; where a second's worth of tries
+// has passed without it, the error word is set and no wait of this thread waits any more.
+constexpr int kWaitTries = 1 << 20;
+constexpr int kErrPipeline = 7;  // RQF_ERR_PIPELINE_TIMEOUT
+struct Waiter {
+  int *error;
+  bool gave_up;
+  __device__ __forceinline__ void operator()(uint32_t bar, uint32_t parity) {
+    if (gave_up) return;
+    for (int i = 0; i < kWaitTries; ++i) {
+      uint32_t done;
+      asm volatile(
+          "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared.b64 p, [%1], %2;\n selp.b32 %0, 1, 0, p;\n}"
+          : "=r"(done)
+          : "r"(bar), "r"(parity)
+          : "memory");
+      if (done) return;
+    }
+    gave_up = true;
+    if (error != nullptr) atomicCAS(error, 0, kErrPipeline);
+  }
+};
 
 // ------------------------------------------------------------ arguments
 struct Strides {
@@ -293,13 +321,14 @@ struct Args {
   long long time;
   int n_chunks;   // chunks of this call's span
   int n_first;    // the first of them
-  // workspace and saved context
+  // workspace and saved context; the tiles in tile_at's order
   __half *khat, *qhat, *tmat, *pmat;
   float *kfac, *qfac, *vec;
   float2 *gsum;  // running sums of g inside a chunk, hi and lo
-  __half *states, *dstates;  // [chunk][hi, lo][v][KD], rows scaled
+  __half *states, *dstates;  // [chunk][16 of v][hi, lo][16][KD], rows scaled, in tile_at's order
   float *scales, *dscales, *ws, *drs, *token_maxes, *vdv;
   float *dq_part, *dk_part;  // (B, T, Hv, K) when key heads are shared
+  int *error;                // the device's error word
 };
 
 __device__ __forceinline__ long long row_length(const Args &a, int b) {

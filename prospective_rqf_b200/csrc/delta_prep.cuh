@@ -56,8 +56,8 @@ __device__ __forceinline__ void prep_rows(const E *src, long long stride_t, int 
     if (NP == 2) *reinterpret_cast<uint4 *>(tile + kC * KD + tile_at<KD>(row, piece)) = lo;
     if (piece == 0) fac[row] = s.inv;
     if (ghat != nullptr) {
-      *reinterpret_cast<uint4 *>(ghat + row * KD + piece * 8) = hi;
-      if (NP == 2) *reinterpret_cast<uint4 *>(ghat + kC * KD + row * KD + piece * 8) = lo;
+      *reinterpret_cast<uint4 *>(ghat + tile_at<KD>(row, piece)) = hi;
+      if (NP == 2) *reinterpret_cast<uint4 *>(ghat + kC * KD + tile_at<KD>(row, piece)) = lo;
       if (piece == 0) gfac[row] = s.inv;
     }
   }
@@ -92,19 +92,18 @@ __device__ __forceinline__ void prep_gram(uint32_t a, uint32_t b, int warp, int 
   }
 }
 
-// One row of 64 floats of T (or half of one) as scaled halves, stored.
-__device__ __forceinline__ void store_square_row(const float *row, int from, float mul, __half *hi_out,
-                                                 __half *lo_out) {
+// Half a row of T' as scaled halves, stored.
+__device__ __forceinline__ void store_square_row(const float *x_row, int row, int from, float mul, __half *out) {
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
     uint4 hi, lo;
-    const float *x = row + from + p * 8;
+    const float *x = x_row + from + p * 8;
     split2(x[0] * mul, x[1] * mul, hi.x, lo.x);
     split2(x[2] * mul, x[3] * mul, hi.y, lo.y);
     split2(x[4] * mul, x[5] * mul, hi.z, lo.z);
     split2(x[6] * mul, x[7] * mul, hi.w, lo.w);
-    *reinterpret_cast<uint4 *>(hi_out + from + p * 8) = hi;
-    *reinterpret_cast<uint4 *>(lo_out + from + p * 8) = lo;
+    *reinterpret_cast<uint4 *>(out + tile_at<kC>(row, from / 8 + p)) = hi;
+    *reinterpret_cast<uint4 *>(out + kC * kC + tile_at<kC>(row, from / 8 + p)) = lo;
   }
 }
 
@@ -228,13 +227,13 @@ __global__ void __launch_bounds__(kPrepThreads) prep_kernel(const Args a) {
     for (int nt = 0; nt < 8; ++nt) {
       if (nt > 2 * warp + 1) continue;
       uint32_t hi, lo;
-      const int j = nt * 8 + 2 * c;
+      const int at0 = tile_at<kC>(i, nt) + 2 * c, at1 = tile_at<kC>(i + 8, nt) + 2 * c;
       split2(qk[nt][0] * p0.mul, qk[nt][1] * p0.mul, hi, lo);
-      *reinterpret_cast<uint32_t *>(P + i * kC + j) = hi;
-      *reinterpret_cast<uint32_t *>(P + kC * kC + i * kC + j) = lo;
+      *reinterpret_cast<uint32_t *>(P + at0) = hi;
+      *reinterpret_cast<uint32_t *>(P + kC * kC + at0) = lo;
       split2(qk[nt][2] * p1.mul, qk[nt][3] * p1.mul, hi, lo);
-      *reinterpret_cast<uint32_t *>(P + (i + 8) * kC + j) = hi;
-      *reinterpret_cast<uint32_t *>(P + kC * kC + (i + 8) * kC + j) = lo;
+      *reinterpret_cast<uint32_t *>(P + at1) = hi;
+      *reinterpret_cast<uint32_t *>(P + kC * kC + at1) = lo;
     }
     if (c == 0) {
       vec[kRowP * kC + i] = p0.inv;
@@ -272,8 +271,7 @@ __global__ void __launch_bounds__(kPrepThreads) prep_kernel(const Args a) {
     for (int j = 0; j < 32; ++j) mx = fmaxf(mx, fabsf(T[row * kLdA + from + j]));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     const Scale s = scale_for(mx);
-    __half *out = a.tmat + chunk * 2 * kC * kC + row * kC;
-    store_square_row(T + row * kLdA, from, s.mul, out, out + kC * kC);
+    store_square_row(T + row * kLdA, row, from, s.mul, a.tmat + chunk * 2 * kC * kC);
     if (from == 0) vec[kRowT * kC + row] = s.inv;
   }
   if (tid < kC) {

@@ -13,6 +13,9 @@
 
 using namespace rqf::delta;
 
+// rqf_b200.cu: the current device's error word.
+int *rqf_internal_error_word();
+
 namespace {
 
 constexpr int64_t kMaxGrid = 0x7fffffffLL;
@@ -104,6 +107,7 @@ Strides strides(const int64_t (&s)[3]) { return {s[0], s[1], s[2]}; }
 
 void common_args(const rqf_delta_problem *p, const Sizes &s, Args *a) {
   *a = Args{};
+  a->error = rqf_internal_error_word();
   a->sq = strides(p->q_stride), a->sk = strides(p->k_stride), a->sv = strides(p->v_stride);
   a->sg = strides(p->g_stride), a->sb = strides(p->beta_stride);
   a->lengths = reinterpret_cast<const long long *>(p->lengths);

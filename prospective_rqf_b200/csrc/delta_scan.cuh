@@ -9,7 +9,7 @@
 // runs with no trip through shared memory.  That is why these products use
 // m16n8k16 and not tcgen05: the chain from one chunk to the next is three
 // dependent products of 64 x 64 x 128 at most, so what counts is the time from
-// one product's sums to the next one's operand.  Tiles come by cp.async, one
+// one product's sums to the next one's operand.  Tiles come by bulk copies, one
 // chunk ahead.
 #pragma once
 
@@ -31,16 +31,16 @@ constexpr size_t scan_smem() {
   return 2 * (size_t)Stage<KD, Elem<E>::kParts>::kBytes + (size_t)W * kC * 16 * sizeof(E);
 }
 
-template <int KD, int NP, int THREADS>
+template <int KD, int NP>
 __device__ __forceinline__ void load_stage(uint32_t dst, const Args &a, long long kv_chunk,
-                                           long long chunk, int tid) {
+                                           long long chunk, uint32_t bar) {
   using S = Stage<KD, NP>;
-  copy_tile<KD>(dst + S::kK, a.khat + kv_chunk * NP * kC * KD, NP * kC, tid, THREADS);
-  copy_tile<KD>(dst + S::kQ, a.qhat + kv_chunk * NP * kC * KD, NP * kC, tid, THREADS);
-  copy_tile<kC>(dst + S::kT, a.tmat + chunk * 2 * kC * kC, 2 * kC, tid, THREADS);
-  copy_tile<kC>(dst + S::kP, a.pmat + chunk * 2 * kC * kC, 2 * kC, tid, THREADS);
-  const float *vec = a.vec + chunk * kVec * kC;
-  for (int i = tid; i < kVec * kC / 4; i += THREADS) copy16(dst + S::kV + i * 16, vec + i * 4);
+  bar_expect(bar, S::kBytes);
+  bulk_load(dst + S::kK, a.khat + kv_chunk * NP * kC * KD, S::kKq, bar);
+  bulk_load(dst + S::kQ, a.qhat + kv_chunk * NP * kC * KD, S::kKq, bar);
+  bulk_load(dst + S::kT, a.tmat + chunk * 2 * kC * kC, 2 * kC * kC * 2, bar);
+  bulk_load(dst + S::kP, a.pmat + chunk * 2 * kC * kC, 2 * kC * kC * 2, bar);
+  bulk_load(dst + S::kV, a.vec + chunk * kVec * kC, kVec * kC * 4, bar);
 }
 
 // A warp's own 64 x 16 tile of v, o, dO or dv in shared memory, [t][16 of V].
@@ -249,13 +249,13 @@ __device__ __forceinline__ void save_scales(float *scales, float m0, float m1, i
   }
 }
 template <int KD>
-__device__ __forceinline__ void save_frag(__half *hi_rows, long long plane, int ks, int lane,
-                                          const uint32_t (&hi)[4], const uint32_t (&lo)[4]) {
+__device__ __forceinline__ void save_frag(__half *tiles, int ks, int lane, const uint32_t (&hi)[4],
+                                          const uint32_t (&lo)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    __half *to = hi_rows + ((lane >> 2) + (i & 1) * 8) * KD + ks * 16 + (i >> 1) * 8 + 2 * (lane & 3);
+    __half *to = tiles + tile_at<KD>((lane >> 2) + (i & 1) * 8, ks * 2 + (i >> 1)) + 2 * (lane & 3);
     *reinterpret_cast<uint32_t *>(to) = hi[i];
-    *reinterpret_cast<uint32_t *>(to + plane) = lo[i];
+    *reinterpret_cast<uint32_t *>(to + 16 * KD) = lo[i];
   }
 }
 // And of w, dr and do the largest magnitude of each token in each warp's columns.
@@ -317,29 +317,34 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
   float S[KD / 8][4];
   load_state<KD>(a.s0 ? a.s0 + bh * a.kdim * a.vdim : nullptr, on ? v0 : a.vdim, a.kdim, a.vdim, lane, S);
 
-  if (chunks > 0) {
-    load_stage<KD, NP, W * 32>(base, a, kv_first, first, tid);
-    copy_commit();
-    if (on) Tile::load(tile, v, a.sv.t, (int)min((long long)kC, len), cols, lane);
-    copy_commit();
+  __shared__ __align__(8) uint64_t bars[2];
+  const uint32_t bar = smem_u32(bars);
+  Waiter wait{a.error, false};
+  if (tid == 0) {
+    bar_init(bar);
+    bar_init(bar + 8);
+    bars_ready();
+    if (chunks > 0) load_stage<KD, NP>(base, a, kv_first, first, bar);
   }
+  if (chunks > 0 && on) Tile::load(tile, v, a.sv.t, (int)min((long long)kC, len), cols, lane);
+  copy_commit();
+  __syncthreads();
   for (int n = 0; n < chunks; ++n) {
     const uint32_t st = base + (n & 1) * St::kBytes;
     const float *vec = reinterpret_cast<const float *>(smem + (n & 1) * St::kBytes + St::kV);
     const long long t0 = (long long)n * kC;
-    copy_wait<1>();  // this chunk's tiles; its v may still be on the way
-    __syncthreads();
-    if (n + 1 < chunks)
-      load_stage<KD, NP, W * 32>(base + ((n + 1) & 1) * St::kBytes, a, kv_first + n + 1,
-                                 first + n + 1, tid);
-    copy_commit();
+    wait(bar + (n & 1) * 8, (n >> 1) & 1);
+    __syncthreads();  // all are done with the other stage
+    if (tid == 0 && n + 1 < chunks)
+      load_stage<KD, NP>(base + ((n + 1) & 1) * St::kBytes, a, kv_first + n + 1, first + n + 1,
+                         bar + ((n + 1) & 1) * 8);
     if (on) {
       float m0, m1;
       row_max(S, m0, m1);
       const float big0 = m0, big1 = m1;
       const Scale s0 = scale_for(m0), s1 = scale_for(m1);
       if (SAVE) save_scales(a.scales + (first + n) * a.vp + v0, m0, m1, lane);
-      __half *keep = SAVE ? a.states + ((first + n) * 2 * a.vp + v0) * KD : nullptr;
+      __half *keep = SAVE ? a.states + ((first + n) * a.vp + v0) * 2 * KD : nullptr;
       float r[8][4], qs[8][4];  // r without beta, from here to w
       zero(r);
       zero(qs);
@@ -347,11 +352,11 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
       for (int ks = 0; ks < KD / 16; ++ks) {
         uint32_t hi[4], lo[4];
         split_frag(S, ks, s0.mul, s1.mul, hi, lo);
-        if (SAVE) save_frag<KD>(keep, (long long)a.vp * KD, ks, lane, hi, lo);
+        if (SAVE) save_frag<KD>(keep, ks, lane, hi, lo);
         step_rows<KD, NP>(r, hi, lo, st + St::kK, kC * KD * 2, ks, 0, lane);
         step_rows<KD, NP>(qs, hi, lo, st + St::kQ, kC * KD * 2, ks, 0, lane);
       }
-      copy_wait<1>();
+      copy_wait<0>();  // v
       __syncwarp();
       {
         float x[8][4];

@@ -480,6 +480,29 @@ int btf_backward(int drive, const float *c1, const float *c2, const float *tap1,
 
 }  // namespace
 
+// The current device's error word, for the other sources' kernels (null where there is no
+// device).  Its address is the same for the life of the device's context.
+int *rqf_internal_error_word() {
+  constexpr int kDevices = 64;
+  static std::mutex guard;
+  static int *words[kDevices] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevices) {
+    (void)cudaGetLastError();
+    return nullptr;
+  }
+  const std::lock_guard<std::mutex> lock(guard);
+  if (words[dev] == nullptr) {
+    void *p = nullptr;
+    if (cudaGetSymbolAddress(&p, g_rqf_error) != cudaSuccess) {
+      (void)cudaGetLastError();
+      return nullptr;
+    }
+    words[dev] = static_cast<int *>(p);
+  }
+  return words[dev];
+}
+
 extern "C" {
 
 int rqf_abi_version(void) { return kAbiVersion; }
