@@ -291,57 +291,86 @@ struct Grad {
   static constexpr int kEnd = kRing + kStages * kStage, kNeed = kDK + kC * KD * 4;
   static constexpr int kCoef = kEnd > kNeed ? kEnd : kNeed;  // vec's rows, qfac
   static constexpr int kFloats = kCoef + (kVec + 1) * kC * 4;
-  // rows of 64: q.dq by half, v.dv, w's scale with beta, gates' sums hi and lo; then the rows'
-  // scales of S, dS, dS'
-  static constexpr int kBytes = kFloats + 6 * kC * 4 + 3 * kVB * 4;
+  // rows of 64: q.dq by half, v.dv, gates' sums hi and lo; then the rows' scales of S, dS, dS'
+  static constexpr int kBytes = kFloats + 5 * kC * 4 + 3 * kVB * 4;
 };
 
-// A 32-bit tile [v][token] as halves hi, lo, each token's column under its own scale.
+// A 32-bit tile [v][token] by way of registers: loaded, and later stored as halves hi, lo, each
+// token's column under its own scale.
 template <int VB, int THREADS>
-__device__ __forceinline__ void split_tokens(unsigned char *hi_tile, unsigned char *lo_tile, const float *src,
-                                             int rows, const float *inv, int tid) {
-  const int p = tid & 7;
-  float mul[8];
+struct TokenTile {
+  static constexpr int kEach = VB * 8 / THREADS;
+  float x[kEach][8];
+  __device__ __forceinline__ void load(const float *src, int rows, int tid) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) mul[j] = inverse_pow2(inv[p * 8 + j]);
+    for (int it = 0; it < kEach; ++it) {
+      const int row = (tid >> 3) + it * (THREADS / 8);
 #pragma unroll
-  for (int it = 0; it < VB * 8 / THREADS; ++it) {
-    const int row = (tid >> 3) + it * (THREADS / 8);
-    float x[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = 0.f;
-    if (row < rows) load8<float>(src + row * kC + p * 8, x);
-    uint4 hi, lo;
-    split2(x[0] * mul[0], x[1] * mul[1], hi.x, lo.x);
-    split2(x[2] * mul[2], x[3] * mul[3], hi.y, lo.y);
-    split2(x[4] * mul[4], x[5] * mul[5], hi.z, lo.z);
-    split2(x[6] * mul[6], x[7] * mul[7], hi.w, lo.w);
-    *reinterpret_cast<uint4 *>(hi_tile + 2 * tile_at<kC>(row, p)) = hi;
-    *reinterpret_cast<uint4 *>(lo_tile + 2 * tile_at<kC>(row, p)) = lo;
+      for (int j = 0; j < 8; ++j) x[it][j] = 0.f;
+      if (row < rows) load8<float>(src + row * kC + (tid & 7) * 8, x[it]);
+    }
   }
-}
+  __device__ __forceinline__ void store(unsigned char *hi_tile, unsigned char *lo_tile, const float *inv, int tid) {
+    const int p = tid & 7;
+    float mul[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mul[j] = inverse_pow2(inv[p * 8 + j]);
+#pragma unroll
+    for (int it = 0; it < kEach; ++it) {
+      const int row = (tid >> 3) + it * (THREADS / 8);
+      uint4 hi, lo;
+      split2(x[it][0] * mul[0], x[it][1] * mul[1], hi.x, lo.x);
+      split2(x[it][2] * mul[2], x[it][3] * mul[3], hi.y, lo.y);
+      split2(x[it][4] * mul[4], x[it][5] * mul[5], hi.z, lo.z);
+      split2(x[it][6] * mul[6], x[it][7] * mul[7], hi.w, lo.w);
+      *reinterpret_cast<uint4 *>(hi_tile + 2 * tile_at<kC>(row, p)) = hi;
+      *reinterpret_cast<uint4 *>(lo_tile + 2 * tile_at<kC>(row, p)) = lo;
+    }
+  }
+};
 
-// A token-major tile of do [t][v] as halves, each token's row under its own scale.
+// The same of a token-major tile of do [t][v], each token's row under its own scale.
 template <typename E, int VB, int NP, int THREADS>
-__device__ __forceinline__ void split_dout(unsigned char *tile, const E *src, long long stride, int live,
-                                           int cols, const float *inv, int tid) {
-  constexpr int kPieces = VB / 8;
+struct DoutTile {
+  static constexpr int kPieces = VB / 8, kEach = kC * kPieces / THREADS;
+  float x[kEach][8];
+  __device__ __forceinline__ void load(const E *src, long long stride, int live, int cols, int tid) {
 #pragma unroll
-  for (int it = 0; it < kC * kPieces / THREADS; ++it) {
-    const int t = (tid + it * THREADS) / kPieces, p = tid % kPieces;
+    for (int it = 0; it < kEach; ++it) {
+      const int t = (tid + it * THREADS) / kPieces, p = tid % kPieces;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[it][j] = 0.f;
+      if (t < live && p * 8 < cols) load8<E>(src + t * stride + p * 8, x[it]);
+    }
+  }
+  __device__ __forceinline__ void store(unsigned char *tile, const float *inv, int tid) {
+#pragma unroll
+    for (int it = 0; it < kEach; ++it) {
+      const int t = (tid + it * THREADS) / kPieces, p = tid % kPieces;
+      const float mul = inverse_pow2(inv[t]);
+      uint4 hi, lo;
+      split2(x[it][0] * mul, x[it][1] * mul, hi.x, lo.x);
+      split2(x[it][2] * mul, x[it][3] * mul, hi.y, lo.y);
+      split2(x[it][4] * mul, x[it][5] * mul, hi.z, lo.z);
+      split2(x[it][6] * mul, x[it][7] * mul, hi.w, lo.w);
+      *reinterpret_cast<uint4 *>(tile + 2 * tile_at<VB>(t, p)) = hi;
+      if (NP == 2) *reinterpret_cast<uint4 *>(tile + kC * VB * 2 + 2 * tile_at<VB>(t, p)) = lo;
+    }
+  }
+};
+
+// Reduction of values `stride` apart, eight loads at a time.
+template <bool SUM>
+__device__ __forceinline__ float reduce_strided(const float *p, int count, int stride) {
+  float all = 0.f;
+  for (int j = 0; j < count; j += 8) {
     float x[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = 0.f;
-    if (t < live && p * 8 < cols) load8<E>(src + t * stride + p * 8, x);
-    const float mul = inverse_pow2(inv[t]);
-    uint4 hi, lo;
-    split2(x[0] * mul, x[1] * mul, hi.x, lo.x);
-    split2(x[2] * mul, x[3] * mul, hi.y, lo.y);
-    split2(x[4] * mul, x[5] * mul, hi.z, lo.z);
-    split2(x[6] * mul, x[7] * mul, hi.w, lo.w);
-    *reinterpret_cast<uint4 *>(tile + 2 * tile_at<VB>(t, p)) = hi;
-    if (NP == 2) *reinterpret_cast<uint4 *>(tile + kC * VB * 2 + 2 * tile_at<VB>(t, p)) = lo;
+    for (int i = 0; i < 8; ++i) x[i] = j + i < count ? p[(j + i) * stride] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) all = SUM ? all + x[i] : fmaxf(all, x[i]);
   }
+  return all;
 }
 
 // 16 columns of V of S, dS and dS' into one stage of the ring.
@@ -453,8 +482,8 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
   const uint32_t base = smem_u32(smem);
   const float *vec = reinterpret_cast<const float *>(smem + L::kCoef), *qfac = vec + kVec * kC;
   const float *kfac = vec + kRowK * kC, *beta = vec + kRowBeta * kC;
-  float *qdq = reinterpret_cast<float *>(smem + L::kFloats), *vdv = qdq + 2 * kC, *wb = vdv + kC;
-  float *g_hi = wb + kC, *g_lo = g_hi + kC, *rho = g_lo + kC;  // rho: [S, dS, dS'][v]
+  float *qdq = reinterpret_cast<float *>(smem + L::kFloats), *vdv = qdq + 2 * kC;
+  float *g_hi = vdv + kC, *g_lo = g_hi + kC, *rho = g_lo + kC;  // rho: [S, dS, dS'][v]
   __shared__ float w_inv[kTokenMaxes * kC], per_warp[2][kThreads / 32], both_sums[kThreads / 32];
   float *dr_inv = w_inv + kTokenDR * kC, *do_inv = w_inv + kTokenDO * kC;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
@@ -462,9 +491,10 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
   const int rb = warp & 3, row = rb * 16, half = (warp >> 2) % H;
   const int xcol = half * (KD / H), dcol = half * (kC / H);  // this warp's first columns
   const int dto = rb - half * (ND / 2);  // its last pair of columns of dP or dA: the diagonal's
-  const int n = blockIdx.x % a.n_chunks;
-  const long long bh = blockIdx.x / a.n_chunks;
-  const int b = (int)(bh / a.hv), h = (int)(bh % a.hv), hk = h / a.rep;
+  const unsigned head = blockIdx.x / (unsigned)a.n_chunks;
+  const int n = (int)(blockIdx.x - head * a.n_chunks);
+  const int b = (int)(head / (unsigned)a.hv), h = (int)(head - b * (unsigned)a.hv), hk = h / a.rep;
+  const long long bh = head;
   const long long t0 = (long long)n * kC, len = row_length(a, b);
   const int here = (int)min((long long)kC, a.time - t0);  // tokens of this chunk, live or not
   const int live = len <= t0 ? 0 : (int)min((long long)kC, len - t0);
@@ -502,31 +532,24 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
     for (int i = 0; i < L::kStages - 1; ++i)
       if (i < steps) load_states<E, KD>(base + L::kRing + i * L::kStage, a, chunk, slot, i * 16, bar + i * 8);
   }
+  const float *w_rows = a.ws + chunk * a.vp * kC, *dr_rows = a.drs + chunk * a.vp * kC;
+  const E *do_rows = static_cast<const E *>(a.dout) + gb * a.vdim;
+  const long long so = (long long)a.hv * a.vdim;
   // the largest row scales of S, dS and dS', to which all rows' are taken
   const float *row_scales[3] = {a.scales + chunk * a.vp, a.dscales + slot * a.vp, a.dscales + (slot + 1) * a.vp};
   float big[3];
 #pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    float x = 0.f;
-    for (int j = lane; j < a.vp; j += 32) x = fmaxf(x, row_scales[i][j]);
-    big[i] = x;
-  }
+  for (int i = 0; i < 3; ++i)
+    big[i] = reduce_strided<false>(row_scales[i] + lane, (a.vp - lane + 31) / 32, 32);
   if (tid < kTokenMaxes * kC) {
     const float *m = a.token_maxes + (chunk * kTokenMaxes + tid / kC) * steps * kC + tid % kC;
-    float x = 0.f;
-#pragma unroll 4
-    for (int j = 0; j < steps; ++j) x = fmaxf(x, m[j * kC]);
-    w_inv[tid] = scale_for(x).inv;
+    w_inv[tid] = scale_for(reduce_strided<false>(m, steps, kC)).inv;
   } else if (tid < kTokenMaxes * kC + kC) {
     const int t = tid - kTokenMaxes * kC;
     const float2 x = a.gsum[chunk * kC + t];
     g_hi[t] = x.x;
     g_lo[t] = x.y;
-    const float *m = a.vdv + chunk * steps * kC + t;
-    float s = 0.f;
-#pragma unroll 4
-    for (int j = 0; j < steps; ++j) s += m[j * kC];
-    vdv[t] = s;
+    vdv[t] = reduce_strided<true>(a.vdv + chunk * steps * kC + t, steps, kC);
   }
 #pragma unroll
   for (int i = 0; i < 3; ++i)
@@ -542,14 +565,16 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
   for (int step = 0; step < steps; ++step) {
     const int v0 = step * 16, local = v0 % VB;
     if (local == 0) {
-      if (v0 > 0) __syncthreads();
       const int rows = min(VB, a.vp - v0);
-      split_tokens<VB, kThreads>(smem + L::kW, smem + L::kW + VB * kC * 2, a.ws + (chunk * a.vp + v0) * kC, rows,
-                                 w_inv, tid);
-      split_tokens<VB, kThreads>(smem + L::kDR, smem + L::kDR + VB * kC * 2, a.drs + (chunk * a.vp + v0) * kC,
-                                 rows, dr_inv, tid);
-      split_dout<E, VB, NP, kThreads>(smem + L::kDO, static_cast<const E *>(a.dout) + (gb * a.vdim + v0),
-                                      (long long)a.hv * a.vdim, live, a.vdim - v0, do_inv, tid);
+      if (v0 > 0) __syncthreads();  // all are done with the block before
+      TokenTile<VB, kThreads> w_tile, dr_tile;
+      DoutTile<E, VB, NP, kThreads> do_tile;
+      w_tile.load(w_rows + v0 * kC, rows, tid);
+      dr_tile.load(dr_rows + v0 * kC, rows, tid);
+      do_tile.load(do_rows + v0, so, live, a.vdim - v0, tid);
+      w_tile.store(smem + L::kW, smem + L::kW + VB * kC * 2, w_inv, tid);
+      dr_tile.store(smem + L::kDR, smem + L::kDR + VB * kC * 2, dr_inv, tid);
+      do_tile.store(smem + L::kDO, do_inv, tid);
 #pragma unroll
       for (int i = 0; i < 3; ++i)
         if (tid < rows) rho[i * VB + tid] = row_scales[i][v0 + tid] * inverse_pow2(big[i]);
