@@ -29,36 +29,45 @@
 namespace rqf {
 namespace delta {
 
-template <typename E, int KD, int W>
+template <typename E, int KD, int W, bool OUT>
 __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) {
   constexpr int NP = Elem<E>::kParts;
   using St = Stage<KD, NP>;
   using Tile = WarpTile<E>;
   extern __shared__ __align__(128) unsigned char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, c = lane & 3;
-  const int blocks = (a.vp / 16 + W - 1) / W;
-  const long long bh = blockIdx.x / blocks;
-  const int b = (int)(bh / a.hv), h = (int)(bh % a.hv), hk = h / a.rep;
-  const int w = (int)(blockIdx.x % blocks) * W + warp;
+  const unsigned blocks = (a.vp / 16 + W - 1) / W, spans = OUT ? a.segs : a.segs - 1;
+  const unsigned which = blockIdx.x / blocks, head = which / spans;
+  const int seg = (int)(which - head * spans) + (OUT ? 0 : 1);  // the first one's start is nobody's end
+  const long long bh = head;
+  const int b = (int)(head / (unsigned)a.hv), h = (int)(head - b * (unsigned)a.hv), hk = h / a.rep;
+  const int w = (int)(blockIdx.x - which * blocks) * W + warp;
   const int v0 = w * 16;
   const bool on = v0 < a.vp;
   const int cols = min(16, a.vdim - v0);
-  const long long len = row_length(a, b);
-  const int chunks = (int)((len + kC - 1) / kC);
-  const long long kv_first = ((long long)b * a.hk + hk) * a.n_chunks, first = bh * a.n_chunks;
-  const long long slot = bh * (a.n_chunks + 1);
+  const long long row_len = row_length(a, b);
+  const int row_chunks = (int)((row_len + kC - 1) / kC);
+  const int n0 = seg * a.seg_chunks;
+  const int chunks = max(0, min(row_chunks, n0 + a.seg_chunks) - n0);
+  const long long len = row_len - (long long)n0 * kC, left = a.time - (long long)n0 * kC;
+  const long long kv_first = ((long long)b * a.hk + hk) * a.n_chunks + n0, first = bh * a.n_chunks + n0;
+  const long long slot = bh * (a.n_chunks + 1) + n0;
   const uint32_t base = smem_u32(smem);
   unsigned char *mine = smem + 2 * St::kBytes + warp * kC * 16 * sizeof(E);
   const uint32_t tile = smem_u32(mine);
-  const E *v = static_cast<const E *>(a.v) + b * a.sv.b + h * a.sv.h + v0;
+  const E *v = static_cast<const E *>(a.v) + b * a.sv.b + (long long)n0 * kC * a.sv.t + h * a.sv.h + v0;
   const long long so = (long long)a.hv * a.vdim;  // do and dv are dense
-  const long long at = ((long long)b * a.time * a.hv + h) * a.vdim + v0;
+  const long long at = (((long long)b * a.time + (long long)n0 * kC) * a.hv + h) * a.vdim + v0;
   const E *dout = static_cast<const E *>(a.dout) + at;
   E *dv = static_cast<E *>(a.dv) + at;
 
   float S[KD / 8][4];  // dS'
-  load_state<KD>(a.dsT ? a.dsT + bh * a.kdim * a.vdim : nullptr, on ? v0 : a.vdim, a.kdim, a.vdim, lane,
-                 S);
+  {
+    const float *from = seg == a.segs - 1 ? (a.dsT ? a.dsT + bh * a.kdim * a.vdim : nullptr)
+                        : OUT             ? a.grad_starts + (bh * a.segs + seg) * a.kdim * a.vdim
+                                          : nullptr;
+    load_state<KD>(from, a.vdim, on ? v0 : a.vdim, a.kdim, a.vdim, lane, S);
+  }
 
   __shared__ __align__(8) uint64_t bars[2];
   const uint32_t bar = smem_u32(bars);
@@ -91,23 +100,23 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
       row_max(S, m0, m1);
       const float big0 = m0, big1 = m1;
       const Scale s0 = scale_for(m0), s1 = scale_for(m1);
-      save_scales(a.dscales + (slot + n + 1) * a.vp + v0, m0, m1, lane);
+      if (OUT) save_scales(a.dscales + (slot + n + 1) * a.vp + v0, m0, m1, lane);
       __half *keep = a.dstates + ((slot + n + 1) * a.vp + v0) * 2 * KD;
       float du[8][4], dr[8][4], x[8][4];
       zero(dr);  // k dS' first
 #pragma unroll
       for (int ks = 0; ks < KD / 16; ++ks) {
         split_frag(S, ks, s0.mul, s1.mul, hi, lo);
-        save_frag<KD>(keep, ks, lane, hi, lo);
+        if (OUT) save_frag<KD>(keep, ks, lane, hi, lo);
         step_rows<KD, NP>(dr, hi, lo, st + St::kK, kC * KD * 2, ks, 0, lane);
       }
       copy_wait<0>();
       __syncwarp();
       Tile::get(tile, mine, lane, x);
       __syncwarp();  // v takes the place of do
-      Tile::load(tile, v + t0 * a.sv.t, a.sv.t, (int)min((long long)kC, len - t0), cols, lane);
+      if (OUT) Tile::load(tile, v + t0 * a.sv.t, a.sv.t, (int)min((long long)kC, len - t0), cols, lane);
       copy_commit();
-      save_token_max(a.token_maxes, first + n, kTokenDO, a.vp / 16, w, x, lane);
+      if (OUT) save_token_max(a.token_maxes, first + n, kTokenDO, a.vp / 16, w, x, lane);
       Scale x0, x1;
       {
         float y[8][4];
@@ -170,31 +179,33 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
         du[nt][2] = f.x * dr[nt][2];
         du[nt][3] = f.y * dr[nt][3];
       }
-      save_rows(a.drs + ((first + n) * a.vp + v0) * kC, lane, du);  // dr with the keys' factors
-      save_token_max(a.token_maxes, first + n, kTokenDR, a.vp / 16, w, du, lane);
+      if (OUT) {
+        save_rows(a.drs + ((first + n) * a.vp + v0) * kC, lane, du);  // dr with the keys' factors
+        save_token_max(a.token_maxes, first + n, kTokenDR, a.vp / 16, w, du, lane);
 #pragma unroll
-      for (int nt = 0; nt < 8; ++nt) {
-        const float2 be = *reinterpret_cast<const float2 *>(vec + kRowBeta * kC + nt * 8 + 2 * c);
-        du[nt][0] *= be.x;
-        du[nt][1] *= be.y;
-        du[nt][2] *= be.x;
-        du[nt][3] *= be.y;
+        for (int nt = 0; nt < 8; ++nt) {
+          const float2 be = *reinterpret_cast<const float2 *>(vec + kRowBeta * kC + nt * 8 + 2 * c);
+          du[nt][0] *= be.x;
+          du[nt][1] *= be.y;
+          du[nt][2] *= be.x;
+          du[nt][3] *= be.y;
+        }
+        copy_wait<0>();
+        __syncwarp();
+        {
+          float y[8][4], m[8][2];
+          Tile::get(tile, mine, lane, y);
+#pragma unroll
+          for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) m[nt][e] = fmaf(y[nt][e], du[nt][e], y[nt][e + 2] * du[nt][e + 2]);
+          save_tokens<true>(a.vdv + ((first + n) * (a.vp / 16) + w) * kC, m, lane);
+        }
+        __syncwarp();
+        Tile::put(mine, lane, du);
+        __syncwarp();
+        Tile::store(mine, dv + t0 * so, so, (int)min((long long)kC, left - t0), cols, lane);
       }
-      copy_wait<0>();
-      __syncwarp();
-      {
-        float y[8][4], m[8][2];
-        Tile::get(tile, mine, lane, y);
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) m[nt][e] = fmaf(y[nt][e], du[nt][e], y[nt][e + 2] * du[nt][e + 2]);
-        save_tokens<true>(a.vdv + ((first + n) * (a.vp / 16) + w) * kC, m, lane);
-      }
-      __syncwarp();
-      Tile::put(mine, lane, du);
-      __syncwarp();
-      Tile::store(mine, dv + t0 * so, so, (int)min((long long)kC, a.time - t0), cols, lane);
       __syncwarp();
       if (n > 0) Tile::load(tile, dout + (t0 - kC) * so, so, kC, cols, lane);
 
@@ -245,7 +256,11 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
   }
   copy_wait<0>();
   if (!on) return;
-  if (chunks > 0) {  // the cotangent of the state that enters the first chunk
+  if (!OUT) {
+    store_state<KD>(a.grad_ends + (bh * a.segs + seg) * a.kdim * a.vp, a.vp, v0, a.kdim, a.vp, lane, S);
+    return;
+  }
+  if (seg == 0 && chunks > 0) {  // the cotangent of the state that enters the first chunk
     float m0, m1;
     row_max(S, m0, m1);
     const Scale s0 = scale_for(m0), s1 = scale_for(m1);
@@ -257,10 +272,11 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
       save_frag<KD>(a.dstates + (slot * a.vp + v0) * 2 * KD, ks, lane, hi, lo);
     }
   }
-  if (a.ds0 != nullptr)
-    store_state<KD>(a.ds0 + bh * a.kdim * a.vdim, v0, a.kdim, a.vdim, lane, S);
+  if (a.ds0 != nullptr && seg == 0)
+    store_state<KD>(a.ds0 + bh * a.kdim * a.vdim, a.vdim, v0, a.kdim, a.vdim, lane, S);
   constexpr int kPer = 16 / sizeof(E), kPieces = 16 / kPer;
-  for (long long t = (long long)chunks * kC + lane / kPieces; t < a.time; t += 32 / kPieces)
+  const long long stop = min(left, (long long)a.seg_chunks * kC);
+  for (long long t = (long long)chunks * kC + lane / kPieces; t < stop; t += 32 / kPieces)
     if ((lane % kPieces) * kPer < cols)
       *reinterpret_cast<uint4 *>(dv + t * so + (lane % kPieces) * kPer) = make_uint4(0, 0, 0, 0);
 }

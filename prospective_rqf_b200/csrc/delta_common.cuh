@@ -319,8 +319,11 @@ struct Args {
   float scale;
   int batch, hk, hv, rep, kdim, vdim, vp;
   long long time;
-  int n_chunks;   // chunks of this call's span
-  int n_first;    // the first of them
+  int n_chunks;
+  // the sequence in segs spans of seg_chunks chunks (delta_scan.cuh)
+  int segs, seg_chunks, kp;  // kp: kdim in whole 16s
+  float *ends, *starts;      // (row, span, K, vp + kp) and (row, span, K, V)
+  float *grad_ends, *grad_starts;  // (row, span, K, vp) and (row, span, K, V)
   // workspace and saved context; the tiles in tile_at's order
   __half *khat, *qhat, *tmat, *pmat;
   float *kfac, *qfac, *vec;

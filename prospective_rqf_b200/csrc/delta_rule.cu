@@ -25,9 +25,20 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 struct Sizes {
-  int64_t chunks, bhn, bkn, vp;
-  int kd, parts;
+  int64_t chunks, bhn, bkn, vp, kp;
+  int kd, parts, segs, seg_chunks;
 };
+
+// Spans of the sequence.  A span costs its chunks twice (once for its ends, with K more columns,
+// once proper), so cutting pays where rows x columns of 16 leave most of the 592 schedulers idle:
+// three spans at least, each of four chunks at least.
+void cut(int64_t warps, Sizes *s) {
+  int64_t n = warps > 0 ? 592 / warps : 1;
+  if (n > s->chunks / 4) n = s->chunks / 4;
+  if (n < 3) n = 1;
+  s->seg_chunks = (int)ceil_div(s->chunks, n);
+  s->segs = s->chunks > 0 ? (int)ceil_div(s->chunks, s->seg_chunks) : 1;
+}
 
 // RQF_OK and the derived sizes, or why the shape is refused.
 int sizes_of(const rqf_delta_problem *p, Sizes *s) {
@@ -46,12 +57,14 @@ int sizes_of(const rqf_delta_problem *p, Sizes *s) {
   // every grid is a product of these
   if (p->batch > kMaxGrid || p->value_heads > kMaxGrid || p->value_dim > kMaxGrid || s->chunks > kMaxGrid)
     return RQF_ERR_SHAPE;
-  const double grid = (double)p->batch * (double)p->value_heads;
-  if (grid * (double)(s->chunks > 0 ? s->chunks : 1) > (double)kMaxGrid ||
-      grid * (double)(s->vp / 16) > (double)kMaxGrid)
+  const double heads = (double)p->batch * (double)p->value_heads;
+  if (heads * (double)(s->chunks > 0 ? s->chunks : 1) > (double)kMaxGrid ||
+      heads * (double)(s->vp / 16) > (double)kMaxGrid)
     return RQF_ERR_SHAPE;
   s->bhn = p->batch * p->value_heads * s->chunks;
   s->bkn = p->batch * p->key_heads * s->chunks;
+  s->kp = ceil_div(p->key_dim, 16) * 16;
+  cut(p->batch * p->value_heads * (s->vp / 16), s);
   return RQF_OK;
 }
 
@@ -68,8 +81,13 @@ struct Carver {
 
 // What the forward leaves: the chunks' state-free part, and with `save` what
 // the backward needs besides.
-size_t carve_context(void *buffer, const Sizes &s, bool save, Args *a) {
+size_t carve_context(void *buffer, const rqf_delta_problem *p, const Sizes &s, bool save, Args *a) {
   Carver c{static_cast<unsigned char *>(buffer)};
+  if (s.segs > 1) {
+    const size_t spans = (size_t)p->batch * p->value_heads * s.segs * p->key_dim;
+    c.take(a->ends, spans * (s.vp + s.kp));
+    c.take(a->starts, spans * p->value_dim);
+  }
   c.take(a->khat, (size_t)s.bkn * s.parts * kC * s.kd);
   c.take(a->qhat, (size_t)s.bkn * s.parts * kC * s.kd);
   c.take(a->kfac, (size_t)s.bkn * kC);
@@ -94,6 +112,11 @@ size_t carve_workspace(void *buffer, const rqf_delta_problem *p, const Sizes &s,
   c.take(a->dscales, slots * s.vp);
   c.take(a->vdv, (size_t)s.bhn * (s.vp / 16) * kC);
   c.take(a->drs, (size_t)s.bhn * s.vp * kC);
+  if (s.segs > 1) {
+    const size_t spans = (size_t)p->batch * p->value_heads * s.segs * p->key_dim;
+    c.take(a->grad_ends, spans * s.vp);
+    c.take(a->grad_starts, spans * p->value_dim);
+  }
   a->dq_part = a->dk_part = nullptr;
   if (p->value_heads != p->key_heads) {
     const size_t n = (size_t)p->batch * p->time * p->value_heads * p->key_dim;
@@ -115,6 +138,7 @@ void common_args(const rqf_delta_problem *p, const Sizes &s, Args *a) {
   a->batch = (int)p->batch, a->hk = (int)p->key_heads, a->hv = (int)p->value_heads;
   a->rep = a->hv / a->hk, a->kdim = (int)p->key_dim, a->vdim = (int)p->value_dim, a->vp = (int)s.vp;
   a->time = p->time, a->n_chunks = (int)s.chunks;
+  a->segs = s.segs, a->seg_chunks = s.seg_chunks, a->kp = (int)s.kp;
 }
 
 int check_inputs(const rqf_delta_problem *p, const void *q, const void *k, const void *v, const float *g,
@@ -136,48 +160,55 @@ int launch(F kernel, int64_t grid, int threads, size_t smem, const Args &a, cuda
   return cudaGetLastError() == cudaSuccess ? RQF_OK : RQF_ERR_LAUNCH;
 }
 
-// CTAs of the pass from chunk to chunk: four warps (64 columns of V) while
-// those are at most one to an SM, eight where there are more.  With eight the
-// chunk's tiles are loaded once for 128 columns and a scheduler has two warps.
-template <typename E, int KD>
-int scan_warps(const Args &a) {
-  constexpr bool fits = scan_smem<E, KD, 8>() <= kMaxSmem;
-  return fits && a.vp > 64 && (int64_t)a.batch * a.hv * ceil_div(a.vp, 64) > 148 ? 8 : 4;
+// A pass from chunk to chunk over `columns` of V (and of the identity) of `spans` spans: CTAs of
+// four warps (64 columns) while those are at most one to an SM, of eight where there are more.
+// With eight the chunk's tiles are loaded once for 128 columns and a scheduler has two warps.
+template <typename E, int KD, typename Four, typename Eight>
+int run_pass(Four four, Eight eight, int64_t spans, int64_t columns, const Args &a, cudaStream_t st) {
+  const int64_t rows = (int64_t)a.batch * a.hv * spans;
+  if constexpr (scan_smem<E, KD, 8>() <= kMaxSmem)
+    if (columns > 64 && rows * ceil_div(columns, 64) > 148)
+      return launch(eight, rows * ceil_div(columns, 128), 256, scan_smem<E, KD, 8>(), a, st);
+  return launch(four, rows * ceil_div(columns, 64), 128, scan_smem<E, KD, 4>(), a, st);
+}
+template <typename E, int KD, int PASS>
+int run_scan(const Args &a, cudaStream_t st) {
+  const bool ends = PASS == kEnds;
+  return run_pass<E, KD>(scan_kernel<E, KD, 4, PASS>, scan_kernel<E, KD, 8, PASS>, ends ? a.segs - 1 : a.segs,
+                         ends ? a.vp + a.kp : a.vp, a, st);
+}
+template <typename E, int KD, bool OUT>
+int run_scan_backward(const Args &a, cudaStream_t st) {
+  return run_pass<E, KD>(scan_backward_kernel<E, KD, 4, OUT>, scan_backward_kernel<E, KD, 8, OUT>,
+                         OUT ? a.segs : a.segs - 1, a.vp, a, st);
+}
+template <bool BACK>
+int run_combine(const Args &a, cudaStream_t st) {
+  combine_kernel<BACK><<<(unsigned)(a.batch * a.hv * (a.vp / 16)), kCombineThreads, 0, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? RQF_OK : RQF_ERR_LAUNCH;
 }
 
-template <typename E, int KD, int W>
-int run_scan(const Args &a, bool save, cudaStream_t st) {
-  const int64_t grid = (int64_t)a.batch * a.hv * ceil_div(a.vp / 16, W);
-  constexpr size_t smem = scan_smem<E, KD, W>();
-  return save ? launch(scan_kernel<E, KD, W, true>, grid, W * 32, smem, a, st)
-              : launch(scan_kernel<E, KD, W, false>, grid, W * 32, smem, a, st);
-}
 template <typename E, int KD>
 int run_forward(const Args &a, bool save, cudaStream_t st) {
-  constexpr int NP = Elem<E>::kParts;
-  if (a.n_chunks > 0) {
-    const int rc = launch(prep_kernel<E, KD>, (int64_t)a.batch * a.hv * a.n_chunks, kPrepThreads,
-                          prep_smem<KD, NP>(), a, st);
-    if (rc != RQF_OK) return rc;
+  int rc = RQF_OK;
+  if (a.n_chunks > 0)
+    rc = launch(prep_kernel<E, KD>, (int64_t)a.batch * a.hv * a.n_chunks, kPrepThreads,
+                prep_smem<KD, Elem<E>::kParts>(), a, st);
+  if (rc == RQF_OK && a.segs > 1) {
+    rc = run_scan<E, KD, kEnds>(a, st);
+    if (rc == RQF_OK) rc = run_combine<false>(a, st);
   }
-  if constexpr (scan_smem<E, KD, 8>() <= kMaxSmem)
-    if (scan_warps<E, KD>(a) == 8) return run_scan<E, KD, 8>(a, save, st);
-  return run_scan<E, KD, 4>(a, save, st);
-}
-template <typename E, int KD, int W>
-int run_scan_backward(const Args &a, cudaStream_t st) {
-  return launch(scan_backward_kernel<E, KD, W>, (int64_t)a.batch * a.hv * ceil_div(a.vp / 16, W), W * 32,
-                scan_smem<E, KD, W>(), a, st);
+  if (rc != RQF_OK) return rc;
+  return save ? run_scan<E, KD, kKeep>(a, st) : run_scan<E, KD, kOutput>(a, st);
 }
 template <typename E, int KD>
 int run_backward(const Args &a, cudaStream_t st) {
-  int rc;
-  if constexpr (scan_smem<E, KD, 8>() <= kMaxSmem) {
-    if (scan_warps<E, KD>(a) == 8) rc = run_scan_backward<E, KD, 8>(a, st);
-    else rc = run_scan_backward<E, KD, 4>(a, st);
-  } else {
-    rc = run_scan_backward<E, KD, 4>(a, st);
+  int rc = RQF_OK;
+  if (a.segs > 1) {
+    rc = run_scan_backward<E, KD, false>(a, st);
+    if (rc == RQF_OK) rc = run_combine<true>(a, st);
   }
+  if (rc == RQF_OK) rc = run_scan_backward<E, KD, true>(a, st);
   if (rc != RQF_OK || a.n_chunks == 0) return rc;
   rc = launch(gradient_kernel<E, KD>, (int64_t)a.batch * a.hv * a.n_chunks,
               Grad<E, KD>::kThreads, Grad<E, KD>::kBytes, a, st);
@@ -212,7 +243,7 @@ size_t rqf_gated_delta_context_bytes(const rqf_delta_problem *problem, int save)
   Sizes s;
   Args a{};
   if (sizes_of(problem, &s) != RQF_OK) return SIZE_MAX;
-  return carve_context(nullptr, s, save != 0, &a);
+  return carve_context(nullptr, problem, s, save != 0, &a);
 }
 
 size_t rqf_gated_delta_backward_workspace_bytes(const rqf_delta_problem *problem) {
@@ -237,7 +268,7 @@ int rqf_gated_delta_forward(const rqf_delta_problem *problem, const void *q, con
   common_args(problem, s, &a);
   a.q = q, a.k = k, a.v = v, a.g = log_decay, a.beta = beta, a.s0 = initial_state, a.o = o;
   a.sT = final_state;
-  carve_context(context, s, save != 0, &a);
+  carve_context(context, problem, s, save != 0, &a);
   return by_type(problem->dtype, s.kd, [&](auto e, auto kd) {
     return run_forward<decltype(e), decltype(kd)::value>(a, save != 0, reinterpret_cast<cudaStream_t>(stream));
   });
@@ -266,7 +297,7 @@ int rqf_gated_delta_backward(const rqf_delta_problem *problem, const void *v, co
   a.v = v, a.dout = grad_o, a.dsT = grad_final_state;
   a.dq = grad_q, a.dk = grad_k, a.dv = grad_v, a.dg = grad_log_decay, a.dbeta = grad_beta;
   a.ds0 = grad_initial_state;
-  carve_context(const_cast<void *>(context), s, true, &a);
+  carve_context(const_cast<void *>(context), problem, s, true, &a);
   carve_workspace(workspace, problem, s, &a);
   return by_type(problem->dtype, s.kd, [&](auto e, auto kd) {
     return run_backward<decltype(e), decltype(kd)::value>(a, reinterpret_cast<cudaStream_t>(stream));

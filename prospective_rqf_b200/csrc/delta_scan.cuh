@@ -11,6 +11,13 @@
 // dependent products of 64 x 64 x 128 at most, so what counts is the time from
 // one product's sums to the next one's operand.  Tiles come by bulk copies, one
 // chunk ahead.
+//
+// Where rows x columns give fewer warps than the schedulers, the sequence is cut
+// into spans that run side by side.  The state leaves a span as M S + N, so a
+// first pass takes each span from a state of 0 (N) and from the identity (M, K
+// more columns beside V's, with values of 0) without its output, combine_kernel
+// carries S from span to span, and the pass proper starts every span from there.
+// The cotangents go back the same way, dS = M^T dS' + N'.
 #pragma once
 
 #include "delta_common.cuh"
@@ -31,15 +38,23 @@ constexpr size_t scan_smem() {
   return 2 * (size_t)Stage<KD, Elem<E>::kParts>::kBytes + (size_t)W * kC * 16 * sizeof(E);
 }
 
-template <int KD, int NP>
+// What a pass is for.
+enum Pass {
+  kOutput,  // o and the last state
+  kKeep,    // and what the backward needs
+  kEnds     // each span's M and N alone
+};
+
+template <int KD, int NP, int PASS = kKeep>
 __device__ __forceinline__ void load_stage(uint32_t dst, const Args &a, long long kv_chunk,
                                            long long chunk, uint32_t bar) {
   using S = Stage<KD, NP>;
-  bar_expect(bar, S::kBytes);
+  constexpr int kSquares = 2 * kC * kC * 2;
+  bar_expect(bar, PASS == kEnds ? S::kBytes - S::kKq - kSquares : S::kBytes);
   bulk_load(dst + S::kK, a.khat + kv_chunk * NP * kC * KD, S::kKq, bar);
-  bulk_load(dst + S::kQ, a.qhat + kv_chunk * NP * kC * KD, S::kKq, bar);
-  bulk_load(dst + S::kT, a.tmat + chunk * 2 * kC * kC, 2 * kC * kC * 2, bar);
-  bulk_load(dst + S::kP, a.pmat + chunk * 2 * kC * kC, 2 * kC * kC * 2, bar);
+  if (PASS != kEnds) bulk_load(dst + S::kQ, a.qhat + kv_chunk * NP * kC * KD, S::kKq, bar);
+  bulk_load(dst + S::kT, a.tmat + chunk * 2 * kC * kC, kSquares, bar);
+  if (PASS != kEnds) bulk_load(dst + S::kP, a.pmat + chunk * 2 * kC * kC, kSquares, bar);
   bulk_load(dst + S::kV, a.vec + chunk * kVec * kC, kVec * kC * 4, bar);
 }
 
@@ -202,9 +217,10 @@ __device__ __forceinline__ void zero(float (&x)[NT][4]) {
     for (int j = 0; j < 4; ++j) x[i][j] = 0.f;
 }
 
-// The warp's 16 x KD state against a (K, V) matrix in global memory.
+// The warp's 16 x KD state against a matrix (K, ld) in global memory, of whose columns vdim are
+// the state's.
 template <int KD>
-__device__ __forceinline__ void load_state(const float *src, int v0, int kdim, int vdim, int lane,
+__device__ __forceinline__ void load_state(const float *src, int ld, int v0, int kdim, int vdim, int lane,
                                            float (&S)[KD / 8][4]) {
   const int g = lane >> 2, c = lane & 3;
 #pragma unroll
@@ -212,11 +228,11 @@ __device__ __forceinline__ void load_state(const float *src, int v0, int kdim, i
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int k = nt * 8 + 2 * c + (i & 1), v = v0 + g + (i >> 1) * 8;
-      S[nt][i] = src != nullptr && k < kdim && v < vdim ? src[(long long)k * vdim + v] : 0.f;
+      S[nt][i] = src != nullptr && k < kdim && v < vdim ? src[(long long)k * ld + v] : 0.f;
     }
 }
 template <int KD>
-__device__ __forceinline__ void store_state(float *dst, int v0, int kdim, int vdim, int lane,
+__device__ __forceinline__ void store_state(float *dst, int ld, int v0, int kdim, int vdim, int lane,
                                             const float (&S)[KD / 8][4]) {
   const int g = lane >> 2, c = lane & 3;
 #pragma unroll
@@ -224,8 +240,17 @@ __device__ __forceinline__ void store_state(float *dst, int v0, int kdim, int vd
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int k = nt * 8 + 2 * c + (i & 1), v = v0 + g + (i >> 1) * 8;
-      if (k < kdim && v < vdim) dst[(long long)k * vdim + v] = S[nt][i];
+      if (k < kdim && v < vdim) dst[(long long)k * ld + v] = S[nt][i];
     }
+}
+// Columns v0.. of the identity.
+template <int KD>
+__device__ __forceinline__ void identity_state(int v0, int lane, float (&S)[KD / 8][4]) {
+  const int g = lane >> 2, c = lane & 3;
+#pragma unroll
+  for (int nt = 0; nt < KD / 8; ++nt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) S[nt][i] = nt * 8 + 2 * c + (i & 1) == v0 + g + (i >> 1) * 8 ? 1.f : 0.f;
 }
 // Accumulator tiles to a [v][LD] buffer of 32-bit values, at the warp's rows.
 template <int NT>
@@ -289,33 +314,48 @@ __device__ __forceinline__ void save_token_max(float *maxes, long long chunk, in
   save_tokens<false>(maxes + ((chunk * kTokenMaxes + which) * warps + w) * kC, m, lane);
 }
 
-template <typename E, int KD, int W, bool SAVE>
+template <typename E, int KD, int W, int PASS>
 __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
+  constexpr bool SAVE = PASS == kKeep, OUT = PASS != kEnds;
   constexpr int NP = Elem<E>::kParts;
   using St = Stage<KD, NP>;
   using Tile = WarpTile<E>;
   extern __shared__ __align__(128) unsigned char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int c = lane & 3;
-  const int blocks = (a.vp / 16 + W - 1) / W;  // CTAs of a head
-  const long long bh = blockIdx.x / blocks;
-  const int b = (int)(bh / a.hv), h = (int)(bh % a.hv), hk = h / a.rep;
-  const int w = (int)(blockIdx.x % blocks) * W + warp;  // this warp's 16 columns of V
+  const unsigned blocks = ((OUT ? a.vp : a.vp + a.kp) / 16 + W - 1) / W;  // CTAs of a head's span
+  const unsigned spans = OUT ? a.segs : a.segs - 1;  // the last one's end is nobody's start
+  const unsigned at = blockIdx.x / blocks, head = at / spans;
+  const int seg = (int)(at - head * spans);
+  const long long bh = head;
+  const int b = (int)(head / (unsigned)a.hv), h = (int)(head - b * (unsigned)a.hv), hk = h / a.rep;
+  const int w = (int)(blockIdx.x - at * blocks) * W + warp;  // this warp's 16 columns of V
   const int v0 = w * 16;
-  const bool on = v0 < a.vp;
-  const int cols = min(16, a.vdim - v0);
-  const long long len = row_length(a, b);
-  const int chunks = (int)((len + kC - 1) / kC);
-  const long long kv_first = ((long long)b * a.hk + hk) * a.n_chunks, first = bh * a.n_chunks;
+  const bool identity = !OUT && v0 >= a.vp;
+  const bool on = identity ? seg > 0 && v0 < a.vp + a.kp : v0 < a.vp;
+  const int cols = identity ? 0 : min(16, a.vdim - v0);
+  const long long row_len = row_length(a, b);
+  const int row_chunks = (int)((row_len + kC - 1) / kC);
+  const int n0 = seg * a.seg_chunks;  // this span's first chunk
+  const int chunks = max(0, min(row_chunks, n0 + a.seg_chunks) - n0);
+  const long long len = row_len - (long long)n0 * kC;
+  const long long kv_first = ((long long)b * a.hk + hk) * a.n_chunks + n0, first = bh * a.n_chunks + n0;
   const uint32_t base = smem_u32(smem);
   unsigned char *mine = smem + 2 * St::kBytes + warp * kC * 16 * sizeof(E);
   const uint32_t tile = smem_u32(mine);
-  const E *v = static_cast<const E *>(a.v) + b * a.sv.b + h * a.sv.h + v0;
-  E *o = static_cast<E *>(a.o) + ((long long)b * a.time * a.hv + h) * a.vdim + v0;
-  const long long so = (long long)a.hv * a.vdim;
+  const E *v = static_cast<const E *>(a.v) + b * a.sv.b + (long long)n0 * kC * a.sv.t + h * a.sv.h + (identity ? 0 : v0);
+  const long long so = (long long)a.hv * a.vdim, left = a.time - (long long)n0 * kC;
+  E *o = OUT ? static_cast<E *>(a.o) + (((long long)b * a.time + (long long)n0 * kC) * a.hv + h) * a.vdim + v0 : nullptr;
 
   float S[KD / 8][4];
-  load_state<KD>(a.s0 ? a.s0 + bh * a.kdim * a.vdim : nullptr, on ? v0 : a.vdim, a.kdim, a.vdim, lane, S);
+  if (identity) {
+    identity_state<KD>(v0 - a.vp, lane, S);
+  } else {
+    const float *from = seg == 0 ? (a.s0 ? a.s0 + bh * a.kdim * a.vdim : nullptr)
+                        : OUT   ? a.starts + (bh * a.segs + seg) * a.kdim * a.vdim
+                                : nullptr;
+    load_state<KD>(from, a.vdim, on ? v0 : a.vdim, a.kdim, a.vdim, lane, S);
+  }
 
   __shared__ __align__(8) uint64_t bars[2];
   const uint32_t bar = smem_u32(bars);
@@ -324,7 +364,7 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
     bar_init(bar);
     bar_init(bar + 8);
     bars_ready();
-    if (chunks > 0) load_stage<KD, NP>(base, a, kv_first, first, bar);
+    if (chunks > 0) load_stage<KD, NP, PASS>(base, a, kv_first, first, bar);
   }
   if (chunks > 0 && on) Tile::load(tile, v, a.sv.t, (int)min((long long)kC, len), cols, lane);
   copy_commit();
@@ -336,8 +376,8 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
     wait(bar + (n & 1) * 8, (n >> 1) & 1);
     __syncthreads();  // all are done with the other stage
     if (tid == 0 && n + 1 < chunks)
-      load_stage<KD, NP>(base + ((n + 1) & 1) * St::kBytes, a, kv_first + n + 1, first + n + 1,
-                         bar + ((n + 1) & 1) * 8);
+      load_stage<KD, NP, PASS>(base + ((n + 1) & 1) * St::kBytes, a, kv_first + n + 1, first + n + 1,
+                               bar + ((n + 1) & 1) * 8);
     if (on) {
       float m0, m1;
       row_max(S, m0, m1);
@@ -354,7 +394,7 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
         split_frag(S, ks, s0.mul, s1.mul, hi, lo);
         if (SAVE) save_frag<KD>(keep, ks, lane, hi, lo);
         step_rows<KD, NP>(r, hi, lo, st + St::kK, kC * KD * 2, ks, 0, lane);
-        step_rows<KD, NP>(qs, hi, lo, st + St::kQ, kC * KD * 2, ks, 0, lane);
+        if (OUT) step_rows<KD, NP>(qs, hi, lo, st + St::kQ, kC * KD * 2, ks, 0, lane);
       }
       copy_wait<0>();  // v
       __syncwarp();
@@ -418,27 +458,29 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
         u[nt][2] *= be.x;
         u[nt][3] *= be.y;
       }
-      row_max(u, m0, m1);
-      x0 = scale_for(m0), x1 = scale_for(m1);
-      zero(y);
+      if (OUT) {
+        row_max(u, m0, m1);
+        x0 = scale_for(m0), x1 = scale_for(m1);
+        zero(y);
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        split_frag(u, ks, x0.mul, x1.mul, hi, lo);
-        step_rows<kC, 2>(y, hi, lo, st + St::kP, kC * kC * 2, ks, ks, lane);
-      }
+        for (int ks = 0; ks < 4; ++ks) {
+          split_frag(u, ks, x0.mul, x1.mul, hi, lo);
+          step_rows<kC, 2>(y, hi, lo, st + St::kP, kC * kC * 2, ks, ks, lane);
+        }
 #pragma unroll
-      for (int nt = 0; nt < 8; ++nt) {
-        const float2 p = *reinterpret_cast<const float2 *>(vec + kRowP * kC + nt * 8 + 2 * c);
-        const float2 q = *reinterpret_cast<const float2 *>(vec + kRowO * kC + nt * 8 + 2 * c);
-        y[nt][0] = p.x * (x0.inv * y[nt][0]) + q.x * (s0.inv * qs[nt][0]);
-        y[nt][1] = p.y * (x0.inv * y[nt][1]) + q.y * (s0.inv * qs[nt][1]);
-        y[nt][2] = p.x * (x1.inv * y[nt][2]) + q.x * (s1.inv * qs[nt][2]);
-        y[nt][3] = p.y * (x1.inv * y[nt][3]) + q.y * (s1.inv * qs[nt][3]);
+        for (int nt = 0; nt < 8; ++nt) {
+          const float2 p = *reinterpret_cast<const float2 *>(vec + kRowP * kC + nt * 8 + 2 * c);
+          const float2 q = *reinterpret_cast<const float2 *>(vec + kRowO * kC + nt * 8 + 2 * c);
+          y[nt][0] = p.x * (x0.inv * y[nt][0]) + q.x * (s0.inv * qs[nt][0]);
+          y[nt][1] = p.y * (x0.inv * y[nt][1]) + q.y * (s0.inv * qs[nt][1]);
+          y[nt][2] = p.x * (x1.inv * y[nt][2]) + q.x * (s1.inv * qs[nt][2]);
+          y[nt][3] = p.y * (x1.inv * y[nt][3]) + q.y * (s1.inv * qs[nt][3]);
+        }
+        __syncwarp();
+        Tile::put(mine, lane, y);
+        __syncwarp();
+        Tile::store(mine, o + t0 * so, so, (int)min((long long)kC, left - t0), cols, lane);
       }
-      __syncwarp();
-      Tile::put(mine, lane, y);
-      __syncwarp();
-      Tile::store(mine, o + t0 * so, so, (int)min((long long)kC, a.time - t0), cols, lane);
       __syncwarp();
       if (n + 1 < chunks)
         Tile::load(tile, v + (t0 + kC) * a.sv.t, a.sv.t, (int)min((long long)kC, len - t0 - kC),
@@ -479,13 +521,65 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
   }
   copy_wait<0>();
   if (!on) return;
-  if (a.sT != nullptr)
-    store_state<KD>(a.sT + bh * a.kdim * a.vdim, v0, a.kdim, a.vdim, lane, S);
-  // tokens past the row's end: zeros
+  if (!OUT) {
+    const int ld = a.vp + a.kp;
+    store_state<KD>(a.ends + (bh * a.segs + seg) * a.kdim * ld, ld, v0, a.kdim, ld, lane, S);
+    return;
+  }
+  if (a.sT != nullptr && seg == a.segs - 1)
+    store_state<KD>(a.sT + bh * a.kdim * a.vdim, a.vdim, v0, a.kdim, a.vdim, lane, S);
+  // this span's tokens past the row's end: zeros
   constexpr int kPer = 16 / sizeof(E), kPieces = 16 / kPer;
-  for (long long t = (long long)chunks * kC + lane / kPieces; t < a.time; t += 32 / kPieces)
+  const long long stop = min(left, (long long)a.seg_chunks * kC);
+  for (long long t = (long long)chunks * kC + lane / kPieces; t < stop; t += 32 / kPieces)
     if ((lane % kPieces) * kPer < cols)
       *reinterpret_cast<uint4 *>(o + t * so + (lane % kPieces) * kPer) = make_uint4(0, 0, 0, 0);
+}
+
+// The states that spans start from, S_{i+1} = M_i S_i + N_i from the first span's end on; with
+// BACK the cotangents that they end with, dS_i = M_i^T dS_{i+1} + N'_i from the last one's.  A CTA
+// has 16 columns of V of one head: a thread one row of K and 8 of the columns.
+constexpr int kCombineThreads = 256;
+template <bool BACK>
+__global__ void __launch_bounds__(kCombineThreads) combine_kernel(const Args a) {
+  __shared__ __align__(16) float S[128][16];
+  const int blocks = a.vp / 16, ld = a.vp + a.kp, K = a.kdim;
+  const long long bh = blockIdx.x / blocks;
+  const int v0 = (int)(blockIdx.x % blocks) * 16;
+  const int k = threadIdx.x >> 1, c0 = (threadIdx.x & 1) * 8;
+  const float *N = BACK ? a.grad_ends : a.ends;
+  float *to = BACK ? a.grad_starts : a.starts;
+  const int ldn = BACK ? a.vp : ld;
+  const int from = BACK ? a.segs - 1 : 0, step = BACK ? -1 : 1, stop = BACK ? 0 : a.segs - 1;
+  float x[8];
+  for (int i = from; i != stop; i += step) {
+    const long long at = bh * a.segs + i;
+    if (k < K) {
+      load8<float>(N + (at * K + k) * ldn + v0 + c0, x);
+      if (i != from) {
+        const float *M = a.ends + at * K * ld + a.vp + (BACK ? k : (long long)k * ld);
+#pragma unroll 8
+        for (int l = 0; l < K; ++l) {
+          const float m = M[BACK ? (long long)l * ld : l];
+          const float4 p = *reinterpret_cast<const float4 *>(&S[l][c0]);
+          const float4 q = *reinterpret_cast<const float4 *>(&S[l][c0 + 4]);
+          x[0] = fmaf(m, p.x, x[0]), x[1] = fmaf(m, p.y, x[1]);
+          x[2] = fmaf(m, p.z, x[2]), x[3] = fmaf(m, p.w, x[3]);
+          x[4] = fmaf(m, q.x, x[4]), x[5] = fmaf(m, q.y, x[5]);
+          x[6] = fmaf(m, q.z, x[6]), x[7] = fmaf(m, q.w, x[7]);
+        }
+      }
+    }
+    __syncthreads();
+    if (k < K) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        S[k][c0 + j] = x[j];
+        if (v0 + c0 + j < a.vdim) to[((at + step) * K + k) * a.vdim + v0 + c0 + j] = x[j];
+      }
+    }
+    __syncthreads();
+  }
 }
 
 }  // namespace delta

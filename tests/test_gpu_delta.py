@@ -88,6 +88,14 @@ def test_rows_of_unlike_lengths(dtype):
         assert not o[b, m:].any()
 
 
+@pytest.mark.parametrize("dtype,hv,K,V,T", [(F32, 1, 40, 24, 1000), (BF16, 2, 128, 128, 833), (F16, 2, 64, 72, 769)])
+@pytest.mark.parametrize("lengths", [None, [0, 1], [700, 64], [257, 769]])
+def test_few_rows_over_long_sequences(dtype, hv, K, V, T, lengths):
+    """Long sequences of few rows are cut into spans, of which short rows leave some empty."""
+    n = None if lengths is None else torch.tensor(lengths).cuda()
+    _check(inputs(2, T, 1, hv, K, V, dtype, decay=5.0), _state(2, hv, K, V), n)
+
+
 def test_lengths_out_of_range_are_taken_into_range():
     args = inputs(2, 70, 1, 1, 32, 32, F32)
     full = rqf.gated_delta_scan(*args, lengths=torch.tensor([70, 0]).cuda())
