@@ -19,49 +19,67 @@ namespace rqf {
 namespace delta {
 
 constexpr int kPrepThreads = 128;
-constexpr int kLdA = kC + 1;  // row of A and T in shared memory
+constexpr int kLdA = kC + 4;  // row of B and T' in shared memory, whole float4s
 
 template <int KD, int NP>
 constexpr size_t prep_smem() {
   const size_t tiles = 2 * (size_t)NP * kC * KD * sizeof(__half);
   const size_t squares = 2 * (size_t)kC * kLdA * sizeof(float);
-  return (tiles > squares ? tiles : squares) + kC * (sizeof(double) + 4 * sizeof(float));
+  return (tiles > squares ? tiles : squares) + kC * 5 * sizeof(float);
 }
 
-// q or k of one chunk: rows scaled by a power of two to halves, in shared
-// memory and, for one of the value heads that share them, in the workspace.
+// q or k of one chunk: rows scaled by a power of two to halves, in shared memory and, for one of
+// the value heads that share them, in the workspace.  All loads come before the first use: what a
+// chunk waits for is memory, and this is its only wait.
 template <typename E, int KD, int NP>
-__device__ __forceinline__ void prep_rows(const E *src, long long stride_t, int live, int kdim,
-                                          __half *tile, float *fac, __half *ghat, float *gfac) {
-  constexpr int kLanes = KD / 8;  // lanes of a row, eight elements each
-  const int piece = threadIdx.x % kLanes;
-#pragma unroll 2
-  for (int row = threadIdx.x / kLanes; row < kC; row += kPrepThreads / kLanes) {
-    float x[8];
+struct Rows {
+  static constexpr int kLanes = KD / 8;  // lanes of a row, eight elements each
+  static constexpr int kEach = kC * kLanes / kPrepThreads;
+  static constexpr int kWords = sizeof(E) == 4 ? 2 : 1;
+  uint4 raw[kEach][kWords];
+  __device__ __forceinline__ void load(const E *src, long long stride_t, int live, int kdim) {
+    const int piece = threadIdx.x % kLanes;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
-    if (row < live && piece * 8 < kdim) load8<E>(src + row * stride_t + piece * 8, x);
-    float m = 0.f;
+    for (int it = 0; it < kEach; ++it) {
+      const int row = threadIdx.x / kLanes + it * (kPrepThreads / kLanes);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[i]));
-#pragma unroll
-    for (int d = kLanes / 2; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    const Scale s = scale_for(m);
-    uint4 hi, lo;
-    split2(x[0] * s.mul, x[1] * s.mul, hi.x, lo.x);
-    split2(x[2] * s.mul, x[3] * s.mul, hi.y, lo.y);
-    split2(x[4] * s.mul, x[5] * s.mul, hi.z, lo.z);
-    split2(x[6] * s.mul, x[7] * s.mul, hi.w, lo.w);
-    *reinterpret_cast<uint4 *>(tile + tile_at<KD>(row, piece)) = hi;
-    if (NP == 2) *reinterpret_cast<uint4 *>(tile + kC * KD + tile_at<KD>(row, piece)) = lo;
-    if (piece == 0) fac[row] = s.inv;
-    if (ghat != nullptr) {
-      *reinterpret_cast<uint4 *>(ghat + tile_at<KD>(row, piece)) = hi;
-      if (NP == 2) *reinterpret_cast<uint4 *>(ghat + kC * KD + tile_at<KD>(row, piece)) = lo;
-      if (piece == 0) gfac[row] = s.inv;
+      for (int w = 0; w < kWords; ++w)
+        raw[it][w] = row < live && piece * 8 < kdim
+                         ? *reinterpret_cast<const uint4 *>(src + row * stride_t + piece * 8 + w * 4)
+                         : make_uint4(0, 0, 0, 0);
     }
   }
-}
+  __device__ __forceinline__ void store(__half *tile, float *fac, __half *ghat, float *gfac) {
+    const int piece = threadIdx.x % kLanes;
+#pragma unroll
+    for (int it = 0; it < kEach; ++it) {
+      const int row = threadIdx.x / kLanes + it * (kPrepThreads / kLanes);
+      float x[8], m = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = Elem<E>::get(reinterpret_cast<const E *>(&raw[it][0])[i]);
+        m = fmaxf(m, fabsf(x[i]));
+      }
+#pragma unroll
+      for (int d = kLanes / 2; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+      const Scale s = scale_for(m);
+      uint4 hi, lo;
+      split2(x[0] * s.mul, x[1] * s.mul, hi.x, lo.x);
+      split2(x[2] * s.mul, x[3] * s.mul, hi.y, lo.y);
+      split2(x[4] * s.mul, x[5] * s.mul, hi.z, lo.z);
+      split2(x[6] * s.mul, x[7] * s.mul, hi.w, lo.w);
+      const int at = tile_at<KD>(row, piece);
+      *reinterpret_cast<uint4 *>(tile + at) = hi;
+      if (NP == 2) *reinterpret_cast<uint4 *>(tile + kC * KD + at) = lo;
+      if (piece == 0) fac[row] = s.inv;
+      if (ghat != nullptr) {
+        *reinterpret_cast<uint4 *>(ghat + at) = hi;
+        if (NP == 2) *reinterpret_cast<uint4 *>(ghat + kC * KD + at) = lo;
+        if (piece == 0) gfac[row] = s.inv;
+      }
+    }
+  }
+};
 
 // acc += A(16 rows m0) B^T(64 rows) over KD, tiles [row][KD]; tiles above the
 // diagonal are left out.
@@ -97,7 +115,8 @@ __device__ __forceinline__ void store_square_row(const float *x_row, int row, in
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
     uint4 hi, lo;
-    const float *x = x_row + from + p * 8;
+    float x[8];
+    load8<float>(x_row + from + p * 8, x);
     split2(x[0] * mul, x[1] * mul, hi.x, lo.x);
     split2(x[2] * mul, x[3] * mul, hi.y, lo.y);
     split2(x[4] * mul, x[5] * mul, hi.z, lo.z);
@@ -119,6 +138,7 @@ __device__ __forceinline__ void merge_blocks(const float *A, float *T, const flo
   float x[kEach];
 #pragma unroll
   for (int i = 0; i < kEach; ++i) x[i] = A[(base + N + r0 + i) * kLdA + base + col];
+#pragma unroll 8
   for (int l = 0; l < N; ++l) {
     const float t = beta[base + l] * T[(base + l) * kLdA + base + col];
 #pragma unroll
@@ -127,6 +147,7 @@ __device__ __forceinline__ void merge_blocks(const float *A, float *T, const flo
 #pragma unroll
   for (int i = 0; i < kEach; ++i) T[(base + N + r0 + i) * kLdA + base + col] = x[i];
   __syncthreads();
+#pragma unroll 8
   for (int l = 0; l < N; ++l) {
     const float t = beta[base + N + l] * T[(base + N + l) * kLdA + base + col];
 #pragma unroll
@@ -147,50 +168,52 @@ __global__ void __launch_bounds__(kPrepThreads) prep_kernel(const Args a) {
   constexpr size_t kSquares = 2 * (size_t)kC * kLdA * sizeof(float);
   __half *kt = reinterpret_cast<__half *>(smem), *qt = kt + NP * kC * KD;
   float *A = reinterpret_cast<float *>(smem), *T = A + kC * kLdA;  // take the tiles' place
-  double *G = reinterpret_cast<double *>(smem + (kTiles > kSquares ? kTiles : kSquares));
-  float *beta = reinterpret_cast<float *>(G + kC), *kfac = beta + kC, *qfac = kfac + kC;
+  float *g_hi = reinterpret_cast<float *>(smem + (kTiles > kSquares ? kTiles : kSquares)), *g_lo = g_hi + kC;
+  float *beta = g_lo + kC, *kfac = beta + kC, *qfac = kfac + kC;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int n = blockIdx.x % a.n_chunks;
-  const long long bh = blockIdx.x / a.n_chunks;  // b Hv + h
-  const int b = (int)(bh / a.hv), h = (int)(bh % a.hv), hk = h / a.rep;
+  const unsigned head = blockIdx.x / (unsigned)a.n_chunks;  // b Hv + h
+  const int n = (int)(blockIdx.x - head * a.n_chunks);
+  const int b = (int)(head / (unsigned)a.hv), h = (int)(head - b * (unsigned)a.hv), hk = h / a.rep;
+  const long long bh = head;
   const long long t0 = (long long)n * kC, left = row_length(a, b) - t0;
   if (left <= 0) return;  // nothing reads a chunk past its row's end
   const int live = left < kC ? (int)left : kC;
 
-  // decays: running sums of g in 64 bits, since differences of them count
+  Rows<E, KD, NP> k_rows, q_rows;
+  k_rows.load(static_cast<const E *>(a.k) + b * a.sk.b + t0 * a.sk.t + hk * a.sk.h, a.sk.t, live, a.kdim);
+  q_rows.load(static_cast<const E *>(a.q) + b * a.sq.b + t0 * a.sq.t + hk * a.sq.h, a.sq.t, live, a.kdim);
+  // decays: running sums of g in 64 bits, since differences of them count; kept as two floats
   if (warp == 0) {
-    double s[2];
+    float g[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int t = 2 * lane + i;
-      float g = 0.f, be = 0.f;
+      float be = 0.f;
       if (t < live) {
-        g = a.g[b * a.sg.b + (t0 + t) * a.sg.t + h * a.sg.h];
+        g[i] = a.g[b * a.sg.b + (t0 + t) * a.sg.t + h * a.sg.h];
         be = a.beta[b * a.sb.b + (t0 + t) * a.sb.t + h * a.sb.h];
-        if (g < kMinDecay) g = kMinDecay;
       }
+      if (g[i] < kMinDecay) g[i] = kMinDecay;
       beta[t] = be;
-      s[i] = (double)g + (i ? s[0] : 0.0);
     }
-    double run = s[1];
+    const double pair = (double)g[0] + (double)g[1];
+    double run = pair;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const double up = __shfl_up_sync(0xffffffffu, run, d);
       if (lane >= d) run += up;
     }
-    const double before = run - s[1];
-    G[2 * lane] = before + s[0];
-    G[2 * lane + 1] = run;
+    const double first = run - pair + (double)g[0];
+    g_hi[2 * lane] = (float)first;
+    g_lo[2 * lane] = (float)(first - (float)first);
+    g_hi[2 * lane + 1] = (float)run;
+    g_lo[2 * lane + 1] = (float)(run - (float)run);
   }
   const long long kv_chunk = ((long long)b * a.hk + hk) * a.n_chunks + n;
   const bool keep = h % a.rep == 0;
-  prep_rows<E, KD, NP>(static_cast<const E *>(a.k) + b * a.sk.b + t0 * a.sk.t + hk * a.sk.h, a.sk.t,
-                       live, a.kdim, kt, kfac, keep ? a.khat + kv_chunk * NP * kC * KD : nullptr,
-                       a.kfac + kv_chunk * kC);
-  prep_rows<E, KD, NP>(static_cast<const E *>(a.q) + b * a.sq.b + t0 * a.sq.t + hk * a.sq.h, a.sq.t,
-                       live, a.kdim, qt, qfac, keep ? a.qhat + kv_chunk * NP * kC * KD : nullptr,
-                       a.qfac + kv_chunk * kC);
+  k_rows.store(kt, kfac, keep ? a.khat + kv_chunk * NP * kC * KD : nullptr, a.kfac + kv_chunk * kC);
+  q_rows.store(qt, qfac, keep ? a.qhat + kv_chunk * NP * kC * KD : nullptr, a.qfac + kv_chunk * kC);
   __syncthreads();
 
   float kk[8][4], qk[8][4];
@@ -202,19 +225,29 @@ __global__ void __launch_bounds__(kPrepThreads) prep_kernel(const Args a) {
   prep_gram<KD, NP>(smem_u32(qt), smem_u32(kt), warp, lane, qk);
   __syncthreads();
 
-  for (int i = tid; i < kC * kLdA; i += kPrepThreads) T[i] = 0.f;
+  for (int i = tid * 4; i < kC * kLdA; i += kPrepThreads * 4)
+    *reinterpret_cast<float4 *>(T + i) = make_float4(0.f, 0.f, 0.f, 0.f);
   const int g = lane >> 2, c = lane & 3;
   float m[2] = {0.f, 0.f};
+  {
+    const int i0 = warp * 16 + g;
+    const float gh[2] = {g_hi[i0], g_hi[i0 + 8]}, gl[2] = {g_lo[i0], g_lo[i0 + 8]};
+    const float kf[2] = {kfac[i0], kfac[i0 + 8]}, qf[2] = {a.scale * qfac[i0], a.scale * qfac[i0 + 8]};
 #pragma unroll
-  for (int nt = 0; nt < 8; ++nt) {
-    if (nt > 2 * warp + 1) continue;
+    for (int nt = 0; nt < 8; ++nt) {
+      if (nt > 2 * warp + 1) continue;
+      const int j = nt * 8 + 2 * c;
+      const float2 hj = *reinterpret_cast<const float2 *>(g_hi + j), lj = *reinterpret_cast<const float2 *>(g_lo + j);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int i = warp * 16 + g + (e >> 1) * 8, j = nt * 8 + 2 * c + (e & 1);
-      const float d = i >= j ? expf((float)(G[i] - G[j])) : 0.f;
-      A[i * kLdA + j] = i > j ? kfac[i] * (kfac[i] * (d * kk[nt][e])) : 0.f;
-      qk[nt][e] = i >= j ? a.scale * d * qfac[i] * qk[nt][e] : 0.f;
-      m[e >> 1] = fmaxf(m[e >> 1], fabsf(qk[nt][e]));
+      for (int e = 0; e < 4; ++e) {
+        const int r = e >> 1, i = i0 + r * 8, jj = j + (e & 1);
+        const float d = __expf((gh[r] - (e & 1 ? hj.y : hj.x)) + (gl[r] - (e & 1 ? lj.y : lj.x)));
+        kk[nt][e] = i > jj ? kf[r] * (kf[r] * (d * kk[nt][e])) : 0.f;
+        qk[nt][e] = i >= jj ? qf[r] * (d * qk[nt][e]) : 0.f;
+        m[r] = fmaxf(m[r], fabsf(qk[nt][e]));
+      }
+      *reinterpret_cast<float2 *>(A + i0 * kLdA + j) = make_float2(kk[nt][0], kk[nt][1]);
+      *reinterpret_cast<float2 *>(A + (i0 + 8) * kLdA + j) = make_float2(kk[nt][2], kk[nt][3]);
     }
   }
   const long long chunk = bh * a.n_chunks + n;
@@ -245,20 +278,24 @@ __global__ void __launch_bounds__(kPrepThreads) prep_kernel(const Args a) {
   // T': diagonal blocks of 16 by substitution, then 32 and 64
   if (tid < kC) {
     const int base = tid & ~15, col = tid & 15;
-    float t[16];
+    float t[16], below[16];  // the column of I + diag(beta) T', and of T'
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
+      float row[16];
+#pragma unroll
+      for (int l = 0; l < i; l += 4)
+        *reinterpret_cast<float4 *>(row + l) = *reinterpret_cast<const float4 *>(A + (base + i) * kLdA + base + l);
       float x = 0.f, y = 0.f;
 #pragma unroll
       for (int l = 0; l < i; ++l) {
-        const float e = A[(base + i) * kLdA + base + l];
-        if (l & 1) y = fmaf(e, t[l], y);
-        else x = fmaf(e, t[l], x);
+        if (l & 1) y = fmaf(row[l], t[l], y);
+        else x = fmaf(row[l], t[l], x);
       }
-      // t: the column of I + diag(beta) T'
-      t[i] = i < col ? 0.f : i == col ? 1.f : -beta[base + i] * (x + y);
-      if (i > col) T[(base + i) * kLdA + base + col] = -(x + y);
+      below[i] = i > col ? -(x + y) : 0.f;
+      t[i] = i < col ? 0.f : i == col ? 1.f : beta[base + i] * below[i];
     }
+#pragma unroll
+    for (int i = 1; i < 16; ++i) T[(base + i) * kLdA + base + col] = below[i];
   }
   __syncthreads();
   merge_blocks<16>(A, T, beta, tid);
@@ -267,26 +304,26 @@ __global__ void __launch_bounds__(kPrepThreads) prep_kernel(const Args a) {
   {
     const int row = tid >> 1, from = (tid & 1) * 32;
     float mx = 0.f;
-#pragma unroll 8
-    for (int j = 0; j < 32; ++j) mx = fmaxf(mx, fabsf(T[row * kLdA + from + j]));
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float4 x = *reinterpret_cast<const float4 *>(T + row * kLdA + from + j);
+      mx = fmaxf(fmaxf(mx, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
+    }
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     const Scale s = scale_for(mx);
     store_square_row(T + row * kLdA, row, from, s.mul, a.tmat + chunk * 2 * kC * kC);
     if (from == 0) vec[kRowT * kC + row] = s.inv;
   }
   if (tid < kC) {
-    const double last = G[kC - 1];
-    const float eg = expf((float)G[tid]), ec = expf((float)(last - G[tid]));
+    const float eg = __expf(g_hi[tid] + g_lo[tid]);
+    const float ec = __expf((g_hi[kC - 1] - g_hi[tid]) + (g_lo[kC - 1] - g_lo[tid]));
     vec[kRowKS * kC + tid] = kfac[tid] * (kfac[tid] * eg);
     vec[kRowBeta * kC + tid] = beta[tid];
     vec[kRowK * kC + tid] = kfac[tid];
     vec[kRowO * kC + tid] = a.scale * eg * qfac[tid];
     vec[kRowEG * kC + tid] = eg;
     vec[kRowEC * kC + tid] = ec;
-    if (a.gsum != nullptr) {
-      const float hi = (float)G[tid];
-      a.gsum[chunk * kC + tid] = make_float2(hi, (float)(G[tid] - hi));
-    }
+    if (a.gsum != nullptr) a.gsum[chunk * kC + tid] = make_float2(g_hi[tid], g_lo[tid]);
   }
 }
 

@@ -538,45 +538,52 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
 
 // The states that spans start from, S_{i+1} = M_i S_i + N_i from the first span's end on; with
 // BACK the cotangents that they end with, dS_i = M_i^T dS_{i+1} + N'_i from the last one's.  A CTA
-// has 16 columns of V of one head: a thread one row of K and 8 of the columns.
-constexpr int kCombineThreads = 256;
+// has 16 columns of V of one head, a thread one row of K and 4 of the columns; what bounds it is
+// the chain of spans, each a wait for M, so 32 of M's values are loaded at once.
+constexpr int kCombineThreads = 512;
 template <bool BACK>
 __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const Args a) {
   __shared__ __align__(16) float S[128][16];
   const int blocks = a.vp / 16, ld = a.vp + a.kp, K = a.kdim;
   const long long bh = blockIdx.x / blocks;
   const int v0 = (int)(blockIdx.x % blocks) * 16;
-  const int k = threadIdx.x >> 1, c0 = (threadIdx.x & 1) * 8;
+  const int k = threadIdx.x >> 2, c0 = (threadIdx.x & 3) * 4;
   const float *N = BACK ? a.grad_ends : a.ends;
   float *to = BACK ? a.grad_starts : a.starts;
   const int ldn = BACK ? a.vp : ld;
   const int from = BACK ? a.segs - 1 : 0, step = BACK ? -1 : 1, stop = BACK ? 0 : a.segs - 1;
-  float x[8];
   for (int i = from; i != stop; i += step) {
     const long long at = bh * a.segs + i;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     if (k < K) {
-      load8<float>(N + (at * K + k) * ldn + v0 + c0, x);
-      if (i != from) {
-        const float *M = a.ends + at * K * ld + a.vp + (BACK ? k : (long long)k * ld);
-#pragma unroll 8
-        for (int l = 0; l < K; ++l) {
-          const float m = M[BACK ? (long long)l * ld : l];
-          const float4 p = *reinterpret_cast<const float4 *>(&S[l][c0]);
-          const float4 q = *reinterpret_cast<const float4 *>(&S[l][c0 + 4]);
-          x[0] = fmaf(m, p.x, x[0]), x[1] = fmaf(m, p.y, x[1]);
-          x[2] = fmaf(m, p.z, x[2]), x[3] = fmaf(m, p.w, x[3]);
-          x[4] = fmaf(m, q.x, x[4]), x[5] = fmaf(m, q.y, x[5]);
-          x[6] = fmaf(m, q.z, x[6]), x[7] = fmaf(m, q.w, x[7]);
+      x = *reinterpret_cast<const float4 *>(N + (at * K + k) * ldn + v0 + c0);
+      const float *M = a.ends + at * K * ld + a.vp + (BACK ? k : (long long)k * ld);
+      for (int l0 = 0; i != from && l0 < K; l0 += 32) {
+        float m[32];
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          if (BACK) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m[j + e] = l0 + j < K ? M[(long long)(l0 + j + e) * ld] : 0.f;
+          } else {
+            const float4 y = l0 + j < K ? *reinterpret_cast<const float4 *>(M + l0 + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+            m[j] = y.x, m[j + 1] = y.y, m[j + 2] = y.z, m[j + 3] = y.w;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          if (l0 + j >= K) continue;
+          const float4 p = *reinterpret_cast<const float4 *>(&S[l0 + j][c0]);
+          x.x = fmaf(m[j], p.x, x.x), x.y = fmaf(m[j], p.y, x.y);
+          x.z = fmaf(m[j], p.z, x.z), x.w = fmaf(m[j], p.w, x.w);
         }
       }
     }
     __syncthreads();
     if (k < K) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        S[k][c0 + j] = x[j];
-        if (v0 + c0 + j < a.vdim) to[((at + step) * K + k) * a.vdim + v0 + c0 + j] = x[j];
-      }
+      *reinterpret_cast<float4 *>(&S[k][c0]) = x;
+      if (v0 + c0 < a.vdim)
+        *reinterpret_cast<float4 *>(to + ((at + step) * K + k) * a.vdim + v0 + c0) = x;
     }
     __syncthreads();
   }
