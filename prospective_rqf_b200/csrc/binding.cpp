@@ -64,8 +64,8 @@ void same_cuda(std::initializer_list<const Tensor *> ts) {
   }
 }
 
-// A shape for a message.  Numbers go into messages as strings: the streams of
-// this module's libstdc++ and of torch's do not share their number formatting.
+// A shape for a message.  Numbers go into messages as strings: a number put into
+// torch's message stream from this module crashed.
 std::string text(at::IntArrayRef sizes) {
   std::string out = "(";
   for (size_t i = 0; i < sizes.size(); ++i) out += (i ? ", " : "") + std::to_string(sizes[i]);
@@ -302,71 +302,76 @@ PyObject *delta_step(PyObject *, PyObject *const *a, Py_ssize_t n) {
 // Whether the values fill one span of memory, in whatever order of the axes.
 bool filled(const Tensor &t) { return t.is_contiguous() || t.is_non_overlapping_and_dense(); }
 
+// The tensors of a Python sequence (or one tensor), which keeps them alive, and their table.
 struct List {
-  std::vector<Tensor> t;
+  PyObject *items = nullptr;
+  std::vector<const Tensor *> t;
   std::vector<void *> ptr;
   std::vector<int64_t> numel;
   std::vector<int> dtype;
-  void add(const Tensor &x) {
+  ~List() { Py_XDECREF(items); }
+  List() = default;
+  List(const List &) = delete;
+  void add(const Tensor &x, int type) {
     ptr.push_back(x.data_ptr());
     numel.push_back(x.numel());
-    dtype.push_back(dtype_of(x));
+    dtype.push_back(type);
   }
 };
 
-List list_arg(PyObject *o, const char *name) {
-  List out;
+void fill_list(List &out, PyObject *o, const char *name) {
   if (THPVariable_Check(o)) {
-    out.t.push_back(THPVariable_Unpack(o));
+    Py_INCREF(o);
+    out.items = o;
+    out.t.push_back(&THPVariable_Unpack(o));
   } else {
-    PyObject *items = PySequence_Fast(o, "a tensor or a sequence of tensors is wanted");
-    if (!items) throw python_error();
-    const Py_ssize_t n = PySequence_Fast_GET_SIZE(items);
+    out.items = PySequence_Fast(o, "a tensor or a sequence of tensors is wanted");
+    if (!out.items) throw python_error();
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(out.items);
+    PyObject **const item = PySequence_Fast_ITEMS(out.items);
     out.t.reserve(n);
     for (Py_ssize_t i = 0; i < n; ++i) {
-      PyObject *x = PySequence_Fast_GET_ITEM(items, i);
-      if (!THPVariable_Check(x)) {
-        PyErr_Format(PyExc_TypeError, "%s must hold tensors, got %s", name, Py_TYPE(x)->tp_name);
-        Py_DECREF(items);
+      if (!THPVariable_Check(item[i])) {
+        PyErr_Format(PyExc_TypeError, "%s must hold tensors, got %s", name, Py_TYPE(item[i])->tp_name);
         throw python_error();
       }
-      out.t.push_back(THPVariable_Unpack(x));
+      out.t.push_back(&THPVariable_Unpack(item[i]));
     }
-    Py_DECREF(items);
   }
   out.ptr.reserve(out.t.size());
   out.numel.reserve(out.t.size());
   out.dtype.reserve(out.t.size());
-  for (const Tensor &t : out.t) {
-    TORCH_CHECK_VALUE(dtype_of(t) >= 0, name, " must be float32, bfloat16, float16 or complex64, got ",
-                      t.scalar_type());
-    TORCH_CHECK_VALUE(!t.is_conj() && !t.is_neg(), name, " must not be lazy conjugates or negatives: resolve them first");
-    TORCH_CHECK(t.is_cuda(), "prospective_rqf_b200 runs on CUDA tensors only (no CPU fallback); got a tensor on ",
-                t.device());
-    TORCH_CHECK(t.get_device() == out.t[0].get_device(), "tensors on different devices: ", out.t[0].device(), " and ",
-                t.device());
+  for (const Tensor *t : out.t) {
+    TORCH_CHECK_VALUE(dtype_of(*t) >= 0, name, " must be float32, bfloat16, float16 or complex64, got ",
+                      t->scalar_type());
+    TORCH_CHECK_VALUE(!t->is_conj() && !t->is_neg(), name,
+                      " must not be lazy conjugates or negatives: resolve them first");
+    TORCH_CHECK(t->is_cuda(), "prospective_rqf_b200 runs on CUDA tensors only (no CPU fallback); got a tensor on ",
+                t->device());
+    TORCH_CHECK(t->get_device() == out.t[0]->get_device(), "tensors on different devices: ", out.t[0]->device(),
+                " and ", t->device());
   }
-  return out;
 }
 
 // grad_norm(grads) -> norm
 PyObject *grad_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
   if (!arity(n, 1, "grad_norm")) return nullptr;
   return guarded([&]() -> PyObject * {
-    List g = list_arg(a[0], "grads");
+    List g;
+    fill_list(g, a[0], "grads");
     if (g.t.empty()) return wrap(at::zeros({}));
-    const c10::cuda::CUDAGuard device(g.t[0].device());
+    const c10::cuda::CUDAGuard device(g.t[0]->device());
     std::vector<Tensor> copies;
-    for (const Tensor &t : g.t) {
-      if (filled(t)) {
-        g.add(t);
+    for (const Tensor *t : g.t) {
+      if (filled(*t)) {
+        g.add(*t, dtype_of(*t));
       } else {
-        copies.push_back(t.contiguous());
-        g.add(copies.back());
+        copies.push_back(t->contiguous());
+        g.add(copies.back(), dtype_of(*t));
       }
     }
     const int64_t count = static_cast<int64_t>(g.t.size());
-    Tensor norm = at::empty({}, g.t[0].options().dtype(at::kFloat));
+    Tensor norm = at::empty({}, g.t[0]->options().dtype(at::kFloat));
     Tensor scratch = scratch_of(rqf_grad_norm_scratch_bytes(count), norm);
     check(rqf_global_grad_norm(g.ptr.data(), g.numel.data(), g.dtype.data(), count, norm.data_ptr<float>(),
                                data(scratch), stream_on(norm)),
@@ -382,36 +387,38 @@ PyObject *clip_grads(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const double max_norm = PyFloat_AsDouble(a[1]);
     if (PyErr_Occurred()) throw python_error();
     TORCH_CHECK_VALUE(max_norm >= 0.0, "max_norm must not be negative, got ", std::to_string(max_norm));
-    List g = list_arg(a[0], "grads");
+    List g, out;
+    fill_list(g, a[0], "grads");
     const bool in_place = a[2] == Py_None;
-    List out;
     if (!in_place) {
-      out = list_arg(a[2], "out");
+      fill_list(out, a[2], "out");
       TORCH_CHECK_VALUE(out.t.size() == g.t.size(), std::to_string(g.t.size()), " gradients and ",
                         std::to_string(out.t.size()), " outputs");
     }
     if (g.t.empty()) return wrap(at::zeros({}));
-    const c10::cuda::CUDAGuard device(g.t[0].device());
+    const c10::cuda::CUDAGuard device(g.t[0]->device());
+    TORCH_CHECK(in_place || out.t[0]->get_device() == g.t[0]->get_device(), "tensors on different devices: ",
+                g.t[0]->device(), " and ", out.t[0]->device());
     std::vector<Tensor> copies;
     std::vector<std::pair<Tensor, Tensor>> back;
     std::vector<void *> to;
     to.reserve(g.t.size());
     for (size_t i = 0; i < g.t.size(); ++i) {
-      const Tensor &t = g.t[i];
-      const Tensor &o = in_place ? t : out.t[i];
+      const Tensor &t = *g.t[i];
+      const Tensor &o = in_place ? t : *out.t[i];
+      const int type = dtype_of(t);
       TORCH_CHECK_VALUE(in_place || (o.sizes() == t.sizes() && o.scalar_type() == t.scalar_type()), "out ",
                         o.scalar_type(), " ", text(o.sizes()), " does not match ", t.scalar_type(), " ",
                         text(t.sizes()));
-      TORCH_CHECK(in_place || o.get_device() == t.get_device(), "tensors on different devices: ", t.device(), " and ",
-                  o.device());
-      if (filled(o) && (in_place || (t.is_contiguous() && o.is_contiguous()) || t.strides() == o.strides())) {
-        g.add(t);
+      const bool dense = o.is_contiguous();
+      if ((dense && (in_place || t.is_contiguous())) || (filled(o) && t.strides() == o.strides())) {
+        g.add(t, type);
         to.push_back(o.data_ptr());
         continue;
       }
       // what does not lie in memory as its output does goes through a dense copy
       copies.push_back(t.clone(at::MemoryFormat::Contiguous));
-      g.add(copies.back());
+      g.add(copies.back(), type);
       to.push_back(copies.back().data_ptr());
       back.emplace_back(o, copies.back());
     }
@@ -424,12 +431,12 @@ PyObject *clip_grads(PyObject *, PyObject *const *a, Py_ssize_t n) {
                         "a tensor stands in grads twice: it would be scaled twice");
     }
     const int64_t count = static_cast<int64_t>(g.t.size());
-    Tensor norm = at::empty({}, g.t[0].options().dtype(at::kFloat));
+    Tensor norm = at::empty({}, g.t[0]->options().dtype(at::kFloat));
     Tensor scratch = scratch_of(rqf_grad_norm_scratch_bytes(count), norm);
     check(rqf_clip_grads(g.ptr.data(), to.data(), g.numel.data(), g.dtype.data(), count,
                          static_cast<float>(max_norm), norm.data_ptr<float>(), data(scratch), stream_on(norm)),
           "rqf_clip_grads");
-    for (const Tensor &o : in_place ? g.t : out.t) written(o);
+    for (const Tensor *o : in_place ? g.t : out.t) written(*o);
     for (auto &[o, c] : back) o.copy_(c);
     return wrap(norm);
   });

@@ -39,7 +39,7 @@ struct Table {
   int count, tiles;
   Entry e[N];
 };
-constexpr int kTables[3] = {32, 120, 960};  // 1, 4 and 30 KB of arguments
+constexpr int kTables[4] = {32, 120, 320, 960};  // 1, 4, 10 and 30 KB of arguments
 
 template <typename E>
 __device__ __forceinline__ float to_float(E x) {

@@ -2193,7 +2193,7 @@ int rqf_gated_delta_step(const rqf_delta_problem *problem, const void *q, const 
 // ------------------------------------------------ gradient norm and clipping
 namespace {
 
-constexpr int64_t kGradTable = gradnorm::kTables[2];
+constexpr int64_t kGradTable = gradnorm::kTables[3];
 
 int64_t grad_launches(int64_t n) { return n <= 0 ? 0 : ceil_div(n, kGradTable); }
 
@@ -2246,8 +2246,10 @@ int grad_launch(const void *const *grads, void *const *outs, const int64_t *nume
       rc = grad_pass<gradnorm::kTables[0]>(entries, count, (int)tiles, clip, to, *n_partials, max_norm, norm, st);
     else if (count <= gradnorm::kTables[1])
       rc = grad_pass<gradnorm::kTables[1]>(entries, count, (int)tiles, clip, to, *n_partials, max_norm, norm, st);
-    else
+    else if (count <= gradnorm::kTables[2])
       rc = grad_pass<gradnorm::kTables[2]>(entries, count, (int)tiles, clip, to, *n_partials, max_norm, norm, st);
+    else
+      rc = grad_pass<gradnorm::kTables[3]>(entries, count, (int)tiles, clip, to, *n_partials, max_norm, norm, st);
     if (rc != RQF_OK) return rc;
     sums += (int)(tiles < gradnorm::kMaxGrid ? tiles : gradnorm::kMaxGrid);
   }

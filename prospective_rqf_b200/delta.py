@@ -20,17 +20,22 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _abi, _timing
-from .ops import _done, _nbytes
+from .ops import _SYNC_CHECK, _nbytes
 
 __all__ = ["gated_delta_scan", "gated_delta_step"]
 
 
-def _timed(name, tensors, call):
-    """The call, under the active KernelTimer if there is one."""
+def _call(name, tensors, fn, *args):
+    """fn(*args), under the active KernelTimer if there is one and with the package's check of
+    device errors after it if that is on."""
     if _timing._ACTIVE is None:
-        return call()
-    with _timing.launch(name, tensors[0].numel(), _nbytes(*tensors)):
-        return call()
+        out = fn(*args)
+    else:
+        with _timing.launch(name, tensors[0].numel(), _nbytes(*tensors)):
+            out = fn(*args)
+    if _SYNC_CHECK:
+        _abi.check_device_errors(tensors[0].device)
+    return out
 
 
 class _GatedDeltaScan(torch.autograd.Function):
@@ -49,10 +54,9 @@ class _GatedDeltaScan(torch.autograd.Function):
     def backward(ctx, grad_o, grad_last):
         *inputs, context = ctx.saved_tensors
         need = ctx.needs_input_grad
-        grads = _timed("rqf_gated_delta_backward", inputs[:3], lambda: _abi.native().delta_backward(
-            *inputs, context, ctx.scale, grad_o, grad_last, need[5]))
-        _done(context.device)
-        dq, dk, dv, dg, db, ds0 = grads
+        dq, dk, dv, dg, db, ds0 = _call(
+            "rqf_gated_delta_backward", inputs[:3], _abi.native().delta_backward, *inputs, context,
+            ctx.scale, grad_o, grad_last, need[5])
         dg, db = dg.to(ctx.types[0]), db.to(ctx.types[1])
         return tuple(x if n else None for x, n in zip((dq, dk, dv, dg, db, ds0, None, None), need))
 
@@ -77,12 +81,10 @@ def gated_delta_scan(q, k, v, log_decay, beta, *, scale: float | None = None, in
     gradient is wanted, the states that enter each 64 tokens are kept for the backward."""
     args = (q, k, v, log_decay, beta, initial_state)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
-        o, last = _timed("rqf_gated_delta_forward", args[:3],
-                         lambda: _GatedDeltaScan.apply(*args, lengths, scale))
+        o, last = _call("rqf_gated_delta_forward", args[:3], _GatedDeltaScan.apply, *args, lengths, scale)
     else:
-        o, last, _ = _timed("rqf_gated_delta_forward", args[:3], lambda: _abi.native().delta_forward(
-            *args, lengths, scale, False))
-    _done(o.device)
+        o, last, _ = _call("rqf_gated_delta_forward", args[:3], _abi.native().delta_forward, *args,
+                           lengths, scale, False)
     return (o, last) if return_state else o
 
 
@@ -95,7 +97,5 @@ def gated_delta_step(q, k, v, log_decay, beta, state, *, slots=None, scale: floa
     are distinct integers; a negative one is an idle row, whose output is 0.  One past the pool
     is taken as idle too and raises from check_device_errors().  Returns o (batch, value_heads,
     V) in v's type.  No gradient is recorded."""
-    o = _timed("rqf_gated_delta_step", (q, k, v), lambda: _abi.native().delta_step(
-        q, k, v, log_decay, beta, state, slots, scale))
-    _done(o.device)
-    return o
+    return _call("rqf_gated_delta_step", (q, k, v), _abi.native().delta_step, q, k, v, log_decay, beta,
+                 state, slots, scale)
