@@ -29,6 +29,11 @@
 namespace rqf {
 namespace delta {
 
+template <typename E, int KD, int W>
+constexpr size_t backward_smem() {
+  return 2 * (size_t)Stage<KD, Elem<E>::kParts>::kBytes + (size_t)W * kC * 16 * sizeof(E);
+}
+
 template <typename E, int KD, int W, bool OUT>
 __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) {
   constexpr int NP = Elem<E>::kParts;

@@ -160,27 +160,32 @@ int launch(F kernel, int64_t grid, int threads, size_t smem, const Args &a, cuda
   return cudaGetLastError() == cudaSuccess ? RQF_OK : RQF_ERR_LAUNCH;
 }
 
-// A pass from chunk to chunk over `columns` of V (and of the identity) of `spans` spans: CTAs of
-// four warps (64 columns) while those are at most one to an SM, of eight where there are more.
-// With eight the chunk's tiles are loaded once for 128 columns and a scheduler has two warps.
-template <typename E, int KD, typename Four, typename Eight>
-int run_pass(Four four, Eight eight, int64_t spans, int64_t columns, const Args &a, cudaStream_t st) {
-  const int64_t rows = (int64_t)a.batch * a.hv * spans;
-  if constexpr (scan_smem<E, KD, 8>() <= kMaxSmem)
-    if (columns > 64 && rows * ceil_div(columns, 64) > 148)
-      return launch(eight, rows * ceil_div(columns, 128), 256, scan_smem<E, KD, 8>(), a, st);
-  return launch(four, rows * ceil_div(columns, 64), 128, scan_smem<E, KD, 4>(), a, st);
-}
+// A pass from chunk to chunk over `columns` of V (and of the identity): CTAs of four warps on the
+// states (64 columns) while those are at most one to an SM, of eight where there are more and they
+// fit.  With eight the chunk's tiles are loaded once for 128 columns and a scheduler has two warps.
+// With output four already are eight warps.
+bool eight_warps(int64_t rows, int64_t columns) { return columns > 64 && rows * ceil_div(columns, 64) > 148; }
+
 template <typename E, int KD, int PASS>
 int run_scan(const Args &a, cudaStream_t st) {
-  const bool ends = PASS == kEnds;
-  return run_pass<E, KD>(scan_kernel<E, KD, 4, PASS>, scan_kernel<E, KD, 8, PASS>, ends ? a.segs - 1 : a.segs,
-                         ends ? a.vp + a.kp : a.vp, a, st);
+  constexpr bool out = PASS != kEnds;
+  const int64_t rows = (int64_t)a.batch * a.hv * (out ? a.segs : a.segs - 1), columns = out ? a.vp : a.vp + a.kp;
+  using Eight = Layout<E, KD, 8, PASS>;
+  if constexpr (!out && Eight::kStages == 2)
+    if (eight_warps(rows, columns))
+      return launch(scan_kernel<E, KD, 8, PASS>, rows * ceil_div(columns, 128), Eight::kThreads, Eight::kBytes, a, st);
+  using Four = Layout<E, KD, 4, PASS>;
+  return launch(scan_kernel<E, KD, 4, PASS>, rows * ceil_div(columns, 64), Four::kThreads, Four::kBytes, a, st);
 }
 template <typename E, int KD, bool OUT>
 int run_scan_backward(const Args &a, cudaStream_t st) {
-  return run_pass<E, KD>(scan_backward_kernel<E, KD, 4, OUT>, scan_backward_kernel<E, KD, 8, OUT>,
-                         OUT ? a.segs : a.segs - 1, a.vp, a, st);
+  const int64_t rows = (int64_t)a.batch * a.hv * (OUT ? a.segs : a.segs - 1), columns = a.vp;
+  if constexpr (backward_smem<E, KD, 8>() <= kMaxSmem)
+    if (eight_warps(rows, columns))
+      return launch(scan_backward_kernel<E, KD, 8, OUT>, rows * ceil_div(columns, 128), 256,
+                    backward_smem<E, KD, 8>(), a, st);
+  return launch(scan_backward_kernel<E, KD, 4, OUT>, rows * ceil_div(columns, 64), 128,
+                backward_smem<E, KD, 4>(), a, st);
 }
 template <bool BACK>
 int run_combine(const Args &a, cudaStream_t st) {

@@ -4,7 +4,12 @@
 // never meet, so warps share only the chunk's tiles (k, q, T, P), and each
 // product's sums are laid out as the next one's left operand needs them:
 //
-//   (kS)^T = S^T k^T  ->  r^T  ->  w^T = (r / beta)^T + r^T T'^T, u = beta w  ->  o^T, S'^T += u^T k
+//   (kS)^T = S^T k^T  ->  r^T  ->  w^T = (r / beta)^T + r^T T'^T, u = beta w  ->  S'^T += u^T k
+//
+// and what hangs off that chain is a second warp's: it gets S's fragments and w by way of shared
+// memory and makes o = scale e^G q S + P u, and in training writes S and w out.  With all of it in
+// one warp a chunk of 64 x 128 x 128 took 7.5e3 cycles, 1.05e4 when S and w were kept, of which the
+// products fill 4e3.
 //
 // runs with no trip through shared memory.  That is why these products use
 // m16n8k16 and not tcgen05: the chain from one chunk to the next is three
@@ -33,17 +38,34 @@ struct Stage {
   static constexpr int kV = kP + 2 * kC * kC * 2;  // coefficient rows
   static constexpr int kBytes = kV + kVec * kC * 4;
 };
-template <typename E, int KD, int W>
-constexpr size_t scan_smem() {
-  return 2 * (size_t)Stage<KD, Elem<E>::kParts>::kBytes + (size_t)W * kC * 16 * sizeof(E);
-}
-
 // What a pass is for.
 enum Pass {
   kOutput,  // o and the last state
   kKeep,    // and what the backward needs
   kEnds     // each span's M and N alone
 };
+
+// Shared memory of a pass with W warps on the states: tiles (of two chunks where that fits), the
+// warps' tiles of v, and for a pass with output those of o and what the states' warps hand over.
+template <typename E, int KD, int W, int PASS>
+struct Layout {
+  static constexpr bool kOut = PASS != kEnds;
+  static constexpr int kStage = Stage<KD, Elem<E>::kParts>::kBytes;
+  static constexpr int kTile = kC * 16 * (int)sizeof(E);
+  // handed over by a warp: S as fragments, w as accumulators, the rows' largest magnitudes
+  static constexpr int kFrags = KD / 16 * 2 * 32 * 16, kW = 8 * 32 * 16, kHand = kFrags + kW + 16 * 4;
+  static constexpr int kRest = W * (kOut ? 2 * kTile + kHand : kTile);
+  static constexpr int kStages = 2 * kStage + kRest <= 227 * 1024 ? 2 : 1;
+  static constexpr int kV = kStages * kStage, kO = kV + W * kTile, kGive = kO + W * kTile;
+  static constexpr int kBytes = kV + kRest;
+  static constexpr int kThreads = (kOut ? 2 : 1) * W * 32;
+};
+
+// Pairs of warps: one arrives, the other waits.
+__device__ __forceinline__ void pair_arrive(int id) {
+  asm volatile("bar.arrive %0, 64;" ::"r"(id) : "memory");
+}
+__device__ __forceinline__ void pair_wait(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
 template <int KD, int NP, int PASS = kKeep>
 __device__ __forceinline__ void load_stage(uint32_t dst, const Args &a, long long kv_chunk,
@@ -315,21 +337,23 @@ __device__ __forceinline__ void save_token_max(float *maxes, long long chunk, in
 }
 
 template <typename E, int KD, int W, int PASS>
-__global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
+__global__ void __launch_bounds__(Layout<E, KD, W, PASS>::kThreads, 1) scan_kernel(const Args a) {
   constexpr bool SAVE = PASS == kKeep, OUT = PASS != kEnds;
   constexpr int NP = Elem<E>::kParts;
+  using L = Layout<E, KD, W, PASS>;
   using St = Stage<KD, NP>;
   using Tile = WarpTile<E>;
   extern __shared__ __align__(128) unsigned char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int c = lane & 3;
+  const int c = lane & 3, pair = warp % W;
+  const bool states = !OUT || warp < W;  // on the states, or on the output
   const unsigned blocks = ((OUT ? a.vp : a.vp + a.kp) / 16 + W - 1) / W;  // CTAs of a head's span
   const unsigned spans = OUT ? a.segs : a.segs - 1;  // the last one's end is nobody's start
   const unsigned at = blockIdx.x / blocks, head = at / spans;
   const int seg = (int)(at - head * spans);
   const long long bh = head;
   const int b = (int)(head / (unsigned)a.hv), h = (int)(head - b * (unsigned)a.hv), hk = h / a.rep;
-  const int w = (int)(blockIdx.x - at * blocks) * W + warp;  // this warp's 16 columns of V
+  const int w = (int)(blockIdx.x - at * blocks) * W + pair;  // this warp's 16 columns of V
   const int v0 = w * 16;
   const bool identity = !OUT && v0 >= a.vp;
   const bool on = identity ? seg > 0 && v0 < a.vp + a.kp : v0 < a.vp;
@@ -341,7 +365,11 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
   const long long len = row_len - (long long)n0 * kC;
   const long long kv_first = ((long long)b * a.hk + hk) * a.n_chunks + n0, first = bh * a.n_chunks + n0;
   const uint32_t base = smem_u32(smem);
-  unsigned char *mine = smem + 2 * St::kBytes + warp * kC * 16 * sizeof(E);
+  unsigned char *mine = smem + (states ? L::kV : L::kO) + pair * L::kTile;
+  unsigned char *give = smem + L::kGive + pair * L::kHand;
+  uint4 *frags = reinterpret_cast<uint4 *>(give) + lane;                    // [ks][hi, lo][lane]
+  float4 *w_tiles = reinterpret_cast<float4 *>(give + L::kFrags) + lane;    // [nt][lane]
+  float *row_maxes = reinterpret_cast<float *>(give + L::kFrags + L::kW);   // [row]
   const uint32_t tile = smem_u32(mine);
   const E *v = static_cast<const E *>(a.v) + b * a.sv.b + (long long)n0 * kC * a.sv.t + h * a.sv.h + (identity ? 0 : v0);
   const long long so = (long long)a.hv * a.vdim, left = a.time - (long long)n0 * kC;
@@ -350,7 +378,7 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
   float S[KD / 8][4];
   if (identity) {
     identity_state<KD>(v0 - a.vp, lane, S);
-  } else {
+  } else if (states) {
     const float *from = seg == 0 ? (a.s0 ? a.s0 + bh * a.kdim * a.vdim : nullptr)
                         : OUT   ? a.starts + (bh * a.segs + seg) * a.kdim * a.vdim
                                 : nullptr;
@@ -366,56 +394,61 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
     bars_ready();
     if (chunks > 0) load_stage<KD, NP, PASS>(base, a, kv_first, first, bar);
   }
-  if (chunks > 0 && on) Tile::load(tile, v, a.sv.t, (int)min((long long)kC, len), cols, lane);
+  if (states && chunks > 0 && on) Tile::load(tile, v, a.sv.t, (int)min((long long)kC, len), cols, lane);
   copy_commit();
   __syncthreads();
   for (int n = 0; n < chunks; ++n) {
-    const uint32_t st = base + (n & 1) * St::kBytes;
-    const float *vec = reinterpret_cast<const float *>(smem + (n & 1) * St::kBytes + St::kV);
+    const int stage = L::kStages == 2 ? n & 1 : 0;
+    const uint32_t st = base + stage * L::kStage;
+    const float *vec = reinterpret_cast<const float *>(smem + stage * L::kStage + St::kV);
     const long long t0 = (long long)n * kC;
-    wait(bar + (n & 1) * 8, (n >> 1) & 1);
-    __syncthreads();  // all are done with the other stage
-    if (tid == 0 && n + 1 < chunks)
-      load_stage<KD, NP, PASS>(base + ((n + 1) & 1) * St::kBytes, a, kv_first + n + 1, first + n + 1,
-                               bar + ((n + 1) & 1) * 8);
-    if (on) {
-      float m0, m1;
+    if (L::kStages == 2) {
+      wait(bar + stage * 8, (n >> 1) & 1);
+      __syncthreads();  // all are done with the other stage, and with what was handed over
+      if (tid == 0 && n + 1 < chunks)
+        load_stage<KD, NP, PASS>(base + (stage ^ 1) * L::kStage, a, kv_first + n + 1, first + n + 1,
+                                 bar + (stage ^ 1) * 8);
+    } else {
+      __syncthreads();
+      if (tid == 0 && n > 0) load_stage<KD, NP, PASS>(base, a, kv_first + n, first + n, bar);
+      wait(bar, n & 1);
+    }
+    if (!on) continue;
+    uint32_t hi[4], lo[4];
+    float m0, m1, y[8][4];
+    if (states) {
       row_max(S, m0, m1);
       const float big0 = m0, big1 = m1;
       const Scale s0 = scale_for(m0), s1 = scale_for(m1);
-      if (SAVE) save_scales(a.scales + (first + n) * a.vp + v0, m0, m1, lane);
-      __half *keep = SAVE ? a.states + ((first + n) * a.vp + v0) * 2 * KD : nullptr;
-      float r[8][4], qs[8][4];  // r without beta, from here to w
+      if (OUT && c == 0) row_maxes[lane >> 2] = m0, row_maxes[(lane >> 2) + 8] = m1;
+      float r[8][4], u[8][4];  // r without beta, from here to w
       zero(r);
-      zero(qs);
 #pragma unroll
       for (int ks = 0; ks < KD / 16; ++ks) {
-        uint32_t hi[4], lo[4];
         split_frag(S, ks, s0.mul, s1.mul, hi, lo);
-        if (SAVE) save_frag<KD>(keep, ks, lane, hi, lo);
+        if (OUT) {
+          frags[ks * 64] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          frags[ks * 64 + 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
         step_rows<KD, NP>(r, hi, lo, st + St::kK, kC * KD * 2, ks, 0, lane);
-        if (OUT) step_rows<KD, NP>(qs, hi, lo, st + St::kQ, kC * KD * 2, ks, 0, lane);
       }
+      if (OUT) pair_arrive(1 + pair);
       copy_wait<0>();  // v
       __syncwarp();
-      {
-        float x[8][4];
-        Tile::get(tile, mine, lane, x);
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt) {
-          const float2 f = *reinterpret_cast<const float2 *>(vec + kRowKS * kC + nt * 8 + 2 * c);
-          const float2 be = *reinterpret_cast<const float2 *>(vec + kRowK * kC + nt * 8 + 2 * c);
-          r[nt][0] = be.x * x[nt][0] - f.x * (s0.inv * r[nt][0]);
-          r[nt][1] = be.y * x[nt][1] - f.y * (s0.inv * r[nt][1]);
-          r[nt][2] = be.x * x[nt][2] - f.x * (s1.inv * r[nt][2]);
-          r[nt][3] = be.y * x[nt][3] - f.y * (s1.inv * r[nt][3]);
-        }
-      }
-      float u[8][4], y[8][4];
-      uint32_t hi[4], lo[4];
+      Tile::get(tile, mine, lane, y);
+      __syncwarp();
+      if (n + 1 < chunks)
+        Tile::load(tile, v + (t0 + kC) * a.sv.t, a.sv.t, (int)min((long long)kC, len - t0 - kC), cols, lane);
+      copy_commit();
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt) {
+        const float2 f = *reinterpret_cast<const float2 *>(vec + kRowKS * kC + nt * 8 + 2 * c);
+        const float2 k = *reinterpret_cast<const float2 *>(vec + kRowK * kC + nt * 8 + 2 * c);
         const float2 be = *reinterpret_cast<const float2 *>(vec + kRowBeta * kC + nt * 8 + 2 * c);
+        r[nt][0] = k.x * y[nt][0] - f.x * (s0.inv * r[nt][0]);
+        r[nt][1] = k.y * y[nt][1] - f.y * (s0.inv * r[nt][1]);
+        r[nt][2] = k.x * y[nt][2] - f.x * (s1.inv * r[nt][2]);
+        r[nt][3] = k.y * y[nt][3] - f.y * (s1.inv * r[nt][3]);
         y[nt][0] = be.x * r[nt][0];
         y[nt][1] = be.y * r[nt][1];
         y[nt][2] = be.x * r[nt][2];
@@ -436,64 +469,19 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
         u[nt][1] = fmaf(f.y * x0.inv, u[nt][1], r[nt][1]);
         u[nt][2] = fmaf(f.x * x1.inv, u[nt][2], r[nt][2]);
         u[nt][3] = fmaf(f.y * x1.inv, u[nt][3], r[nt][3]);
+        if (OUT) w_tiles[nt * 32] = make_float4(u[nt][0], u[nt][1], u[nt][2], u[nt][3]);
       }
-      if (SAVE) {  // w without the keys' factors
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt) {
-          const float2 f = *reinterpret_cast<const float2 *>(vec + kRowK * kC + nt * 8 + 2 * c);
-          const float fx = inverse_pow2(f.x), fy = inverse_pow2(f.y);
-          r[nt][0] = fx * u[nt][0];
-          r[nt][1] = fy * u[nt][1];
-          r[nt][2] = fx * u[nt][2];
-          r[nt][3] = fy * u[nt][3];
-        }
-        save_rows(a.ws + ((first + n) * a.vp + v0) * kC, lane, r);
-        save_token_max(a.token_maxes, first + n, kTokenW, a.vp / 16, w, r, lane);
-      }
-#pragma unroll
-      for (int nt = 0; nt < 8; ++nt) {
-        const float2 be = *reinterpret_cast<const float2 *>(vec + kRowBeta * kC + nt * 8 + 2 * c);
-        u[nt][0] *= be.x;
-        u[nt][1] *= be.y;
-        u[nt][2] *= be.x;
-        u[nt][3] *= be.y;
-      }
-      if (OUT) {
-        row_max(u, m0, m1);
-        x0 = scale_for(m0), x1 = scale_for(m1);
-        zero(y);
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          split_frag(u, ks, x0.mul, x1.mul, hi, lo);
-          step_rows<kC, 2>(y, hi, lo, st + St::kP, kC * kC * 2, ks, ks, lane);
-        }
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt) {
-          const float2 p = *reinterpret_cast<const float2 *>(vec + kRowP * kC + nt * 8 + 2 * c);
-          const float2 q = *reinterpret_cast<const float2 *>(vec + kRowO * kC + nt * 8 + 2 * c);
-          y[nt][0] = p.x * (x0.inv * y[nt][0]) + q.x * (s0.inv * qs[nt][0]);
-          y[nt][1] = p.y * (x0.inv * y[nt][1]) + q.y * (s0.inv * qs[nt][1]);
-          y[nt][2] = p.x * (x1.inv * y[nt][2]) + q.x * (s1.inv * qs[nt][2]);
-          y[nt][3] = p.y * (x1.inv * y[nt][3]) + q.y * (s1.inv * qs[nt][3]);
-        }
-        __syncwarp();
-        Tile::put(mine, lane, y);
-        __syncwarp();
-        Tile::store(mine, o + t0 * so, so, (int)min((long long)kC, left - t0), cols, lane);
-      }
-      __syncwarp();
-      if (n + 1 < chunks)
-        Tile::load(tile, v + (t0 + kC) * a.sv.t, a.sv.t, (int)min((long long)kC, len - t0 - kC),
-                   cols, lane);
-
+      if (OUT) pair_arrive(1 + W + pair);
       const float gam = vec[kRowEG * kC + kC - 1];
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt) {
+        const float2 be = *reinterpret_cast<const float2 *>(vec + kRowBeta * kC + nt * 8 + 2 * c);
         const float2 f = *reinterpret_cast<const float2 *>(vec + kRowEC * kC + nt * 8 + 2 * c);
-        u[nt][0] *= f.x;
-        u[nt][1] *= f.y;
-        u[nt][2] *= f.x;
-        u[nt][3] *= f.y;
+        const float fx = be.x * f.x, fy = be.y * f.y;
+        u[nt][0] *= fx;
+        u[nt][1] *= fy;
+        u[nt][2] *= fx;
+        u[nt][3] *= fy;
       }
       row_max(u, m0, m1);
       x0 = scale_beside(m0, gam * big0), x1 = scale_beside(m1, gam * big1);
@@ -516,8 +504,73 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
         S[nt][2] *= x1.inv;
         S[nt][3] *= x1.inv;
       }
+    } else if (OUT) {
+      float qs[8][4];
+      zero(qs);
+      zero(y);
+      pair_wait(1 + pair);
+      m0 = row_maxes[lane >> 2], m1 = row_maxes[(lane >> 2) + 8];
+      const Scale s0 = scale_for(m0), s1 = scale_for(m1);
+      if (SAVE) save_scales(a.scales + (first + n) * a.vp + v0, m0, m1, lane);
+      __half *keep = SAVE ? a.states + ((first + n) * a.vp + v0) * 2 * KD : nullptr;
+#pragma unroll
+      for (int ks = 0; ks < KD / 16; ++ks) {
+        const uint4 f = frags[ks * 64], g = frags[ks * 64 + 32];
+        hi[0] = f.x, hi[1] = f.y, hi[2] = f.z, hi[3] = f.w;
+        lo[0] = g.x, lo[1] = g.y, lo[2] = g.z, lo[3] = g.w;
+        step_rows<KD, NP>(qs, hi, lo, st + St::kQ, kC * KD * 2, ks, 0, lane);
+        if (SAVE) save_frag<KD>(keep, ks, lane, hi, lo);
+      }
+      pair_wait(1 + W + pair);
+      float u[8][4];
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt) {
+        const float4 x = w_tiles[nt * 32];
+        u[nt][0] = x.x, u[nt][1] = x.y, u[nt][2] = x.z, u[nt][3] = x.w;
+      }
+      if (SAVE) {  // w without the keys' factors
+        float x[8][4];
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt) {
+          const float2 f = *reinterpret_cast<const float2 *>(vec + kRowK * kC + nt * 8 + 2 * c);
+          const float fx = inverse_pow2(f.x), fy = inverse_pow2(f.y);
+          x[nt][0] = fx * u[nt][0];
+          x[nt][1] = fy * u[nt][1];
+          x[nt][2] = fx * u[nt][2];
+          x[nt][3] = fy * u[nt][3];
+        }
+        save_rows(a.ws + ((first + n) * a.vp + v0) * kC, lane, x);
+        save_token_max(a.token_maxes, first + n, kTokenW, a.vp / 16, w, x, lane);
+      }
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt) {
+        const float2 be = *reinterpret_cast<const float2 *>(vec + kRowBeta * kC + nt * 8 + 2 * c);
+        u[nt][0] *= be.x;
+        u[nt][1] *= be.y;
+        u[nt][2] *= be.x;
+        u[nt][3] *= be.y;
+      }
+      row_max(u, m0, m1);
+      const Scale x0 = scale_for(m0), x1 = scale_for(m1);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        split_frag(u, ks, x0.mul, x1.mul, hi, lo);
+        step_rows<kC, 2>(y, hi, lo, st + St::kP, kC * kC * 2, ks, ks, lane);
+      }
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt) {
+        const float2 p = *reinterpret_cast<const float2 *>(vec + kRowP * kC + nt * 8 + 2 * c);
+        const float2 q = *reinterpret_cast<const float2 *>(vec + kRowO * kC + nt * 8 + 2 * c);
+        y[nt][0] = p.x * (x0.inv * y[nt][0]) + q.x * (s0.inv * qs[nt][0]);
+        y[nt][1] = p.y * (x0.inv * y[nt][1]) + q.y * (s0.inv * qs[nt][1]);
+        y[nt][2] = p.x * (x1.inv * y[nt][2]) + q.x * (s1.inv * qs[nt][2]);
+        y[nt][3] = p.y * (x1.inv * y[nt][3]) + q.y * (s1.inv * qs[nt][3]);
+      }
+      __syncwarp();
+      Tile::put(mine, lane, y);
+      __syncwarp();
+      Tile::store(mine, o + t0 * so, so, (int)min((long long)kC, left - t0), cols, lane);
     }
-    copy_commit();
   }
   copy_wait<0>();
   if (!on) return;
@@ -526,8 +579,11 @@ __global__ void __launch_bounds__(W * 32, 1) scan_kernel(const Args a) {
     store_state<KD>(a.ends + (bh * a.segs + seg) * a.kdim * ld, ld, v0, a.kdim, ld, lane, S);
     return;
   }
-  if (a.sT != nullptr && seg == a.segs - 1)
-    store_state<KD>(a.sT + bh * a.kdim * a.vdim, a.vdim, v0, a.kdim, a.vdim, lane, S);
+  if (states) {
+    if (a.sT != nullptr && seg == a.segs - 1)
+      store_state<KD>(a.sT + bh * a.kdim * a.vdim, a.vdim, v0, a.kdim, a.vdim, lane, S);
+    return;
+  }
   // this span's tokens past the row's end: zeros
   constexpr int kPer = 16 / sizeof(E), kPieces = 16 / kPer;
   const long long stop = min(left, (long long)a.seg_chunks * kC);
