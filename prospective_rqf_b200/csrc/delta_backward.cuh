@@ -380,19 +380,25 @@ struct DoutTile {
   }
 };
 
-// Reduction of values `stride` apart, eight loads at a time.
-template <bool SUM>
-__device__ __forceinline__ float reduce_strided(const float *p, int count, int stride) {
-  float all = 0.f;
-  for (int j = 0; j < count; j += 8) {
-    float x[8];
+// Values `stride` apart, N of them in flight, and their reduction with what lies past them.
+template <int N>
+struct Strided {
+  float x[N];
+  const float *p;
+  int count, stride;
+  __device__ __forceinline__ Strided(const float *from, int n, int step) : p(from), count(n), stride(step) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = j + i < count ? p[(j + i) * stride] : 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) all = SUM ? all + x[i] : fmaxf(all, x[i]);
+    for (int i = 0; i < N; ++i) x[i] = i < count ? p[i * stride] : 0.f;
   }
-  return all;
-}
+  template <bool SUM>
+  __device__ __forceinline__ float reduce() const {
+    float all = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) all = SUM ? all + x[i] : fmaxf(all, x[i]);
+    for (int i = N; i < count; ++i) all = SUM ? all + p[i * stride] : fmaxf(all, p[i * stride]);
+    return all;
+  }
+};
 
 // 16 columns of V of S, dS and dS' into one stage of the ring.
 template <typename E, int KD>
@@ -540,7 +546,7 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
   __shared__ __align__(8) uint64_t bars[L::kStages + 1];
   const uint32_t bar = smem_u32(bars), first_bar = bar + L::kStages * 8;
   Waiter wait{a.error, false};
-  if (tid == 0) {
+  if (tid == kThreads - 32) {
 #pragma unroll
     for (int i = 0; i <= L::kStages; ++i) bar_init(bar + i * 8);
     bars_ready();
@@ -558,19 +564,22 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
   const long long so = (long long)a.hv * a.vdim;
   // the largest row scales of S, dS and dS', to which all rows' are taken
   const float *row_scales[3] = {a.scales + chunk * a.vp, a.dscales + slot * a.vp, a.dscales + (slot + 1) * a.vp};
-  float big[3];
-#pragma unroll
-  for (int i = 0; i < 3; ++i)
-    big[i] = reduce_strided<false>(row_scales[i] + lane, (a.vp - lane + 31) / 32, 32);
-  if (tid < kTokenMaxes * kC) {
-    const float *m = a.token_maxes + (chunk * kTokenMaxes + tid / kC) * steps * kC + tid % kC;
-    w_inv[tid] = scale_for(reduce_strided<false>(m, steps, kC)).inv;
-  } else if (tid < kTokenMaxes * kC + kC) {
-    const int t = tid - kTokenMaxes * kC;
-    const float2 x = a.gsum[chunk * kC + t];
-    g_hi[t] = x.x;
-    g_lo[t] = x.y;
-    vdv[t] = reduce_strided<true>(a.vdv + chunk * steps * kC + t, steps, kC);
+  // all loads before the first reduction: each is a wait for memory
+  const int t = tid % kC, what = min(tid / kC, kTokenMaxes);  // w, dr, do, v.dv of a token
+  const Strided<4> rows0(row_scales[0] + lane, (a.vp - lane + 31) / 32, 32);
+  const Strided<4> rows1(row_scales[1] + lane, (a.vp - lane + 31) / 32, 32);
+  const Strided<4> rows2(row_scales[2] + lane, (a.vp - lane + 31) / 32, 32);
+  const Strided<8> token(what < kTokenMaxes ? a.token_maxes + (chunk * kTokenMaxes + what) * steps * kC + t
+                                            : a.vdv + chunk * steps * kC + t,
+                         tid < (kTokenMaxes + 1) * kC ? steps : 0, kC);
+  const float2 gates = a.gsum[chunk * kC + t];
+  float big[3] = {rows0.template reduce<false>(), rows1.template reduce<false>(), rows2.template reduce<false>()};
+  if (what < kTokenMaxes) {
+    w_inv[tid] = scale_for(token.template reduce<false>()).inv;
+  } else if (tid < (kTokenMaxes + 1) * kC) {
+    g_hi[t] = gates.x;
+    g_lo[t] = gates.y;
+    vdv[t] = token.template reduce<true>();
   }
 #pragma unroll
   for (int i = 0; i < 3; ++i)
