@@ -29,24 +29,40 @@
 namespace rqf {
 namespace delta {
 
+// Shared memory of that pass with W warps on the state's cotangents and W beside them: tiles (of
+// two chunks where that fits), a tile of do or v to a pair, and what a pair hands over: dS' as
+// fragments, P^T do and then dr (whose place dv takes), q^T of the scaled do, the rows' largest
+// magnitudes.
 template <typename E, int KD, int W>
-constexpr size_t backward_smem() {
-  return 2 * (size_t)Stage<KD, Elem<E>::kParts>::kBytes + (size_t)W * kC * 16 * sizeof(E);
-}
+struct BackLayout {
+  static constexpr int kStage = Stage<KD, Elem<E>::kParts>::kBytes;
+  static constexpr int kTile = kC * 16 * (int)sizeof(E);
+  static constexpr int kFrags = KD / 16 * 2 * 32 * 16, kPdo = 8 * 32 * 16, kZ = KD / 8 * 32 * 16;
+  static constexpr int kHand = kFrags + kPdo + kZ + 16 * 4;
+  static constexpr int kRest = W * (kTile + kHand);
+  static constexpr int kStages = 2 * kStage + kRest <= 227 * 1024 ? 2 : 1;
+  static constexpr int kDO = kStages * kStage, kGive = kDO + W * kTile, kBytes = kDO + kRest;
+  static constexpr int kThreads = 2 * W * 32;
+};
 
+// As in the forward's pass, a pair of warps: one on the chain from dS' to dS (k dS', T'^T du,
+// k^T dr), the other on what does not wait for it (P^T do, q^T do) or that nothing waits for (dr,
+// dv, v.dv, and dS' as the next pass reads it).
 template <typename E, int KD, int W, bool OUT>
-__global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) {
+__global__ void __launch_bounds__(BackLayout<E, KD, W>::kThreads, 1) scan_backward_kernel(const Args a) {
   constexpr int NP = Elem<E>::kParts;
+  using L = BackLayout<E, KD, W>;
   using St = Stage<KD, NP>;
   using Tile = WarpTile<E>;
   extern __shared__ __align__(128) unsigned char smem[];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, c = lane & 3;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, c = lane & 3, pair = warp % W;
+  const bool chain = warp < W;
   const unsigned blocks = (a.vp / 16 + W - 1) / W, spans = OUT ? a.segs : a.segs - 1;
   const unsigned which = blockIdx.x / blocks, head = which / spans;
   const int seg = (int)(which - head * spans) + (OUT ? 0 : 1);  // the first one's start is nobody's end
   const long long bh = head;
   const int b = (int)(head / (unsigned)a.hv), h = (int)(head - b * (unsigned)a.hv), hk = h / a.rep;
-  const int w = (int)(blockIdx.x - which * blocks) * W + warp;
+  const int w = (int)(blockIdx.x - which * blocks) * W + pair;
   const int v0 = w * 16;
   const bool on = v0 < a.vp;
   const int cols = min(16, a.vdim - v0);
@@ -58,7 +74,12 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
   const long long kv_first = ((long long)b * a.hk + hk) * a.n_chunks + n0, first = bh * a.n_chunks + n0;
   const long long slot = bh * (a.n_chunks + 1) + n0;
   const uint32_t base = smem_u32(smem);
-  unsigned char *mine = smem + 2 * St::kBytes + warp * kC * 16 * sizeof(E);
+  unsigned char *mine = smem + L::kDO + pair * L::kTile, *give = smem + L::kGive + pair * L::kHand;
+  uint4 *frags = reinterpret_cast<uint4 *>(give) + lane;                          // [ks][hi, lo][lane]
+  unsigned char *pdo_bytes = give + L::kFrags;
+  float4 *pdo = reinterpret_cast<float4 *>(pdo_bytes) + lane;                     // [nt][lane]
+  float4 *z_tiles = reinterpret_cast<float4 *>(pdo_bytes + L::kPdo) + lane;       // [nt][lane]
+  float *row_maxes = reinterpret_cast<float *>(pdo_bytes + L::kPdo + L::kZ);      // [row]
   const uint32_t tile = smem_u32(mine);
   const E *v = static_cast<const E *>(a.v) + b * a.sv.b + (long long)n0 * kC * a.sv.t + h * a.sv.h + v0;
   const long long so = (long long)a.hv * a.vdim;  // do and dv are dense
@@ -66,8 +87,8 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
   const E *dout = static_cast<const E *>(a.dout) + at;
   E *dv = static_cast<E *>(a.dv) + at;
 
-  float S[KD / 8][4];  // dS'
-  {
+  float S[KD / 8][4];  // dS'; in the other warps q^T do
+  if (chain) {
     const float *from = seg == a.segs - 1 ? (a.dsT ? a.dsT + bh * a.kdim * a.vdim : nullptr)
                         : OUT             ? a.grad_starts + (bh * a.segs + seg) * a.kdim * a.vdim
                                           : nullptr;
@@ -83,81 +104,60 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
     bars_ready();
     if (chunks > 0) load_stage<KD, NP>(base, a, kv_first + chunks - 1, first + chunks - 1, bar);
   }
-  if (chunks > 0 && on) {
+  if (!chain && chunks > 0 && on) {
     const long long t0 = (long long)(chunks - 1) * kC;
     Tile::load(tile, dout + t0 * so, so, (int)(len - t0), cols, lane);
   }
   copy_commit();
   __syncthreads();
   for (int n = chunks - 1; n >= 0; --n) {
-    const int turn = chunks - 1 - n;
-    const uint32_t st = base + (turn & 1) * St::kBytes;
-    const float *vec = reinterpret_cast<const float *>(smem + (turn & 1) * St::kBytes + St::kV);
+    const int turn = chunks - 1 - n, stage = L::kStages == 2 ? turn & 1 : 0;
+    const uint32_t st = base + stage * L::kStage;
+    const float *vec = reinterpret_cast<const float *>(smem + stage * L::kStage + St::kV);
     const long long t0 = (long long)n * kC;
-    wait(bar + (turn & 1) * 8, (turn >> 1) & 1);
-    __syncthreads();  // all are done with the other stage
-    if (tid == 0 && n > 0)
-      load_stage<KD, NP>(base + ((turn + 1) & 1) * St::kBytes, a, kv_first + n - 1, first + n - 1,
-                         bar + ((turn + 1) & 1) * 8);
-    if (on) {
-      float m0, m1;
-      uint32_t hi[4], lo[4];
+    if (L::kStages == 2) {
+      wait(bar + stage * 8, (turn >> 1) & 1);
+      __syncthreads();  // all are done with the other stage, and with what was handed over
+      if (tid == 0 && n > 0)
+        load_stage<KD, NP>(base + (stage ^ 1) * L::kStage, a, kv_first + n - 1, first + n - 1, bar + (stage ^ 1) * 8);
+    } else {
+      __syncthreads();
+      if (tid == 0 && turn > 0) load_stage<KD, NP>(base, a, kv_first + n, first + n, bar);
+      wait(bar, turn & 1);
+    }
+    if (!on) continue;
+    uint32_t hi[4], lo[4];
+    float m0, m1;
+    if (chain) {
       row_max(S, m0, m1);
-      const float big0 = m0, big1 = m1;
       const Scale s0 = scale_for(m0), s1 = scale_for(m1);
-      if (OUT) save_scales(a.dscales + (slot + n + 1) * a.vp + v0, m0, m1, lane);
-      __half *keep = a.dstates + ((slot + n + 1) * a.vp + v0) * 2 * KD;
-      float du[8][4], dr[8][4], x[8][4];
+      if (OUT && c == 0) row_maxes[lane >> 2] = m0, row_maxes[(lane >> 2) + 8] = m1;
+      float du[8][4], dr[8][4];
       zero(dr);  // k dS' first
 #pragma unroll
       for (int ks = 0; ks < KD / 16; ++ks) {
         split_frag(S, ks, s0.mul, s1.mul, hi, lo);
-        if (OUT) save_frag<KD>(keep, ks, lane, hi, lo);
+        if (OUT) {
+          frags[ks * 64] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          frags[ks * 64 + 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
         step_rows<KD, NP>(dr, hi, lo, st + St::kK, kC * KD * 2, ks, 0, lane);
       }
-      copy_wait<0>();
-      __syncwarp();
-      Tile::get(tile, mine, lane, x);
-      __syncwarp();  // v takes the place of do
-      if (OUT) Tile::load(tile, v + t0 * a.sv.t, a.sv.t, (int)min((long long)kC, len - t0), cols, lane);
-      copy_commit();
-      if (OUT) save_token_max(a.token_maxes, first + n, kTokenDO, a.vp / 16, w, x, lane);
+      pair_wait(1 + pair);  // P^T do
       Scale x0, x1;
       {
         float y[8][4];
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt) {
-          const float2 p = *reinterpret_cast<const float2 *>(vec + kRowP * kC + nt * 8 + 2 * c);
-          y[nt][0] = x[nt][0] * p.x;
-          y[nt][1] = x[nt][1] * p.y;
-          y[nt][2] = x[nt][2] * p.x;
-          y[nt][3] = x[nt][3] * p.y;
-        }
-        row_max(y, m0, m1);
-        x0 = scale_for(m0), x1 = scale_for(m1);
-        zero(du);
-        // a 16-bit do times powers of two is one half exactly
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          split_frag(y, ks, x0.mul, x1.mul, hi, lo);
-          step_cols<kC, NP, 2>(du, hi, lo, st + St::kP, kC * kC * 2, ks, ks, lane);
-        }
-      }
-#pragma unroll
-      for (int nt = 0; nt < 8; ++nt) {
-        const float2 f = *reinterpret_cast<const float2 *>(vec + kRowEC * kC + nt * 8 + 2 * c);
-        du[nt][0] = x0.inv * du[nt][0] + f.x * (s0.inv * dr[nt][0]);
-        du[nt][1] = x0.inv * du[nt][1] + f.y * (s0.inv * dr[nt][1]);
-        du[nt][2] = x1.inv * du[nt][2] + f.x * (s1.inv * dr[nt][2]);
-        du[nt][3] = x1.inv * du[nt][3] + f.y * (s1.inv * dr[nt][3]);
-      }
-      {
-        float y[8][4];
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt) {
+          const float2 f = *reinterpret_cast<const float2 *>(vec + kRowEC * kC + nt * 8 + 2 * c);
           const float2 t = *reinterpret_cast<const float2 *>(vec + kRowT * kC + nt * 8 + 2 * c);
           const float2 be = *reinterpret_cast<const float2 *>(vec + kRowBeta * kC + nt * 8 + 2 * c);
           const float fx = t.x * be.x, fy = t.y * be.y;
+          const float4 p = pdo[nt * 32];
+          du[nt][0] = fmaf(f.x, s0.inv * dr[nt][0], p.x);
+          du[nt][1] = fmaf(f.y, s0.inv * dr[nt][1], p.y);
+          du[nt][2] = fmaf(f.x, s1.inv * dr[nt][2], p.z);
+          du[nt][3] = fmaf(f.y, s1.inv * dr[nt][3], p.w);
           y[nt][0] = fx * du[nt][0];
           y[nt][1] = fy * du[nt][1];
           y[nt][2] = fx * du[nt][2];
@@ -174,78 +174,43 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
       }
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt) {
-        const float2 f = *reinterpret_cast<const float2 *>(vec + kRowK * kC + nt * 8 + 2 * c);
+        const float2 k = *reinterpret_cast<const float2 *>(vec + kRowKS * kC + nt * 8 + 2 * c);
+        const float2 be = *reinterpret_cast<const float2 *>(vec + kRowBeta * kC + nt * 8 + 2 * c);
+        const float kx = -be.x * k.x, ky = -be.y * k.y;
         dr[nt][0] = fmaf(x0.inv, dr[nt][0], du[nt][0]);
         dr[nt][1] = fmaf(x0.inv, dr[nt][1], du[nt][1]);
         dr[nt][2] = fmaf(x1.inv, dr[nt][2], du[nt][2]);
         dr[nt][3] = fmaf(x1.inv, dr[nt][3], du[nt][3]);
-        du[nt][0] = f.x * dr[nt][0];
-        du[nt][1] = f.y * dr[nt][1];
-        du[nt][2] = f.x * dr[nt][2];
-        du[nt][3] = f.y * dr[nt][3];
-      }
-      if (OUT) {
-        save_rows(a.drs + ((first + n) * a.vp + v0) * kC, lane, du);  // dr with the keys' factors
-        save_token_max(a.token_maxes, first + n, kTokenDR, a.vp / 16, w, du, lane);
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt) {
-          const float2 be = *reinterpret_cast<const float2 *>(vec + kRowBeta * kC + nt * 8 + 2 * c);
-          du[nt][0] *= be.x;
-          du[nt][1] *= be.y;
-          du[nt][2] *= be.x;
-          du[nt][3] *= be.y;
-        }
-        copy_wait<0>();
-        __syncwarp();
-        {
-          float y[8][4], m[8][2];
-          Tile::get(tile, mine, lane, y);
-#pragma unroll
-          for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) m[nt][e] = fmaf(y[nt][e], du[nt][e], y[nt][e + 2] * du[nt][e + 2]);
-          save_tokens<true>(a.vdv + ((first + n) * (a.vp / 16) + w) * kC, m, lane);
-        }
-        __syncwarp();
-        Tile::put(mine, lane, du);
-        __syncwarp();
-        Tile::store(mine, dv + t0 * so, so, (int)min((long long)kC, left - t0), cols, lane);
-      }
-      __syncwarp();
-      if (n > 0) Tile::load(tile, dout + (t0 - kC) * so, so, kC, cols, lane);
-
-      // dS = e^{G_C} dS' + (scale e^G q)^T do - (beta e^G k)^T dr, both under one scale
-      const float gam = vec[kRowEG * kC + kC - 1];
-#pragma unroll
-      for (int nt = 0; nt < 8; ++nt) {
-        const float2 p = *reinterpret_cast<const float2 *>(vec + kRowO * kC + nt * 8 + 2 * c);
-        const float2 k = *reinterpret_cast<const float2 *>(vec + kRowKS * kC + nt * 8 + 2 * c);
-        const float2 be = *reinterpret_cast<const float2 *>(vec + kRowBeta * kC + nt * 8 + 2 * c);
-        const float kx = -be.x * k.x, ky = -be.y * k.y;
-        x[nt][0] *= p.x;
-        x[nt][1] *= p.y;
-        x[nt][2] *= p.x;
-        x[nt][3] *= p.y;
+        if (OUT) pdo[nt * 32] = make_float4(dr[nt][0], dr[nt][1], dr[nt][2], dr[nt][3]);
         dr[nt][0] *= kx;
         dr[nt][1] *= ky;
         dr[nt][2] *= kx;
         dr[nt][3] *= ky;
       }
-      float d0, d1;
-      row_max(x, m0, m1);
-      row_max(dr, d0, d1);
-      x0 = scale_beside(fmaxf(m0, d0), gam * big0), x1 = scale_beside(fmaxf(m1, d1), gam * big1);
+      if (OUT) pair_arrive(1 + 2 * W + pair);  // dS' and dr
+      const float gam = vec[kRowEG * kC + kC - 1];
+      pair_wait(1 + W + pair);  // (scale e^G q)^T do
 #pragma unroll
       for (int nt = 0; nt < KD / 8; ++nt) {
-        S[nt][0] *= gam * x0.mul;
-        S[nt][1] *= gam * x0.mul;
-        S[nt][2] *= gam * x1.mul;
-        S[nt][3] *= gam * x1.mul;
+        const float4 z = z_tiles[nt * 32];
+        S[nt][0] = fmaf(gam, S[nt][0], z.x);
+        S[nt][1] = fmaf(gam, S[nt][1], z.y);
+        S[nt][2] = fmaf(gam, S[nt][2], z.z);
+        S[nt][3] = fmaf(gam, S[nt][3], z.w);
+      }
+      float d0, d1;
+      row_max(S, m0, m1);
+      row_max(dr, d0, d1);
+      x0 = scale_beside(d0, m0), x1 = scale_beside(d1, m1);
+#pragma unroll
+      for (int nt = 0; nt < KD / 8; ++nt) {
+        S[nt][0] *= x0.mul;
+        S[nt][1] *= x0.mul;
+        S[nt][2] *= x1.mul;
+        S[nt][3] *= x1.mul;
       }
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
-        split_frag(x, ks, x0.mul, x1.mul, hi, lo);
-        step_cols<KD, 2, NP>(S, hi, lo, st + St::kQ, kC * KD * 2, ks, KD, lane);
         split_frag(dr, ks, x0.mul, x1.mul, hi, lo);
         step_cols<KD, 2, NP>(S, hi, lo, st + St::kK, kC * KD * 2, ks, KD, lane);
       }
@@ -256,13 +221,119 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
         S[nt][2] *= x1.inv;
         S[nt][3] *= x1.inv;
       }
+    } else {
+      float x[8][4], y[8][4];
+      copy_wait<0>();  // do
+      __syncwarp();
+      Tile::get(tile, mine, lane, x);
+      __syncwarp();
+      if (OUT) Tile::load(tile, v + t0 * a.sv.t, a.sv.t, (int)min((long long)kC, len - t0), cols, lane);
+      else if (n > 0) Tile::load(tile, dout + (t0 - kC) * so, so, kC, cols, lane);
+      copy_commit();
+      Scale x0, x1;
+      {
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt) {
+          const float2 p = *reinterpret_cast<const float2 *>(vec + kRowP * kC + nt * 8 + 2 * c);
+          y[nt][0] = x[nt][0] * p.x;
+          y[nt][1] = x[nt][1] * p.y;
+          y[nt][2] = x[nt][2] * p.x;
+          y[nt][3] = x[nt][3] * p.y;
+        }
+        row_max(y, m0, m1);
+        x0 = scale_for(m0), x1 = scale_for(m1);
+        float u[8][4];
+        zero(u);
+        // a 16-bit do times powers of two is one half exactly
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          split_frag(y, ks, x0.mul, x1.mul, hi, lo);
+          step_cols<kC, NP, 2>(u, hi, lo, st + St::kP, kC * kC * 2, ks, ks, lane);
+        }
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt)
+          pdo[nt * 32] = make_float4(x0.inv * u[nt][0], x0.inv * u[nt][1], x1.inv * u[nt][2], x1.inv * u[nt][3]);
+      }
+      pair_arrive(1 + pair);
+      if (OUT) save_token_max(a.token_maxes, first + n, kTokenDO, a.vp / 16, w, x, lane);
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt) {
+        const float2 p = *reinterpret_cast<const float2 *>(vec + kRowO * kC + nt * 8 + 2 * c);
+        x[nt][0] *= p.x;
+        x[nt][1] *= p.y;
+        x[nt][2] *= p.x;
+        x[nt][3] *= p.y;
+      }
+      row_max(x, m0, m1);
+      x0 = scale_for(m0), x1 = scale_for(m1);
+      zero(S);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        split_frag(x, ks, x0.mul, x1.mul, hi, lo);
+        step_cols<KD, 2, NP>(S, hi, lo, st + St::kQ, kC * KD * 2, ks, KD, lane);
+      }
+#pragma unroll
+      for (int nt = 0; nt < KD / 8; ++nt)
+        z_tiles[nt * 32] = make_float4(x0.inv * S[nt][0], x0.inv * S[nt][1], x1.inv * S[nt][2], x1.inv * S[nt][3]);
+      pair_arrive(1 + W + pair);
+      if (OUT) {
+        pair_wait(1 + 2 * W + pair);  // dS' and dr
+        save_scales(a.dscales + (slot + n + 1) * a.vp + v0, row_maxes[lane >> 2], row_maxes[(lane >> 2) + 8], lane);
+        __half *keep = a.dstates + ((slot + n + 1) * a.vp + v0) * 2 * KD;
+#pragma unroll
+        for (int ks = 0; ks < KD / 16; ++ks) {
+          const uint4 f = frags[ks * 64], g = frags[ks * 64 + 32];
+          hi[0] = f.x, hi[1] = f.y, hi[2] = f.z, hi[3] = f.w;
+          lo[0] = g.x, lo[1] = g.y, lo[2] = g.z, lo[3] = g.w;
+          save_frag<KD>(keep, ks, lane, hi, lo);
+        }
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt) {  // dr with the keys' factors
+          const float2 f = *reinterpret_cast<const float2 *>(vec + kRowK * kC + nt * 8 + 2 * c);
+          const float4 r = pdo[nt * 32];
+          x[nt][0] = f.x * r.x;
+          x[nt][1] = f.y * r.y;
+          x[nt][2] = f.x * r.z;
+          x[nt][3] = f.y * r.w;
+        }
+        save_rows(a.drs + ((first + n) * a.vp + v0) * kC, lane, x);
+        save_token_max(a.token_maxes, first + n, kTokenDR, a.vp / 16, w, x, lane);
+        copy_wait<0>();  // v
+        __syncwarp();
+        Tile::get(tile, mine, lane, y);
+        __syncwarp();
+        if (n > 0) Tile::load(tile, dout + (t0 - kC) * so, so, kC, cols, lane);
+        copy_commit();
+        float m[8][2];
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt) {
+          const float2 be = *reinterpret_cast<const float2 *>(vec + kRowBeta * kC + nt * 8 + 2 * c);
+          x[nt][0] *= be.x;
+          x[nt][1] *= be.y;
+          x[nt][2] *= be.x;
+          x[nt][3] *= be.y;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) m[nt][e] = fmaf(y[nt][e], x[nt][e], y[nt][e + 2] * x[nt][e + 2]);
+        }
+        save_tokens<true>(a.vdv + ((first + n) * (a.vp / 16) + w) * kC, m, lane);
+        Tile::put(pdo_bytes, lane, x);
+        __syncwarp();
+        Tile::store(pdo_bytes, dv + t0 * so, so, (int)min((long long)kC, left - t0), cols, lane);
+      }
     }
-    copy_commit();
   }
   copy_wait<0>();
   if (!on) return;
   if (!OUT) {
-    store_state<KD>(a.grad_ends + (bh * a.segs + seg) * a.kdim * a.vp, a.vp, v0, a.kdim, a.vp, lane, S);
+    if (chain) store_state<KD>(a.grad_ends + (bh * a.segs + seg) * a.kdim * a.vp, a.vp, v0, a.kdim, a.vp, lane, S);
+    return;
+  }
+  if (!chain) {  // this span's tokens past the row's end: zeros
+    constexpr int kPer = 16 / sizeof(E), kPieces = 16 / kPer;
+    const long long stop = min(left, (long long)a.seg_chunks * kC);
+    for (long long t = (long long)chunks * kC + lane / kPieces; t < stop; t += 32 / kPieces)
+      if ((lane % kPieces) * kPer < cols)
+        *reinterpret_cast<uint4 *>(dv + t * so + (lane % kPieces) * kPer) = make_uint4(0, 0, 0, 0);
     return;
   }
   if (seg == 0 && chunks > 0) {  // the cotangent of the state that enters the first chunk
@@ -279,11 +350,6 @@ __global__ void __launch_bounds__(W * 32, 1) scan_backward_kernel(const Args a) 
   }
   if (a.ds0 != nullptr && seg == 0)
     store_state<KD>(a.ds0 + bh * a.kdim * a.vdim, a.vdim, v0, a.kdim, a.vdim, lane, S);
-  constexpr int kPer = 16 / sizeof(E), kPieces = 16 / kPer;
-  const long long stop = min(left, (long long)a.seg_chunks * kC);
-  for (long long t = (long long)chunks * kC + lane / kPieces; t < stop; t += 32 / kPieces)
-    if ((lane % kPieces) * kPer < cols)
-      *reinterpret_cast<uint4 *>(dv + t * so + (lane % kPieces) * kPer) = make_uint4(0, 0, 0, 0);
 }
 
 // ------------------------------------------------------------ all chunks at once

@@ -179,13 +179,9 @@ int run_scan(const Args &a, cudaStream_t st) {
 }
 template <typename E, int KD, bool OUT>
 int run_scan_backward(const Args &a, cudaStream_t st) {
-  const int64_t rows = (int64_t)a.batch * a.hv * (OUT ? a.segs : a.segs - 1), columns = a.vp;
-  if constexpr (backward_smem<E, KD, 8>() <= kMaxSmem)
-    if (eight_warps(rows, columns))
-      return launch(scan_backward_kernel<E, KD, 8, OUT>, rows * ceil_div(columns, 128), 256,
-                    backward_smem<E, KD, 8>(), a, st);
-  return launch(scan_backward_kernel<E, KD, 4, OUT>, rows * ceil_div(columns, 64), 128,
-                backward_smem<E, KD, 4>(), a, st);
+  using Four = BackLayout<E, KD, 4>;
+  const int64_t rows = (int64_t)a.batch * a.hv * (OUT ? a.segs : a.segs - 1);
+  return launch(scan_backward_kernel<E, KD, 4, OUT>, rows * ceil_div(a.vp, 64), Four::kThreads, Four::kBytes, a, st);
 }
 template <bool BACK>
 int run_combine(const Args &a, cudaStream_t st) {
