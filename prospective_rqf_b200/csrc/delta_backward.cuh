@@ -628,6 +628,12 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
   const float *w_rows = a.ws + chunk * a.vp * kC, *dr_rows = a.drs + chunk * a.vp * kC;
   const E *do_rows = static_cast<const E *>(a.dout) + gb * a.vdim;
   const long long so = (long long)a.hv * a.vdim;
+  // the first block of V, in flight while the scales are found
+  TokenTile<VB, kThreads> w_first, dr_first;
+  DoutTile<E, VB, NP, kThreads> do_first;
+  w_first.load(w_rows, min(VB, a.vp), tid);
+  dr_first.load(dr_rows, min(VB, a.vp), tid);
+  do_first.load(do_rows, so, live, a.vdim, tid);
   // the largest row scales of S, dS and dS', to which all rows' are taken
   const float *row_scales[3] = {a.scales + chunk * a.vp, a.dscales + slot * a.vp, a.dscales + (slot + 1) * a.vp};
   // all loads before the first reduction: each is a wait for memory
@@ -653,6 +659,13 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
     for (int d = 16; d > 0; d >>= 1) big[i] = fmaxf(big[i], __shfl_xor_sync(0xffffffffu, big[i], d));
   __syncthreads();
 
+  w_first.store(smem + L::kW, smem + L::kW + VB * kC * 2, w_inv, tid);
+  dr_first.store(smem + L::kDR, smem + L::kDR + VB * kC * 2, dr_inv, tid);
+  do_first.store(smem + L::kDO, do_inv, tid);
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    if (tid < min(VB, a.vp)) rho[i * VB + tid] = row_scales[i][tid] * inverse_pow2(big[i]);
+
   float xa[NX][4], xb[NX][4], d[ND][4];  // X1 or X3; X2; dP or dA
   zero(xa);
   zero(xb);
@@ -660,9 +673,9 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
   float both = 0.f;  // <S, dS>, this thread's part
   for (int step = 0; step < steps; ++step) {
     const int v0 = step * 16, local = v0 % VB;
-    if (local == 0) {
+    if (local == 0 && v0 > 0) {  // the next block of V
       const int rows = min(VB, a.vp - v0);
-      if (v0 > 0) __syncthreads();  // all are done with the block before
+      __syncthreads();  // all are done with the block before
       TokenTile<VB, kThreads> w_tile, dr_tile;
       DoutTile<E, VB, NP, kThreads> do_tile;
       w_tile.load(w_rows + v0 * kC, rows, tid);

@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "../../include/rqf_b200.h"
@@ -19,7 +20,6 @@ int *rqf_internal_error_word();
 namespace {
 
 constexpr int64_t kMaxGrid = 0x7fffffffLL;
-constexpr size_t kMaxSmem = 227 * 1024;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -152,11 +152,19 @@ int check_inputs(const rqf_delta_problem *p, const void *q, const void *k, const
   return RQF_OK;
 }
 
-template <typename F>
-int launch(F kernel, int64_t grid, int threads, size_t smem, const Args &a, cudaStream_t st) {
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return RQF_ERR_LAUNCH;
-  kernel<<<(unsigned)grid, threads, smem, st>>>(a);
+// Launches a kernel with `smem` bytes of dynamic shared memory, which the device is told of once.
+template <auto Kernel>
+int launch(int64_t grid, int threads, size_t smem, const Args &a, cudaStream_t st) {
+  static std::atomic<uint64_t> told{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return RQF_ERR_LAUNCH;
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (dev >= 64 || !(told.load(std::memory_order_relaxed) & bit)) {
+    if (cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+      return RQF_ERR_LAUNCH;
+    told.fetch_or(bit, std::memory_order_relaxed);
+  }
+  Kernel<<<(unsigned)grid, threads, smem, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? RQF_OK : RQF_ERR_LAUNCH;
 }
 
@@ -173,15 +181,15 @@ int run_scan(const Args &a, cudaStream_t st) {
   using Eight = Layout<E, KD, 8, PASS>;
   if constexpr (!out && Eight::kStages == 2)
     if (eight_warps(rows, columns))
-      return launch(scan_kernel<E, KD, 8, PASS>, rows * ceil_div(columns, 128), Eight::kThreads, Eight::kBytes, a, st);
+      return launch<scan_kernel<E, KD, 8, PASS>>(rows * ceil_div(columns, 128), Eight::kThreads, Eight::kBytes, a, st);
   using Four = Layout<E, KD, 4, PASS>;
-  return launch(scan_kernel<E, KD, 4, PASS>, rows * ceil_div(columns, 64), Four::kThreads, Four::kBytes, a, st);
+  return launch<scan_kernel<E, KD, 4, PASS>>(rows * ceil_div(columns, 64), Four::kThreads, Four::kBytes, a, st);
 }
 template <typename E, int KD, bool OUT>
 int run_scan_backward(const Args &a, cudaStream_t st) {
   using Four = BackLayout<E, KD, 4>;
   const int64_t rows = (int64_t)a.batch * a.hv * (OUT ? a.segs : a.segs - 1);
-  return launch(scan_backward_kernel<E, KD, 4, OUT>, rows * ceil_div(a.vp, 64), Four::kThreads, Four::kBytes, a, st);
+  return launch<scan_backward_kernel<E, KD, 4, OUT>>(rows * ceil_div(a.vp, 64), Four::kThreads, Four::kBytes, a, st);
 }
 template <bool BACK>
 int run_combine(const Args &a, cudaStream_t st) {
@@ -193,8 +201,8 @@ template <typename E, int KD>
 int run_forward(const Args &a, bool save, cudaStream_t st) {
   int rc = RQF_OK;
   if (a.n_chunks > 0)
-    rc = launch(prep_kernel<E, KD>, (int64_t)a.batch * a.hv * a.n_chunks, kPrepThreads,
-                prep_smem<KD, Elem<E>::kParts>(), a, st);
+    rc = launch<prep_kernel<E, KD>>((int64_t)a.batch * a.hv * a.n_chunks, kPrepThreads,
+                                    prep_smem<KD, Elem<E>::kParts>(), a, st);
   if (rc == RQF_OK && a.segs > 1) {
     rc = run_scan<E, KD, kEnds>(a, st);
     if (rc == RQF_OK) rc = run_combine<false>(a, st);
@@ -211,8 +219,8 @@ int run_backward(const Args &a, cudaStream_t st) {
   }
   if (rc == RQF_OK) rc = run_scan_backward<E, KD, true>(a, st);
   if (rc != RQF_OK || a.n_chunks == 0) return rc;
-  rc = launch(gradient_kernel<E, KD>, (int64_t)a.batch * a.hv * a.n_chunks,
-              Grad<E, KD>::kThreads, Grad<E, KD>::kBytes, a, st);
+  rc = launch<gradient_kernel<E, KD>>((int64_t)a.batch * a.hv * a.n_chunks, Grad<E, KD>::kThreads,
+                                      Grad<E, KD>::kBytes, a, st);
   if (rc != RQF_OK || a.dq_part == nullptr) return rc;
   const int64_t rows = a.batch * a.time, pairs = rows * a.hk * (a.kdim / 2);
   const int64_t blocks = ceil_div(pairs, 256);
