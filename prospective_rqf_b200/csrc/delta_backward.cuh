@@ -366,10 +366,10 @@ struct Grad {
   static constexpr int kK = 0, kQ = kKq;
   static constexpr int kW = 2 * kKq, kDR = kW + 2 * kVB * kC * 2;  // [v][t] hi, lo
   static constexpr int kDO = kDR + 2 * kVB * kC * 2;               // [t][v] parts
-  // a ring of 16 columns of V: S, dS and dS', hi and lo
+  // a ring of kSub times 16 columns of V: S, dS and dS', hi and lo
   static constexpr int kRing = kDO + NP * kC * kVB * 2;
-  static constexpr int kTile = 16 * KD * 2, kTiles = 6, kStage = kTiles * kTile;
-  static constexpr int kStages = NP == 2 && KD == 128 ? 2 : 4;
+  static constexpr int kTile = 16 * KD * 2, kSub = NP == 2 && KD == 128 ? 1 : 2;
+  static constexpr int kStage = 6 * kTile * kSub, kStages = 2;
   // after the products over V, from w's place on, hi and lo: E with the keys' factors, E with the
   // queries', F with the keys' of its columns and of its rows; then F's part of dk
   static constexpr int kSquare = kC * kC * 2;
@@ -466,16 +466,17 @@ struct Strided {
   }
 };
 
-// 16 columns of V of S, dS and dS' into one stage of the ring.
+// kSub times 16 columns of V (what there is of them) of S, dS and dS' into one stage of the ring.
 template <typename E, int KD>
 __device__ __forceinline__ void load_states(uint32_t stage, const Args &a, long long chunk, long long slot, int v0,
                                             uint32_t bar) {
   using L = Grad<E, KD>;
   const long long plane = 2LL * a.vp * KD, at = 2LL * v0 * KD;
-  bar_expect(bar, L::kStage);
-  bulk_load(stage, a.states + chunk * plane + at, 2 * L::kTile, bar);
-  bulk_load(stage + 2 * L::kTile, a.dstates + slot * plane + at, 2 * L::kTile, bar);
-  bulk_load(stage + 4 * L::kTile, a.dstates + (slot + 1) * plane + at, 2 * L::kTile, bar);
+  const uint32_t bytes = 2 * L::kTile * min(L::kSub, (a.vp - v0) / 16);
+  bar_expect(bar, 3 * bytes);
+  bulk_load(stage, a.states + chunk * plane + at, bytes, bar);
+  bulk_load(stage + 2 * L::kSub * L::kTile, a.dstates + slot * plane + at, bytes, bar);
+  bulk_load(stage + 4 * L::kSub * L::kTile, a.dstates + (slot + 1) * plane + at, bytes, bar);
 }
 
 // A fragment with its contraction's columns times powers of two: f0 for 2c, 2c + 1, f1 for
@@ -609,21 +610,19 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
   const long long chunk = bh * a.n_chunks + n, kv_chunk = ((long long)b * a.hk + hk) * a.n_chunks + n;
   const long long slot = bh * (a.n_chunks + 1) + n;
   const int steps = a.vp / 16;
-  __shared__ __align__(8) uint64_t bars[L::kStages + 1];
-  const uint32_t bar = smem_u32(bars), first_bar = bar + L::kStages * 8;
+  __shared__ __align__(8) uint64_t bars[3];
+  const uint32_t bar = smem_u32(bars), first_bar = bar + 16;
   Waiter wait{a.error, false};
   if (tid == kThreads - 32) {
 #pragma unroll
-    for (int i = 0; i <= L::kStages; ++i) bar_init(bar + i * 8);
+    for (int i = 0; i < 3; ++i) bar_init(bar + i * 8);
     bars_ready();
     bar_expect(first_bar, 2 * L::kKq + (kVec + 1) * kC * 4);
     bulk_load(base + L::kCoef, a.vec + chunk * kVec * kC, kVec * kC * 4, first_bar);
     bulk_load(base + L::kCoef + kVec * kC * 4, a.qfac + kv_chunk * kC, kC * 4, first_bar);
     bulk_load(base + L::kK, a.khat + kv_chunk * NP * kC * KD, L::kKq, first_bar);
     bulk_load(base + L::kQ, a.qhat + kv_chunk * NP * kC * KD, L::kKq, first_bar);
-#pragma unroll
-    for (int i = 0; i < L::kStages - 1; ++i)
-      if (i < steps) load_states<E, KD>(base + L::kRing + i * L::kStage, a, chunk, slot, i * 16, bar + i * 8);
+    load_states<E, KD>(base + L::kRing, a, chunk, slot, 0, bar);
   }
   const float *w_rows = a.ws + chunk * a.vp * kC, *dr_rows = a.drs + chunk * a.vp * kC;
   const E *do_rows = static_cast<const E *>(a.dout) + gb * a.vdim;
@@ -671,9 +670,9 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
   zero(xb);
   zero(d);
   float both = 0.f;  // <S, dS>, this thread's part
-  for (int step = 0; step < steps; ++step) {
-    const int v0 = step * 16, local = v0 % VB;
-    if (local == 0 && v0 > 0) {  // the next block of V
+  for (int step = 0; step < steps; step += L::kSub) {
+    const int v0 = step * 16, turn = step / L::kSub;
+    if (v0 % VB == 0 && v0 > 0) {  // the next block of V
       const int rows = min(VB, a.vp - v0);
       __syncthreads();  // all are done with the block before
       TokenTile<VB, kThreads> w_tile, dr_tile;
@@ -688,59 +687,62 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
       for (int i = 0; i < 3; ++i)
         if (tid < rows) rho[i * VB + tid] = row_scales[i][v0 + tid] * inverse_pow2(big[i]);
     }
-    wait(bar + step % L::kStages * 8, step / L::kStages & 1);
+    wait(bar + turn % 2 * 8, turn / 2 & 1);
     __syncthreads();  // all are done with the stage before
-    if (tid == 0) {
-      const int next = step + L::kStages - 1;
-      if (next < steps)
-        load_states<E, KD>(base + L::kRing + next % L::kStages * L::kStage, a, chunk, slot, next * 16,
-                           bar + next % L::kStages * 8);
-    }
-    const int stage = L::kRing + step % L::kStages * L::kStage;
-    const uint32_t st = base + stage;
-    constexpr uint32_t kWide = VB * kC * 2;
-    if (tid < 16 * KD / 8) {  // a piece of eight of <S, dS>
-      const int r = tid / (KD / 8);
-      const unsigned char *p = smem + stage + 2 * tile_at<KD>(r, tid % (KD / 8));
-      uint4 w[4];
+    if (tid == kThreads - 32 && step + L::kSub < steps)
+      load_states<E, KD>(base + L::kRing + (turn + 1) % 2 * L::kStage, a, chunk, slot, v0 + L::kSub * 16,
+                         bar + (turn + 1) % 2 * 8);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint4 *>(p + j * L::kTile);
-      float sum = 0.f;
+    for (int sub = 0; sub < L::kSub; ++sub) {
+      if (step + sub >= steps) continue;
+      const int local = v0 % VB + sub * 16;
+      const int stage = L::kRing + turn % 2 * L::kStage + 2 * sub * L::kTile;
+      const uint32_t st = base + stage;
+      constexpr int kSet = 2 * L::kSub * L::kTile;  // from S's tiles to dS's, and on to those of dS'
+      constexpr uint32_t kWide = VB * kC * 2;
+      if (tid < 16 * KD / 8) {  // a piece of eight of <S, dS>
+        const int r = tid / (KD / 8);
+        const unsigned char *p = smem + stage + 2 * tile_at<KD>(r, tid % (KD / 8));
+        uint4 w[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 x = half2_float2((&w[0].x)[j]), y = half2_float2((&w[1].x)[j]);
-        const float2 z = half2_float2((&w[2].x)[j]), q = half2_float2((&w[3].x)[j]);
-        sum = fmaf(x.x + y.x, z.x + q.x, fmaf(x.y + y.y, z.y + q.y, sum));
+        for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint4 *>(p + (j >> 1) * kSet + (j & 1) * L::kTile);
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 x = half2_float2((&w[0].x)[j]), y = half2_float2((&w[1].x)[j]);
+          const float2 z = half2_float2((&w[2].x)[j]), q = half2_float2((&w[3].x)[j]);
+          sum = fmaf(x.x + y.x, z.x + q.x, fmaf(x.y + y.y, z.y + q.y, sum));
+        }
+        both = fmaf(sum, rho[local + r] * rho[VB + local + r], both);
       }
-      both = fmaf(sum, rho[local + r] * rho[VB + local + r], both);
-    }
-    const float2 s0 = *reinterpret_cast<const float2 *>(rho + local + 2 * c);
-    const float2 s1 = *reinterpret_cast<const float2 *>(rho + local + 2 * c + 8);
-    if (is_do) {
-      const float2 d0 = *reinterpret_cast<const float2 *>(rho + 2 * VB + local + 2 * c);
-      const float2 d1 = *reinterpret_cast<const float2 *>(rho + 2 * VB + local + 2 * c + 8);
-      uint32_t fo[NP][4], fx[NP][4], fw[2][4];
+      const float2 s0 = *reinterpret_cast<const float2 *>(rho + local + 2 * c);
+      const float2 s1 = *reinterpret_cast<const float2 *>(rho + local + 2 * c + 8);
+      if (is_do) {
+        const float2 d0 = *reinterpret_cast<const float2 *>(rho + 2 * VB + local + 2 * c);
+        const float2 d1 = *reinterpret_cast<const float2 *>(rho + 2 * VB + local + 2 * c + 8);
+        uint32_t fo[NP][4], fx[NP][4], fw[2][4];
 #pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        ldsm4(a_rows<VB>(base + L::kDO + p * kC * VB * 2, row, local, lane), fo[p]);
-        scale_frag(fo[p], s0, s1, fx[p]);
+        for (int p = 0; p < NP; ++p) {
+          ldsm4(a_rows<VB>(base + L::kDO + p * kC * VB * 2, row, local, lane), fo[p]);
+          scale_frag(fo[p], s0, s1, fx[p]);
+        }
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          ldsm4t(a_cols<kC>(base + L::kW + p * kWide, local, row, lane), fw[p]);
+          scale_frag(fw[p], d0, d1, fw[p]);
+        }
+        cols_step<KD, NP, 2>(xa, fx, st, L::kTile, 0, xcol, NX, lane);
+        cols_step<KD, 2, 2>(xb, fw, st + 2 * kSet, L::kTile, 0, xcol, NX, lane);
+        cols_step<kC, NP, 2>(d, fo, base + L::kW, kWide, local, dcol, dto, lane);
+      } else {
+        uint32_t fr[2][4], fx[2][4];
+#pragma unroll
+        for (int p = 0; p < 2; ++p) ldsm4t(a_cols<kC>(base + L::kDR + p * kWide, local, row, lane), fr[p]);
+#pragma unroll
+        for (int p = 0; p < 2; ++p) scale_frag(fr[p], s0, s1, fx[p]);
+        cols_step<KD, 2, 2>(xa, fx, st, L::kTile, 0, xcol, NX, lane);
+        cols_step<kC, 2, 2>(d, fr, base + L::kW, kWide, local, dcol, dto, lane);
       }
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        ldsm4t(a_cols<kC>(base + L::kW + p * kWide, local, row, lane), fw[p]);
-        scale_frag(fw[p], d0, d1, fw[p]);
-      }
-      cols_step<KD, NP, 2>(xa, fx, st, L::kTile, 0, xcol, NX, lane);
-      cols_step<KD, 2, 2>(xb, fw, st + 4 * L::kTile, L::kTile, 0, xcol, NX, lane);
-      cols_step<kC, NP, 2>(d, fo, base + L::kW, kWide, local, dcol, dto, lane);
-    } else {
-      uint32_t fr[2][4], fx[2][4];
-#pragma unroll
-      for (int p = 0; p < 2; ++p) ldsm4t(a_cols<kC>(base + L::kDR + p * kWide, local, row, lane), fr[p]);
-#pragma unroll
-      for (int p = 0; p < 2; ++p) scale_frag(fr[p], s0, s1, fx[p]);
-      cols_step<KD, 2, 2>(xa, fx, st, L::kTile, 0, xcol, NX, lane);
-      cols_step<kC, 2, 2>(d, fr, base + L::kW, kWide, local, dcol, dto, lane);
     }
   }
 #pragma unroll
