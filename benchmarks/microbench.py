@@ -34,6 +34,11 @@ Ops:
              made from x inside the row scan; rqf_fbt_rank1_forward / _backward)
   mosc       the fused multi-oscillator scan (B,T,F) -> (B,T,F), --groups
              oscillators per filter
+  delta      the gated delta rule over sequences with its gradients, bf16, --F
+             wide as heads of 128 x 128 (gated_delta_scan)
+  delta_step its single-token form on --B states of each head (gated_delta_step)
+  clip       the gradients' norm and clipping, --F x --B x --T elements in
+             bf16 as 64 tensors (clip_grads_)
 
 --btf-path forces one (B,T,F) kernel family (1 streaming, 2 tile-resident).
 
@@ -217,16 +222,43 @@ def make_case(op: str, F: int, B: int, T: int, groups: int = 8, truncated: bool 
     return run
 
 
+def make_delta(op, F, B, T):
+    import prospective_rqf_b200 as rqf
+
+    g = torch.Generator(device="cuda").manual_seed(0)
+    rand = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    if op == "clip":
+        n = F * B * T // 64
+        grads = [rand(n).bfloat16() for _ in range(64)]
+        out = [torch.empty_like(x) for x in grads]
+        return lambda: rqf.clip_grads_(grads, 1.0, out=out)
+    heads, lead = F // 128, (B, T) if op == "delta" else (B,)
+    unit = lambda x: torch.nn.functional.normalize(x, dim=-1).bfloat16()  # noqa: E731
+    args = [unit(rand(*lead, heads, 128)), unit(rand(*lead, heads, 128)),
+            rand(*lead, heads, 128).bfloat16(),
+            -torch.nn.functional.softplus(rand(*lead, heads) - 4.0), torch.sigmoid(rand(*lead, heads))]
+    if op == "delta_step":
+        state = rand(B, heads, 128, 128)
+        return lambda: rqf.gated_delta_step(*args, state)
+    args = [t.requires_grad_() for t in args]
+    go = rand(*args[2].shape).bfloat16()
+
+    def run():
+        torch.autograd.grad(rqf.gated_delta_scan(*args), args, go)
+    return run
+
+
 OPS = ("fbt", "fbt_raw", "fbt_skip", "tbptt_fbt", "tbptt_btf", "btf", "btf_real", "btf_pro",
        "selective", "selective_bf16", "projection", "projection_torch", "projection_real", "mosc",
-       "block_scan", "block_scan_bwd", "rank1")
+       "block_scan", "block_scan_bwd", "rank1", "delta", "delta_step", "clip")
 
 
 def measure(op, F, B, T, iters=10, warmup=3, groups=8, truncated=False) -> dict:
     import prospective_rqf_b200 as rqf
     from prospective_rqf_b200 import _timing
 
-    run = make_case(op, F, B, T, groups, truncated)
+    run = (make_delta(op, F, B, T) if op in ("delta", "delta_step", "clip")
+           else make_case(op, F, B, T, groups, truncated))
     for _ in range(warmup):
         run()
     torch.cuda.synchronize()

@@ -25,16 +25,16 @@ from .ops import _SYNC_CHECK, _nbytes
 __all__ = ["gated_delta_scan", "gated_delta_step"]
 
 
-def _call(name, tensors, fn, *args):
-    """fn(*args), under the active KernelTimer if there is one and with the package's check of
-    device errors after it if that is on."""
+def _call(name, v, moved, fn, *args):
+    """fn(*args), under the active KernelTimer if there is one (`moved` are the tensors that the
+    launch must read or write) and with the package's check of device errors if that is on."""
     if _timing._ACTIVE is None:
         out = fn(*args)
     else:
-        with _timing.launch(name, tensors[0].numel(), _nbytes(*tensors)):
+        with _timing.launch(name, v.numel() // v.shape[-1], _nbytes(*moved)):
             out = fn(*args)
     if _SYNC_CHECK:
-        _abi.check_device_errors(tensors[0].device)
+        _abi.check_device_errors(v.device)
     return out
 
 
@@ -55,8 +55,8 @@ class _GatedDeltaScan(torch.autograd.Function):
         *inputs, context = ctx.saved_tensors
         need = ctx.needs_input_grad
         dq, dk, dv, dg, db, ds0 = _call(
-            "rqf_gated_delta_backward", inputs[:3], _abi.native().delta_backward, *inputs, context,
-            ctx.scale, grad_o, grad_last, need[5])
+            "rqf_gated_delta_backward", inputs[2], inputs[:5] * 2 + [inputs[2]],
+            _abi.native().delta_backward, *inputs, context, ctx.scale, grad_o, grad_last, need[5])
         dg, db = dg.to(ctx.types[0]), db.to(ctx.types[1])
         return tuple(x if n else None for x, n in zip((dq, dk, dv, dg, db, ds0, None, None), need))
 
@@ -80,10 +80,11 @@ def gated_delta_scan(q, k, v, log_decay, beta, *, scale: float | None = None, in
     Products are taken to 32-bit accuracy whatever the type (csrc/delta_common.cuh).  While a
     gradient is wanted, the states that enter each 64 tokens are kept for the backward."""
     args = (q, k, v, log_decay, beta, initial_state)
+    moved = (q, k, v, log_decay, beta, v)  # and o, as large as v
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
-        o, last = _call("rqf_gated_delta_forward", args[:3], _GatedDeltaScan.apply, *args, lengths, scale)
+        o, last = _call("rqf_gated_delta_forward", v, moved, _GatedDeltaScan.apply, *args, lengths, scale)
     else:
-        o, last, _ = _call("rqf_gated_delta_forward", args[:3], _abi.native().delta_forward, *args,
+        o, last, _ = _call("rqf_gated_delta_forward", v, moved, _abi.native().delta_forward, *args,
                            lengths, scale, False)
     return (o, last) if return_state else o
 
@@ -97,5 +98,6 @@ def gated_delta_step(q, k, v, log_decay, beta, state, *, slots=None, scale: floa
     are distinct integers; a negative one is an idle row, whose output is 0.  One past the pool
     is taken as idle too and raises from check_device_errors().  Returns o (batch, value_heads,
     V) in v's type.  No gradient is recorded."""
-    return _call("rqf_gated_delta_step", (q, k, v), _abi.native().delta_step, q, k, v, log_decay, beta,
-                 state, slots, scale)
+    rows = state[:v.shape[0]] if _timing._ACTIVE is not None else None  # as many states as rows
+    return _call("rqf_gated_delta_step", v, (q, k, v, v, rows, rows), _abi.native().delta_step, q, k, v,
+                 log_decay, beta, state, slots, scale)

@@ -9,18 +9,28 @@ from __future__ import annotations
 
 import torch
 
-from . import _abi
-from .ops import _done
+from . import _abi, _timing
+from .ops import _SYNC_CHECK, _nbytes
 
 __all__ = ["global_grad_norm", "clip_grads_"]
+
+
+def _call(name, grads, times, fn, *args):
+    if _timing._ACTIVE is None:
+        norm = fn(*args)
+    else:
+        ts = [grads] if isinstance(grads, torch.Tensor) else grads
+        with _timing.launch(name, sum(t.numel() for t in ts), times * _nbytes(*ts)):
+            norm = fn(*args)
+    if _SYNC_CHECK and norm.is_cuda:
+        _abi.check_device_errors(norm.device)
+    return norm
 
 
 def global_grad_norm(grads) -> torch.Tensor:
     """sqrt(sum |g|^2) over all tensors of `grads` (float32, bfloat16, float16, complex64, mixed as
     they come), as a float32 scalar on their device.  The same tensors give the same bits."""
-    norm = _abi.native().grad_norm(grads)
-    _done(norm.device)
-    return norm
+    return _call("rqf_global_grad_norm", grads, 1, _abi.native().grad_norm, grads)
 
 
 def clip_grads_(grads, max_norm: float, *, out=None) -> torch.Tensor:
@@ -29,6 +39,4 @@ def clip_grads_(grads, max_norm: float, *, out=None) -> torch.Tensor:
 
     In place, or into `out`: tensors of the same shapes and types (parts of an optimiser's flat
     buffer, say), which share no memory with `grads`.  A NaN norm makes all NaN."""
-    norm = _abi.native().clip_grads(grads, max_norm, out)
-    _done(norm.device)
-    return norm
+    return _call("rqf_clip_grads", grads, 3, _abi.native().clip_grads, grads, max_norm, out)
