@@ -22,6 +22,10 @@
 // do_t^T besides a_{t+1} dD_{t+1}, so that <S_t, dS_t> = dg_{t+1} + o_t.do_t,
 // where o_t.do_t = q_t.dq_t.  No product of chunk by chunk is needed for it, and
 // the sum runs over one chunk at most.
+//
+// 16000 tokens of 64 heads of 128 x 128: the first 1.36 ms, bound by its chain as the forward's
+// pass is, the second 2.73 ms (4.9 GB, 1.8 TB/s): a chunk fills an SM, and its loads, products and
+// sums follow one another with barriers between.
 #pragma once
 
 #include "delta_scan.cuh"

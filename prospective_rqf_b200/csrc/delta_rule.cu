@@ -30,12 +30,15 @@ struct Sizes {
 };
 
 // Spans of the sequence.  A span costs its chunks twice (once for its ends, with K more columns,
-// once proper), so cutting pays where rows x columns of 16 leave most of the 592 schedulers idle:
-// three spans at least, each of four chunks at least.
+// once proper) and two launches, so cutting pays where rows x columns of 16 leave most of the 592
+// schedulers idle and the sequence is long: 16384 tokens of 8 heads of 128 x 128 take 0.39 ms in
+// nine spans and 1.15 ms in one, 4096 tokens of 32 heads 0.30 ms in two and 0.34 in one, 777 float32
+// tokens of 9 heads with gradients 120 us of kernels in three and 151 in one, but 512 tokens of 8
+// heads of 64 x 64 45 us in two and 41 in one.
 void cut(int64_t warps, Sizes *s) {
   int64_t n = warps > 0 ? 592 / warps : 1;
   if (n > s->chunks / 4) n = s->chunks / 4;
-  if (n < 3) n = 1;
+  if (n < 2 || (n == 2 && s->chunks < 16)) n = 1;
   s->seg_chunks = (int)ceil_div(s->chunks, n);
   s->segs = s->chunks > 0 ? (int)ceil_div(s->chunks, s->seg_chunks) : 1;
 }
@@ -168,21 +171,13 @@ int launch(int64_t grid, int threads, size_t smem, const Args &a, cudaStream_t s
   return cudaGetLastError() == cudaSuccess ? RQF_OK : RQF_ERR_LAUNCH;
 }
 
-// A pass from chunk to chunk over `columns` of V (and of the identity): CTAs of four warps on the
-// states (64 columns) while those are at most one to an SM, of eight where there are more and they
-// fit.  With eight the chunk's tiles are loaded once for 128 columns and a scheduler has two warps.
-// With output four already are eight warps.
-bool eight_warps(int64_t rows, int64_t columns) { return columns > 64 && rows * ceil_div(columns, 64) > 148; }
-
+// The passes from chunk to chunk have four warps on the states to a CTA: 64 columns of V (or, for
+// the ends, of the identity).
 template <typename E, int KD, int PASS>
 int run_scan(const Args &a, cudaStream_t st) {
   constexpr bool out = PASS != kEnds;
-  const int64_t rows = (int64_t)a.batch * a.hv * (out ? a.segs : a.segs - 1), columns = out ? a.vp : a.vp + a.kp;
-  using Eight = Layout<E, KD, 8, PASS>;
-  if constexpr (!out && Eight::kStages == 2)
-    if (eight_warps(rows, columns))
-      return launch<scan_kernel<E, KD, 8, PASS>>(rows * ceil_div(columns, 128), Eight::kThreads, Eight::kBytes, a, st);
   using Four = Layout<E, KD, 4, PASS>;
+  const int64_t rows = (int64_t)a.batch * a.hv * (out ? a.segs : a.segs - 1), columns = out ? a.vp : a.vp + a.kp;
   return launch<scan_kernel<E, KD, 4, PASS>>(rows * ceil_div(columns, 64), Four::kThreads, Four::kBytes, a, st);
 }
 template <typename E, int KD, bool OUT>

