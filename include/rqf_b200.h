@@ -714,6 +714,8 @@ int rqf_two_tap_coefficients_backward(const float *log_theta, const float *log_g
  * bytes and their strides are multiples of 16 bytes.  Products take their
  * operands in halves (two for a 32-bit one) with 32-bit sums: 32-bit accuracy.
  * Non-finite inputs reach all of their 64-token chunk and what follows.
+ * The first call of each entry on a device looks up addresses and attributes
+ * there: make it outside any stream capture.
  *
  * context: rqf_gated_delta_context_bytes(problem, save), 256-byte aligned.
  * With save != 0 the forward keeps in it what the backward needs (the states

@@ -928,33 +928,45 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
     }
     store_grad_rows<E>(a, a.dk, dk_part, gb, row, here, xcol, lane, xb);
   } else if (warp == 4 * H) {
-    // dg: <S, dS> less what the tokens before each gate have had
-    float x[2];
+    // dg_t = dg_{t-1} - x_{t-1} from dg_0 = <S, dS> on, x = q.dq - v.dv.  A gate at the least decay
+    // is closed: its dg is 0, and the sum starts again there, so that nothing of what lies before
+    // it (another document, say) is left in what comes after, not even as rounding.
+    float x[2], v[2], all = 0.f;
+    bool closed[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int t = 2 * lane + i;
       x[i] = qdq[t] + (H == 2 ? qdq[kC + t] : 0.f) - vdv[t];
+      const float gate = t == 0 ? g_hi[0] : (g_hi[t] - g_hi[t - 1]) + (g_lo[t] - g_lo[t - 1]);
+      closed[i] = gate <= 0.999f * kMinDecay;
     }
-    float upto = x[0] + x[1];
-#pragma unroll
-    for (int s = 1; s < 32; s <<= 1) {
-      const float up = __shfl_up_sync(0xffffffffu, upto, s);
-      if (lane >= s) upto += up;
-    }
-    upto = __shfl_up_sync(0xffffffffu, upto, 1);
-    if (lane == 0) upto = 0.f;
-    float all = 0.f;
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) all += both_sums[w];
     all *= big[0] * big[1];
+    const float x_before = __shfl_up_sync(0xffffffffu, x[1], 1);
+    v[0] = closed[0] || lane == 0 ? 0.f : -x_before;
+    v[1] = closed[1] ? 0.f : -x[0];
+    float run = closed[1] ? 0.f : v[0] + v[1];
+    int cut = closed[0] || closed[1];
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const float up = __shfl_up_sync(0xffffffffu, run, s);
+      const int up_cut = __shfl_up_sync(0xffffffffu, cut, s);
+      if (lane >= s) {
+        if (!cut) run += up;
+        cut |= up_cut;
+      }
+    }
+    float before = __shfl_up_sync(0xffffffffu, run, 1);
+    int cut_before = __shfl_up_sync(0xffffffffu, cut, 1);
+    if (lane == 0) before = 0.f, cut_before = 0;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int t = 2 * lane + i;
-      // a gate at the least decay is closed: nothing passes, and its gradient is 0
-      const float gate = t == 0 ? g_hi[0] : (g_hi[t] - g_hi[t - 1]) + (g_lo[t] - g_lo[t - 1]);
+      before = closed[i] ? 0.f : before + v[i];
+      cut_before |= closed[i];
       if (t < here)
-        a.dg[gb + (long long)t * a.hv] =
-            t < live && gate > 0.999f * kMinDecay ? all - (upto + (i ? x[0] : 0.f)) : 0.f;
+        a.dg[gb + (long long)t * a.hv] = t >= live || closed[i] ? 0.f : cut_before ? before : all + before;
     }
   }
 }

@@ -231,6 +231,21 @@ def test_gates_that_clear_or_keep():
     assert not grads[3][:, 5].any() and not grads[3][:, 100].any()
 
 
+def test_a_closed_gate_parts_large_values_from_small_ones():
+    """Two documents in one row, the first with values ten thousand times the second's: the second's
+    gradients are as exact as if it stood alone."""
+    args = inputs(1, 150, 1, 2, 32, 32, F32)
+    args[2][:, :40] *= 1e4
+    args[3][:, 40] = -math.inf
+    go = torch.randn(1, 150, 2, 32, generator=torch.Generator().manual_seed(3)).cuda()
+    leaves = [t.clone().requires_grad_() for t in args]
+    grads = torch.autograd.grad(rqf.gated_delta_scan(*leaves), leaves, go)
+    alone = [t[:, 40:].double().requires_grad_() for t in args]
+    want = torch.autograd.grad(reference(*alone)[0], alone, go[:, 40:].double())
+    for n, a, b in zip(NAMES, grads, want):
+        assert_near(a[:, 40:], b, f"gradient of {n}")
+
+
 def test_keys_that_are_alike():
     """Equal keys with beta = 1 and no decay: the inverse inside a chunk has entries that cancel."""
     args = inputs(1, 128, 1, 1, 32, 32, F32)
