@@ -720,7 +720,7 @@ int rqf_two_tap_coefficients_backward(const float *log_theta, const float *log_g
  * context: rqf_gated_delta_context_bytes(problem, save), 256-byte aligned.
  * With save != 0 the forward keeps in it what the backward needs (the states
  * that enter each chunk among it); the backward is then given the same
- * problem, v and context.  Each size is SIZE_MAX for a refused shape. */
+ * problem (whose strides it does not read) and context.  Each size is SIZE_MAX for a refused shape. */
 enum { RQF_F32 = 0, RQF_BF16 = 1, RQF_F16 = 2, RQF_C64 = 3 };
 
 typedef struct {
@@ -740,7 +740,7 @@ int rqf_gated_delta_forward(const rqf_delta_problem *problem, const void *q, con
                             int save, rqf_stream_t stream);
 /* grad_final_state nullable (zeros); grad_initial_state nullable (not
  * written); the other gradients are written in full. */
-int rqf_gated_delta_backward(const rqf_delta_problem *problem, const void *v, const void *context,
+int rqf_gated_delta_backward(const rqf_delta_problem *problem, const void *context,
                              const void *grad_o, const float *grad_final_state, void *grad_q,
                              void *grad_k, void *grad_v, float *grad_log_decay, float *grad_beta,
                              float *grad_initial_state, void *workspace, rqf_stream_t stream);

@@ -171,7 +171,7 @@ SIGNATURES: dict[str, tuple] = {
     "rqf_gated_delta_forward": (
         _int, [_pdp, _p, _p, _p, _p, _p, _p, _p, _p, _p, _int, _p]),
     "rqf_gated_delta_backward": (
-        _int, [_pdp, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p]),
+        _int, [_pdp, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p]),
     "rqf_gated_delta_step": (
         _int, [_pdp, _p, _p, _p, _p, _p, _p, _int, _i64, _p, _p, _p]),
     "rqf_grad_norm_scratch_bytes": (_sz, [_i64]),

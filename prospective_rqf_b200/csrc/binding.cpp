@@ -258,7 +258,7 @@ PyObject *delta_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (want) ds0 = at::empty({v.size(0), v.size(2), q.size(3), v.size(3)}, g.options());
     const rqf_delta_problem p = describe(q, k, v, g, b, lengths, scale);
     Tensor work = scratch_of(rqf_gated_delta_backward_workspace_bytes(&p), v);
-    check(rqf_gated_delta_backward(&p, data(v), data(context), data(go), floats(gl), data(dq), data(dk), data(dv),
+    check(rqf_gated_delta_backward(&p, data(context), data(go), floats(gl), data(dq), data(dk), data(dv),
                                    dg.data_ptr<float>(), db.data_ptr<float>(),
                                    want ? ds0.data_ptr<float>() : nullptr, data(work), stream_on(v)),
           "rqf_gated_delta_backward");

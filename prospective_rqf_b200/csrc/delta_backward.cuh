@@ -6,22 +6,22 @@
 //   du = P^T do + e^{G_C-G} k dS',   dr = du + T'^T diag(beta) du,   dv = beta dr
 //   dS = e^{G_C} dS' + (scale e^G q)^T do - (beta e^G k)^T dr
 //
-// and keeps dS', dr and v.dv.  The second takes all chunks at once, with S, w
-// from the forward and dS', dr from the first (u = beta w):
+// and keeps dS' and dr.  The second takes all chunks at once, with S, w from the forward and dS',
+// dr from the first (u = beta w):
 //
 //   dP = do u^T,  dA = -dr u^T,  X1 = do S^T,  X2 = u dS'^T,  X3 = dr S^T,
 //   E = scale D dP,  F = beta D dA  (D_ij = e^{G_i-G_j}, lower triangles)
 //   dq = scale e^G X1 + E k
 //   dk = e^{G_C-G} X2 - beta e^G X3 + F k + E^T q + F^T k
 //   dbeta = dr.w
-//   dg_t = <S, dS> - sum_{i<t} (q_i.dq_i - v_i.dv_i)
+//   dg_t = sum_{i>=t} (in_i - back_i) + sum_{j<t} out_j + e^{G_C} <S, dS'>
 //
-// dS the cotangent of the state that enters the chunk.  The last line: with D_t
-// = a_t S_{t-1}, dg_t = <D_t, dD_t>; dD_t = dS_t - k_t dr_t^T and S_t = D_t +
-// k_t u_t^T give <D_t, dD_t> = <S_t, dS_t> - v_t.dv_t, and dS_t has scale q_t
-// do_t^T besides a_{t+1} dD_{t+1}, so that <S_t, dS_t> = dg_{t+1} + o_t.do_t,
-// where o_t.do_t = q_t.dq_t.  No product of chunk by chunk is needed for it, and
-// the sum runs over one chunk at most.
+// dg_t is the sum of all that passes the gate between t - 1 and t.  With E' = E without its
+// diagonal, which passes no gate: in = q.(scale e^G X1 + E' k) + k.(F k - beta e^G X3), all that a
+// token takes; back = k.(E'^T q + F^T k), what of it is given in the chunk; out = k.(e^{G_C-G} X2),
+// what a token leaves for later chunks.  No product of tokens by tokens is needed for it, and
+// where gates are strong its terms are as small as it is: with E's diagonal in them (or with
+// q.dq - v.dv, which is the same sum) dg lost a digit for every e^-2.3 of decay.
 //
 // 16000 tokens of 64 heads of 128 x 128: the first 1.36 ms, bound by its chain as the forward's
 // pass is, the second 2.73 ms (4.9 GB, 1.8 TB/s): a chunk fills an SM, and its loads, products and
@@ -34,7 +34,7 @@ namespace rqf {
 namespace delta {
 
 // Shared memory of that pass with W warps on the state's cotangents and W beside them: tiles (of
-// two chunks where that fits), a tile of do or v to a pair, and what a pair hands over: dS' as
+// two chunks where that fits), a tile of do to a pair, and what a pair hands over: dS' as
 // fragments, P^T do and then dr (whose place dv takes), q^T of the scaled do, the rows' largest
 // magnitudes.
 template <typename E, int KD, int W>
@@ -51,7 +51,7 @@ struct BackLayout {
 
 // As in the forward's pass, a pair of warps: one on the chain from dS' to dS (k dS', T'^T du,
 // k^T dr), the other on what does not wait for it (P^T do, q^T do) or that nothing waits for (dr,
-// dv, v.dv, and dS' as the next pass reads it).
+// dv, and dS' as the next pass reads it).
 template <typename E, int KD, int W, bool OUT>
 __global__ void __launch_bounds__(BackLayout<E, KD, W>::kThreads, 1) scan_backward_kernel(const Args a) {
   constexpr int NP = Elem<E>::kParts;
@@ -76,7 +76,6 @@ __global__ void __launch_bounds__(BackLayout<E, KD, W>::kThreads, 1) scan_backwa
   const int chunks = max(0, min(row_chunks, n0 + a.seg_chunks) - n0);
   const long long len = row_len - (long long)n0 * kC, left = a.time - (long long)n0 * kC;
   const long long kv_first = ((long long)b * a.hk + hk) * a.n_chunks + n0, first = bh * a.n_chunks + n0;
-  const long long slot = bh * (a.n_chunks + 1) + n0;
   const uint32_t base = smem_u32(smem);
   unsigned char *mine = smem + L::kDO + pair * L::kTile, *give = smem + L::kGive + pair * L::kHand;
   uint4 *frags = reinterpret_cast<uint4 *>(give) + lane;                          // [ks][hi, lo][lane]
@@ -85,7 +84,6 @@ __global__ void __launch_bounds__(BackLayout<E, KD, W>::kThreads, 1) scan_backwa
   float4 *z_tiles = reinterpret_cast<float4 *>(pdo_bytes + L::kPdo) + lane;       // [nt][lane]
   float *row_maxes = reinterpret_cast<float *>(pdo_bytes + L::kPdo + L::kZ);      // [row]
   const uint32_t tile = smem_u32(mine);
-  const E *v = static_cast<const E *>(a.v) + b * a.sv.b + (long long)n0 * kC * a.sv.t + h * a.sv.h + v0;
   const long long so = (long long)a.hv * a.vdim;  // do and dv are dense
   const long long at = (((long long)b * a.time + (long long)n0 * kC) * a.hv + h) * a.vdim + v0;
   const E *dout = static_cast<const E *>(a.dout) + at;
@@ -231,8 +229,7 @@ __global__ void __launch_bounds__(BackLayout<E, KD, W>::kThreads, 1) scan_backwa
       __syncwarp();
       Tile::get(tile, mine, lane, x);
       __syncwarp();
-      if (OUT) Tile::load(tile, v + t0 * a.sv.t, a.sv.t, (int)min((long long)kC, len - t0), cols, lane);
-      else if (n > 0) Tile::load(tile, dout + (t0 - kC) * so, so, kC, cols, lane);
+      if (n > 0) Tile::load(tile, dout + (t0 - kC) * so, so, kC, cols, lane);
       copy_commit();
       Scale x0, x1;
       {
@@ -282,8 +279,8 @@ __global__ void __launch_bounds__(BackLayout<E, KD, W>::kThreads, 1) scan_backwa
       pair_arrive(1 + W + pair);
       if (OUT) {
         pair_wait(1 + 2 * W + pair);  // dS' and dr
-        save_scales(a.dscales + (slot + n + 1) * a.vp + v0, row_maxes[lane >> 2], row_maxes[(lane >> 2) + 8], lane);
-        __half *keep = a.dstates + ((slot + n + 1) * a.vp + v0) * 2 * KD;
+        save_scales(a.dscales + (first + n) * a.vp + v0, row_maxes[lane >> 2], row_maxes[(lane >> 2) + 8], lane);
+        __half *keep = a.dstates + ((first + n) * a.vp + v0) * 2 * KD;
 #pragma unroll
         for (int ks = 0; ks < KD / 16; ++ks) {
           const uint4 f = frags[ks * 64], g = frags[ks * 64 + 32];
@@ -302,13 +299,6 @@ __global__ void __launch_bounds__(BackLayout<E, KD, W>::kThreads, 1) scan_backwa
         }
         save_rows(a.drs + ((first + n) * a.vp + v0) * kC, lane, x);
         save_token_max(a.token_maxes, first + n, kTokenDR, a.vp / 16, w, x, lane);
-        copy_wait<0>();  // v
-        __syncwarp();
-        Tile::get(tile, mine, lane, y);
-        __syncwarp();
-        if (n > 0) Tile::load(tile, dout + (t0 - kC) * so, so, kC, cols, lane);
-        copy_commit();
-        float m[8][2];
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt) {
           const float2 be = *reinterpret_cast<const float2 *>(vec + kRowBeta * kC + nt * 8 + 2 * c);
@@ -316,10 +306,8 @@ __global__ void __launch_bounds__(BackLayout<E, KD, W>::kThreads, 1) scan_backwa
           x[nt][1] *= be.y;
           x[nt][2] *= be.x;
           x[nt][3] *= be.y;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) m[nt][e] = fmaf(y[nt][e], x[nt][e], y[nt][e + 2] * x[nt][e + 2]);
         }
-        save_tokens<true>(a.vdv + ((first + n) * (a.vp / 16) + w) * kC, m, lane);
+        __syncwarp();
         Tile::put(pdo_bytes, lane, x);
         __syncwarp();
         Tile::store(pdo_bytes, dv + t0 * so, so, (int)min((long long)kC, left - t0), cols, lane);
@@ -340,18 +328,6 @@ __global__ void __launch_bounds__(BackLayout<E, KD, W>::kThreads, 1) scan_backwa
         *reinterpret_cast<uint4 *>(dv + t * so + (lane % kPieces) * kPer) = make_uint4(0, 0, 0, 0);
     return;
   }
-  if (seg == 0 && chunks > 0) {  // the cotangent of the state that enters the first chunk
-    float m0, m1;
-    row_max(S, m0, m1);
-    const Scale s0 = scale_for(m0), s1 = scale_for(m1);
-    save_scales(a.dscales + slot * a.vp + v0, m0, m1, lane);
-#pragma unroll
-    for (int ks = 0; ks < KD / 16; ++ks) {
-      uint32_t hi[4], lo[4];
-      split_frag(S, ks, s0.mul, s1.mul, hi, lo);
-      save_frag<KD>(a.dstates + (slot * a.vp + v0) * 2 * KD, ks, lane, hi, lo);
-    }
-  }
   if (a.ds0 != nullptr && seg == 0)
     store_state<KD>(a.ds0 + bh * a.kdim * a.vdim, a.vdim, v0, a.kdim, a.vdim, lane, S);
 }
@@ -370,10 +346,10 @@ struct Grad {
   static constexpr int kK = 0, kQ = kKq;
   static constexpr int kW = 2 * kKq, kDR = kW + 2 * kVB * kC * 2;  // [v][t] hi, lo
   static constexpr int kDO = kDR + 2 * kVB * kC * 2;               // [t][v] parts
-  // a ring of kSub times 16 columns of V: S, dS and dS', hi and lo
+  // a ring of kSub times 16 columns of V: S and dS', hi and lo
   static constexpr int kRing = kDO + NP * kC * kVB * 2;
   static constexpr int kTile = 16 * KD * 2, kSub = NP == 2 && KD == 128 ? 1 : 2;
-  static constexpr int kStage = 6 * kTile * kSub, kStages = 2;
+  static constexpr int kStage = 4 * kTile * kSub, kStages = 2;
   // after the products over V, from w's place on, hi and lo: E with the keys' factors, E with the
   // queries', F with the keys' of its columns and of its rows; then F's part of dk
   static constexpr int kSquare = kC * kC * 2;
@@ -382,9 +358,13 @@ struct Grad {
   static constexpr int kEnd = kRing + kStages * kStage, kNeed = kDK + kC * KD * 4;
   static constexpr int kCoef = kEnd > kNeed ? kEnd : kNeed;  // vec's rows, qfac
   static constexpr int kFloats = kCoef + (kVec + 1) * kC * 4;
-  // rows of 64: q.dq by half, v.dv, gates' sums hi and lo; then the rows' scales of S, dS, dS'
-  static constexpr int kBytes = kFloats + 5 * kC * 4 + 3 * kVB * 4;
+  // rows of 64 (enum Sum), then the rows' scales of S and dS'
+  static constexpr int kBytes = kFloats + 23 * kC * 4 + 2 * kVB * 4;
 };
+// Rows of sums: in (less back) of the warps of do and of the others, and out, by half of the columns;
+// the gates' sums; E's diagonal; the largest of E's and F's rows with the keys' factors, by half of
+// the columns, and of their columns with the rows' factors, by block of rows.
+enum Sum { kSumIn = 0, kSumBack = 4, kSumOut = 6, kSumGHi = 8, kSumGLo = 9, kSumDiag = 10, kSumRowMax = 11, kSumColMax = 15 };
 
 // A 32-bit tile [v][token] by way of registers: loaded, and later stored as halves hi, lo, each
 // token's column under its own scale.
@@ -450,7 +430,7 @@ struct DoutTile {
   }
 };
 
-// Values `stride` apart, N of them in flight, and their reduction with what lies past them.
+// Values `stride` apart, N of them in flight, and the largest of them and of what lies past them.
 template <int N>
 struct Strided {
   float x[N];
@@ -460,27 +440,24 @@ struct Strided {
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = i < count ? p[i * stride] : 0.f;
   }
-  template <bool SUM>
   __device__ __forceinline__ float reduce() const {
     float all = x[0];
 #pragma unroll
-    for (int i = 1; i < N; ++i) all = SUM ? all + x[i] : fmaxf(all, x[i]);
-    for (int i = N; i < count; ++i) all = SUM ? all + p[i * stride] : fmaxf(all, p[i * stride]);
+    for (int i = 1; i < N; ++i) all = fmaxf(all, x[i]);
+    for (int i = N; i < count; ++i) all = fmaxf(all, p[i * stride]);
     return all;
   }
 };
 
-// kSub times 16 columns of V (what there is of them) of S, dS and dS' into one stage of the ring.
+// kSub times 16 columns of V (what there is of them) of S and dS' into one stage of the ring.
 template <typename E, int KD>
-__device__ __forceinline__ void load_states(uint32_t stage, const Args &a, long long chunk, long long slot, int v0,
-                                            uint32_t bar) {
+__device__ __forceinline__ void load_states(uint32_t stage, const Args &a, long long chunk, int v0, uint32_t bar) {
   using L = Grad<E, KD>;
-  const long long plane = 2LL * a.vp * KD, at = 2LL * v0 * KD;
+  const long long at = chunk * 2 * a.vp * KD + 2LL * v0 * KD;
   const uint32_t bytes = 2 * L::kTile * min(L::kSub, (a.vp - v0) / 16);
-  bar_expect(bar, 3 * bytes);
-  bulk_load(stage, a.states + chunk * plane + at, bytes, bar);
-  bulk_load(stage + 2 * L::kSub * L::kTile, a.dstates + slot * plane + at, bytes, bar);
-  bulk_load(stage + 4 * L::kSub * L::kTile, a.dstates + (slot + 1) * plane + at, bytes, bar);
+  bar_expect(bar, 2 * bytes);
+  bulk_load(stage, a.states + at, bytes, bar);
+  bulk_load(stage + 2 * L::kSub * L::kTile, a.dstates + at, bytes, bar);
 }
 
 // A fragment with its contraction's columns times powers of two: f0 for 2c, 2c + 1, f1 for
@@ -547,6 +524,29 @@ __device__ __forceinline__ void dot_rows(const float (&x)[NT][4], const unsigned
   d1 = quad_sum(d1);
 }
 
+// x += c0, c1 times the two rows of a half tile in NP parts.
+template <int KD, int NP, int NT>
+__device__ __forceinline__ void add_rows(float (&x)[NT][4], const unsigned char *tile, int row, int col0, int lane,
+                                         float c0, float c1) {
+  const int g = lane >> 2, c = lane & 3;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const unsigned char *t = tile + p * kC * KD * 2;
+      const int piece = col0 / 8 + nt;
+      const float2 k0 = half2_float2(
+          *reinterpret_cast<const uint32_t *>(t + 2 * (tile_at<KD>(row + g, piece) + 2 * c)));
+      const float2 k1 = half2_float2(
+          *reinterpret_cast<const uint32_t *>(t + 2 * (tile_at<KD>(row + g + 8, piece) + 2 * c)));
+      x[nt][0] = fmaf(c0, k0.x, x[nt][0]);
+      x[nt][1] = fmaf(c0, k0.y, x[nt][1]);
+      x[nt][2] = fmaf(c1, k1.x, x[nt][2]);
+      x[nt][3] = fmaf(c1, k1.y, x[nt][3]);
+    }
+  }
+}
+
 // Rows of a gradient to global memory: E where each key head has one value
 // head, else 32-bit parts that are summed after.
 template <typename E, int NT>
@@ -580,9 +580,10 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
   const uint32_t base = smem_u32(smem);
   const float *vec = reinterpret_cast<const float *>(smem + L::kCoef), *qfac = vec + kVec * kC;
   const float *kfac = vec + kRowK * kC, *beta = vec + kRowBeta * kC;
-  float *qdq = reinterpret_cast<float *>(smem + L::kFloats), *vdv = qdq + 2 * kC;
-  float *g_hi = vdv + kC, *g_lo = g_hi + kC, *rho = g_lo + kC;  // rho: [S, dS, dS'][v]
-  __shared__ float w_inv[kTokenMaxes * kC], per_warp[2][kThreads / 32], both_sums[kThreads / 32];
+  float *sums = reinterpret_cast<float *>(smem + L::kFloats);
+  float *g_hi = sums + kSumGHi * kC, *g_lo = sums + kSumGLo * kC, *diag = sums + kSumDiag * kC;
+  float *rho = sums + 23 * kC;  // [S, dS'][v]
+  __shared__ float w_inv[kTokenMaxes * kC], both_sums[kThreads / 32];
   float *dr_inv = w_inv + kTokenDR * kC, *do_inv = w_inv + kTokenDO * kC;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const bool is_do = warp < 4 * H;
@@ -612,7 +613,6 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
     return;
   }
   const long long chunk = bh * a.n_chunks + n, kv_chunk = ((long long)b * a.hk + hk) * a.n_chunks + n;
-  const long long slot = bh * (a.n_chunks + 1) + n;
   const int steps = a.vp / 16;
   __shared__ __align__(8) uint64_t bars[3];
   const uint32_t bar = smem_u32(bars), first_bar = bar + 16;
@@ -626,7 +626,7 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
     bulk_load(base + L::kCoef + kVec * kC * 4, a.qfac + kv_chunk * kC, kC * 4, first_bar);
     bulk_load(base + L::kK, a.khat + kv_chunk * NP * kC * KD, L::kKq, first_bar);
     bulk_load(base + L::kQ, a.qhat + kv_chunk * NP * kC * KD, L::kKq, first_bar);
-    load_states<E, KD>(base + L::kRing, a, chunk, slot, 0, bar);
+    load_states<E, KD>(base + L::kRing, a, chunk, 0, bar);
   }
   const float *w_rows = a.ws + chunk * a.vp * kC, *dr_rows = a.drs + chunk * a.vp * kC;
   const E *do_rows = static_cast<const E *>(a.dout) + gb * a.vdim;
@@ -637,27 +637,20 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
   w_first.load(w_rows, min(VB, a.vp), tid);
   dr_first.load(dr_rows, min(VB, a.vp), tid);
   do_first.load(do_rows, so, live, a.vdim, tid);
-  // the largest row scales of S, dS and dS', to which all rows' are taken
-  const float *row_scales[3] = {a.scales + chunk * a.vp, a.dscales + slot * a.vp, a.dscales + (slot + 1) * a.vp};
+  // the largest row scales of S and dS', to which all rows' are taken
+  const float *row_scales[2] = {a.scales + chunk * a.vp, a.dscales + chunk * a.vp};
   // all loads before the first reduction: each is a wait for memory
-  const int t = tid % kC, what = min(tid / kC, kTokenMaxes);  // w, dr, do, v.dv of a token
+  const int t = tid % kC, what = min(tid / kC, kTokenMaxes - 1);  // w, dr, do of a token
   const Strided<4> rows0(row_scales[0] + lane, (a.vp - lane + 31) / 32, 32);
   const Strided<4> rows1(row_scales[1] + lane, (a.vp - lane + 31) / 32, 32);
-  const Strided<4> rows2(row_scales[2] + lane, (a.vp - lane + 31) / 32, 32);
-  const Strided<8> token(what < kTokenMaxes ? a.token_maxes + (chunk * kTokenMaxes + what) * steps * kC + t
-                                            : a.vdv + chunk * steps * kC + t,
-                         tid < (kTokenMaxes + 1) * kC ? steps : 0, kC);
+  const Strided<8> token(a.token_maxes + (chunk * kTokenMaxes + what) * steps * kC + t,
+                         tid < kTokenMaxes * kC ? steps : 0, kC);
   const float2 gates = a.gsum[chunk * kC + t];
-  float big[3] = {rows0.template reduce<false>(), rows1.template reduce<false>(), rows2.template reduce<false>()};
-  if (what < kTokenMaxes) {
-    w_inv[tid] = scale_for(token.template reduce<false>()).inv;
-  } else if (tid < (kTokenMaxes + 1) * kC) {
-    g_hi[t] = gates.x;
-    g_lo[t] = gates.y;
-    vdv[t] = token.template reduce<true>();
-  }
+  float big[2] = {rows0.reduce(), rows1.reduce()};
+  if (tid < kTokenMaxes * kC) w_inv[tid] = scale_for(token.reduce()).inv;
+  if (tid < kC) g_hi[t] = gates.x, g_lo[t] = gates.y;
 #pragma unroll
-  for (int i = 0; i < 3; ++i)
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) big[i] = fmaxf(big[i], __shfl_xor_sync(0xffffffffu, big[i], d));
   __syncthreads();
@@ -666,14 +659,14 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
   dr_first.store(smem + L::kDR, smem + L::kDR + VB * kC * 2, dr_inv, tid);
   do_first.store(smem + L::kDO, do_inv, tid);
 #pragma unroll
-  for (int i = 0; i < 3; ++i)
+  for (int i = 0; i < 2; ++i)
     if (tid < min(VB, a.vp)) rho[i * VB + tid] = row_scales[i][tid] * inverse_pow2(big[i]);
 
   float xa[NX][4], xb[NX][4], d[ND][4];  // X1 or X3; X2; dP or dA
   zero(xa);
   zero(xb);
   zero(d);
-  float both = 0.f;  // <S, dS>, this thread's part
+  float both = 0.f;  // <S, dS'>, this thread's part
   for (int step = 0; step < steps; step += L::kSub) {
     const int v0 = step * 16, turn = step / L::kSub;
     if (v0 % VB == 0 && v0 > 0) {  // the next block of V
@@ -688,13 +681,13 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
       dr_tile.store(smem + L::kDR, smem + L::kDR + VB * kC * 2, dr_inv, tid);
       do_tile.store(smem + L::kDO, do_inv, tid);
 #pragma unroll
-      for (int i = 0; i < 3; ++i)
+      for (int i = 0; i < 2; ++i)
         if (tid < rows) rho[i * VB + tid] = row_scales[i][v0 + tid] * inverse_pow2(big[i]);
     }
     wait(bar + turn % 2 * 8, turn / 2 & 1);
     __syncthreads();  // all are done with the stage before
     if (tid == kThreads - 32 && step + L::kSub < steps)
-      load_states<E, KD>(base + L::kRing + (turn + 1) % 2 * L::kStage, a, chunk, slot, v0 + L::kSub * 16,
+      load_states<E, KD>(base + L::kRing + (turn + 1) % 2 * L::kStage, a, chunk, v0 + L::kSub * 16,
                          bar + (turn + 1) % 2 * 8);
 #pragma unroll
     for (int sub = 0; sub < L::kSub; ++sub) {
@@ -702,9 +695,9 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
       const int local = v0 % VB + sub * 16;
       const int stage = L::kRing + turn % 2 * L::kStage + 2 * sub * L::kTile;
       const uint32_t st = base + stage;
-      constexpr int kSet = 2 * L::kSub * L::kTile;  // from S's tiles to dS's, and on to those of dS'
+      constexpr int kSet = 2 * L::kSub * L::kTile;  // from S's tiles to those of dS'
       constexpr uint32_t kWide = VB * kC * 2;
-      if (tid < 16 * KD / 8) {  // a piece of eight of <S, dS>
+      if (tid < 16 * KD / 8) {  // a piece of eight of <S, dS'>
         const int r = tid / (KD / 8);
         const unsigned char *p = smem + stage + 2 * tile_at<KD>(r, tid % (KD / 8));
         uint4 w[4];
@@ -722,8 +715,8 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
       const float2 s0 = *reinterpret_cast<const float2 *>(rho + local + 2 * c);
       const float2 s1 = *reinterpret_cast<const float2 *>(rho + local + 2 * c + 8);
       if (is_do) {
-        const float2 d0 = *reinterpret_cast<const float2 *>(rho + 2 * VB + local + 2 * c);
-        const float2 d1 = *reinterpret_cast<const float2 *>(rho + 2 * VB + local + 2 * c + 8);
+        const float2 d0 = *reinterpret_cast<const float2 *>(rho + VB + local + 2 * c);
+        const float2 d1 = *reinterpret_cast<const float2 *>(rho + VB + local + 2 * c + 8);
         uint32_t fo[NP][4], fx[NP][4], fw[2][4];
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
@@ -736,7 +729,7 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
           scale_frag(fw[p], d0, d1, fw[p]);
         }
         cols_step<KD, NP, 2>(xa, fx, st, L::kTile, 0, xcol, NX, lane);
-        cols_step<KD, 2, 2>(xb, fw, st + 2 * kSet, L::kTile, 0, xcol, NX, lane);
+        cols_step<KD, 2, 2>(xb, fw, st + kSet, L::kTile, 0, xcol, NX, lane);
         cols_step<kC, NP, 2>(d, fo, base + L::kW, kWide, local, dcol, dto, lane);
       } else {
         uint32_t fr[2][4], fx[2][4];
@@ -759,12 +752,13 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
   const float x_inv0 = left_inv[row + g], x_inv1 = left_inv[row + g + 8];
   const float l0 = lfac[row + g], l1 = lfac[row + g + 8];
   const float b0 = beta[row + g], b1 = beta[row + g + 8];
-  float max_k = 0.f, max_l = 0.f;
+  float row_m[2] = {0.f, 0.f}, col_m[ND][2];
   {
     const float lead0 = is_do ? a.scale * x_inv0 : -x_inv0 * b0, lead1 = is_do ? a.scale * x_inv1 : -x_inv1 * b1;
     const float gh0 = g_hi[row + g], gl0 = g_lo[row + g], gh1 = g_hi[row + g + 8], gl1 = g_lo[row + g + 8];
 #pragma unroll
     for (int nt = 0; nt < ND; ++nt) {
+      col_m[nt][0] = col_m[nt][1] = 0.f;
       if (nt / 2 > dto) continue;
       const int j = dcol + nt * 8 + 2 * c;
       const float2 wi = *reinterpret_cast<const float2 *>(w_inv + j);
@@ -780,19 +774,31 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
           a.dbeta[gb + (long long)i * a.hv] = i < live ? x * (e >> 1 ? x_inv1 : x_inv0) : 0.f;
         const float diff = ((e >> 1 ? gh1 : gh0) - (e & 1 ? gh.y : gh.x)) + ((e >> 1 ? gl1 : gl0) - (e & 1 ? gl.y : gl.x));
         const bool in = is_do ? i >= jj : i > jj;
-        const float ef = in ? ((e >> 1 ? lead1 : lead0) * x) * ((e & 1 ? be.y : be.x) * __expf(diff)) : 0.f;
+        float ef = in ? ((e >> 1 ? lead1 : lead0) * x) * ((e & 1 ? be.y : be.x) * __expf(diff)) : 0.f;
+        if (is_do && i == jj) {  // E's diagonal apart
+          diag[i] = ef;
+          ef = 0.f;
+        }
         d[nt][e] = ef;
-        max_k = fmaxf(max_k, fabsf(ef * (e & 1 ? kf.y : kf.x)));
-        max_l = fmaxf(max_l, fabsf(ef * (e >> 1 ? l1 : l0)));
+        row_m[e >> 1] = fmaxf(row_m[e >> 1], fabsf(ef * (e & 1 ? kf.y : kf.x)));
+        col_m[nt][e & 1] = fmaxf(col_m[nt][e & 1], fabsf(ef * (e >> 1 ? l1 : l0)));
       }
     }
   }
+  {
+    float *to = sums + (kSumRowMax + (is_do ? 0 : H) + half) * kC;
+    row_m[0] = quad_max(row_m[0]), row_m[1] = quad_max(row_m[1]);
+    if (c == 0) to[row + g] = row_m[0], to[row + g + 8] = row_m[1];
+    to = sums + (kSumColMax + (is_do ? 0 : 4) + rb) * kC + dcol + 2 * c;
 #pragma unroll
-  for (int s = 16; s > 0; s >>= 1) {
-    max_k = fmaxf(max_k, __shfl_xor_sync(0xffffffffu, max_k, s));
-    max_l = fmaxf(max_l, __shfl_xor_sync(0xffffffffu, max_l, s));
+    for (int nt = 0; nt < ND; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) col_m[nt][e] = fmaxf(col_m[nt][e], __shfl_xor_sync(0xffffffffu, col_m[nt][e], x));
+      if (g == 0) *reinterpret_cast<float2 *>(to + nt * 8) = make_float2(col_m[nt][0], col_m[nt][1]);
+    }
   }
-  if (lane == 0) per_warp[0][warp] = max_k, per_warp[1][warp] = max_l;
   // X's true values
   {
     const float e0 = vec[kRowEG * kC + row + g], e1 = vec[kRowEG * kC + row + g + 8];
@@ -809,44 +815,46 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
       const float u1 = (w_inv[row + g + 8] * b1) * vec[kRowEC * kC + row + g + 8];
 #pragma unroll
       for (int nt = 0; nt < NX; ++nt) {
-        xb[nt][0] = u0 * (big[2] * xb[nt][0]);
-        xb[nt][1] = u0 * (big[2] * xb[nt][1]);
-        xb[nt][2] = u1 * (big[2] * xb[nt][2]);
-        xb[nt][3] = u1 * (big[2] * xb[nt][3]);
+        xb[nt][0] = u0 * (big[1] * xb[nt][0]);
+        xb[nt][1] = u0 * (big[1] * xb[nt][1]);
+        xb[nt][2] = u1 * (big[1] * xb[nt][2]);
+        xb[nt][3] = u1 * (big[1] * xb[nt][3]);
       }
     }
   }
   __syncthreads();  // w, dr, do and the ring are read; the maxima are there
-  Scale sk, sl, sle;  // of E or F with column factors, with row factors, and of E with row factors
+  // a row's scale along it, a column's down it: tokens of any size keep their bits beside others
+  const auto row_scale = [&](int i) {
+    const float *m = sums + (kSumRowMax + (is_do ? 0 : H)) * kC + i;
+    return scale_for(H == 2 ? fmaxf(m[0], m[kC]) : m[0]);
+  };
+  const auto col_scale = [&](int j) {
+    const float *m = sums + (kSumColMax + (is_do ? 0 : 4)) * kC + j;
+    return scale_for(fmaxf(fmaxf(m[0], m[kC]), fmaxf(m[2 * kC], m[3 * kC])));
+  };
+  const Scale sk0 = row_scale(row + g), sk1 = row_scale(row + g + 8);
+  const Scale sl0 = col_scale(row + g), sl1 = col_scale(row + g + 8);
   {
-    float m[3] = {0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < 4 * H; ++w) {
-      m[0] = fmaxf(m[0], per_warp[0][(is_do ? 0 : 4 * H) + w]);
-      m[1] = fmaxf(m[1], per_warp[1][(is_do ? 0 : 4 * H) + w]);
-      m[2] = fmaxf(m[2], per_warp[1][w]);
-    }
-    sk = scale_for(m[0]), sl = scale_for(m[1]), sle = scale_for(m[2]);
     unsigned char *cols = smem + (is_do ? L::kE : L::kF), *rows = smem + (is_do ? L::kEq : L::kFk);
-    const float r0 = l0 * sl.mul, r1 = l1 * sl.mul;
 #pragma unroll
     for (int nt = 0; nt < ND; ++nt) {
       if (nt / 2 > dto) continue;  // never read: products stop at the diagonal
       const float2 kf = *reinterpret_cast<const float2 *>(kfac + dcol + nt * 8 + 2 * c);
-      const float kx = kf.x * sk.mul, ky = kf.y * sk.mul;
+      const Scale cx = col_scale(dcol + nt * 8 + 2 * c), cy = col_scale(dcol + nt * 8 + 2 * c + 1);
+      const float k0 = sk0.mul, k1 = sk1.mul;
       const int at0 = 2 * (tile_at<kC>(row + g, dcol / 8 + nt) + 2 * c);
       const int at1 = 2 * (tile_at<kC>(row + g + 8, dcol / 8 + nt) + 2 * c);
       uint32_t hi, lo;
-      split2(d[nt][0] * kx, d[nt][1] * ky, hi, lo);
+      split2(d[nt][0] * kf.x * k0, d[nt][1] * kf.y * k0, hi, lo);
       *reinterpret_cast<uint32_t *>(cols + at0) = hi;
       *reinterpret_cast<uint32_t *>(cols + L::kSquare + at0) = lo;
-      split2(d[nt][2] * kx, d[nt][3] * ky, hi, lo);
+      split2(d[nt][2] * kf.x * k1, d[nt][3] * kf.y * k1, hi, lo);
       *reinterpret_cast<uint32_t *>(cols + at1) = hi;
       *reinterpret_cast<uint32_t *>(cols + L::kSquare + at1) = lo;
-      split2(d[nt][0] * r0, d[nt][1] * r0, hi, lo);
+      split2(d[nt][0] * l0 * cx.mul, d[nt][1] * l0 * cy.mul, hi, lo);
       *reinterpret_cast<uint32_t *>(rows + at0) = hi;
       *reinterpret_cast<uint32_t *>(rows + L::kSquare + at0) = lo;
-      split2(d[nt][2] * r1, d[nt][3] * r1, hi, lo);
+      split2(d[nt][2] * l1 * cx.mul, d[nt][3] * l1 * cy.mul, hi, lo);
       *reinterpret_cast<uint32_t *>(rows + at1) = hi;
       *reinterpret_cast<uint32_t *>(rows + L::kSquare + at1) = lo;
     }
@@ -868,11 +876,16 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
 #pragma unroll
     for (int nt = 0; nt < NX; ++nt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) xa[nt][e] = fmaf(y[nt][e], sk.inv, xa[nt][e]);
+      for (int e = 0; e < 4; ++e) xa[nt][e] = fmaf(y[nt][e], e < 2 ? sk0.inv : sk1.inv, xa[nt][e]);
+    const float k0 = kfac[row + g], k1 = kfac[row + g + 8], e0 = diag[row + g], e1 = diag[row + g + 8];
     float d0, d1;
     dot_rows<KD, NP>(xa, smem + L::kQ, row, xcol, lane, d0, d1);
-    if (c == 0) qdq[half * kC + row + g] = l0 * d0, qdq[half * kC + row + g + 8] = l1 * d1;
+    float *in = sums + (kSumIn + half) * kC, *back = sums + (kSumBack + half) * kC, *out = sums + (kSumOut + half) * kC;
+    if (c == 0) in[row + g] = l0 * d0, in[row + g + 8] = l1 * d1;
+    add_rows<KD, NP>(xa, smem + L::kK, row, xcol, lane, e0 * k0, e1 * k1);
     store_grad_rows<E>(a, a.dq, dq_part, gb, row, here, xcol, lane, xa);
+    dot_rows<KD, NP>(xb, smem + L::kK, row, xcol, lane, d0, d1);
+    if (c == 0) out[row + g] = k0 * d0, out[row + g + 8] = k1 * d1;
     zero(y);
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {  // E^T q
@@ -885,7 +898,10 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
 #pragma unroll
     for (int nt = 0; nt < NX; ++nt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) xb[nt][e] = fmaf(y[nt][e], sle.inv, xb[nt][e]);
+      for (int e = 0; e < 4; ++e) xb[nt][e] = fmaf(y[nt][e], e < 2 ? sl0.inv : sl1.inv, xb[nt][e]);
+    dot_rows<KD, NP>(y, smem + L::kK, row, xcol, lane, d0, d1);
+    if (c == 0) back[row + g] = k0 * (sl0.inv * d0), back[row + g + 8] = k1 * (sl1.inv * d1);
+    add_rows<KD, NP>(xb, smem + L::kQ, row, xcol, lane, e0 * l0, e1 * l1);
   } else {
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {  // F k
@@ -898,7 +914,9 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
 #pragma unroll
     for (int nt = 0; nt < NX; ++nt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) xa[nt][e] = fmaf(y[nt][e], sk.inv, xa[nt][e]);
+      for (int e = 0; e < 4; ++e) xa[nt][e] = fmaf(y[nt][e], e < 2 ? sk0.inv : sk1.inv, xa[nt][e]);
+    float d0, d1, f0, f1;
+    dot_rows<KD, NP>(xa, smem + L::kK, row, xcol, lane, d0, d1);
     zero(y);
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {  // F^T k
@@ -908,10 +926,13 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
       for (int p = 0; p < 2; ++p) ldsm4t(a_cols<kC>(base + L::kFk + p * L::kSquare, ks * 16, row, lane), f[p]);
       cols_step<KD, 2, NP>(y, f, base + L::kK, kC * KD * 2, ks * 16, xcol, NX, lane);
     }
+    dot_rows<KD, NP>(y, smem + L::kK, row, xcol, lane, f0, f1);
+    float *in = sums + (kSumIn + 2 + half) * kC;
+    if (c == 0) in[row + g] = l0 * (d0 - sl0.inv * f0), in[row + g + 8] = l1 * (d1 - sl1.inv * f1);
 #pragma unroll
     for (int nt = 0; nt < NX; ++nt) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) xa[nt][e] = fmaf(y[nt][e], sl.inv, xa[nt][e]);
+      for (int e = 0; e < 4; ++e) xa[nt][e] = fmaf(y[nt][e], e < 2 ? sl0.inv : sl1.inv, xa[nt][e]);
       exchange[(2 * nt) * 32] = make_float2(xa[nt][0], xa[nt][1]);
       exchange[(2 * nt + 1) * 32] = make_float2(xa[nt][2], xa[nt][3]);
     }
@@ -928,45 +949,50 @@ __global__ void __launch_bounds__(Grad<E, KD>::kThreads, KD >= 64 ? 1 : 2) gradi
     }
     store_grad_rows<E>(a, a.dk, dk_part, gb, row, here, xcol, lane, xb);
   } else if (warp == 4 * H) {
-    // dg_t = dg_{t-1} - x_{t-1} from dg_0 = <S, dS> on, x = q.dq - v.dv.  A gate at the least decay
-    // is closed: its dg is 0, and the sum starts again there, so that nothing of what lies before
-    // it (another document, say) is left in what comes after, not even as rounding.
-    float x[2], v[2], all = 0.f;
+    // dg.  A gate at the least decay is closed: its dg is 0, and what comes after it gives nothing
+    // to the tokens before it; the sum over later tokens ends there, so that not even rounding of
+    // what lies on its other side (another document, say) is left.
+    float v[2], out[2], through = 0.f;
     bool closed[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int t = 2 * lane + i;
-      x[i] = qdq[t] + (H == 2 ? qdq[kC + t] : 0.f) - vdv[t];
+      v[i] = out[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < H; ++j) {
+        v[i] += sums[(kSumIn + j) * kC + t] + sums[(kSumIn + 2 + j) * kC + t] - sums[(kSumBack + j) * kC + t];
+        out[i] += sums[(kSumOut + j) * kC + t];
+      }
       const float gate = t == 0 ? g_hi[0] : (g_hi[t] - g_hi[t - 1]) + (g_lo[t] - g_lo[t - 1]);
       closed[i] = gate <= 0.999f * kMinDecay;
     }
 #pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) all += both_sums[w];
-    all *= big[0] * big[1];
-    const float x_before = __shfl_up_sync(0xffffffffu, x[1], 1);
-    v[0] = closed[0] || lane == 0 ? 0.f : -x_before;
-    v[1] = closed[1] ? 0.f : -x[0];
-    float run = closed[1] ? 0.f : v[0] + v[1];
-    int cut = closed[0] || closed[1];
+    for (int w = 0; w < kThreads / 32; ++w) through += both_sums[w];
+    through = vec[kRowEG * kC + kC - 1] * (big[0] * big[1] * through);
+    // this lane's two tokens and the later ones, `joined` to the next lane's while no gate between
+    // is closed; and all before it for out
+    int next_closed = __shfl_down_sync(0xffffffffu, (int)closed[0], 1);
+    if (lane == 31) next_closed = 1;
+    float later = v[0] + (closed[1] ? 0.f : v[1]), upto = out[0] + out[1];
+    int joined = !closed[1] && !next_closed;
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
-      const float up = __shfl_up_sync(0xffffffffu, run, s);
-      const int up_cut = __shfl_up_sync(0xffffffffu, cut, s);
-      if (lane >= s) {
-        if (!cut) run += up;
-        cut |= up_cut;
+      const float down = __shfl_down_sync(0xffffffffu, later, s), up = __shfl_up_sync(0xffffffffu, upto, s);
+      const int down_joined = __shfl_down_sync(0xffffffffu, joined, s);
+      if (lane + s < 32) {
+        if (joined) later += down;
+        joined &= down_joined;
       }
+      if (lane >= s) upto += up;
     }
-    float before = __shfl_up_sync(0xffffffffu, run, 1);
-    int cut_before = __shfl_up_sync(0xffffffffu, cut, 1);
-    if (lane == 0) before = 0.f, cut_before = 0;
+    const float next = __shfl_down_sync(0xffffffffu, later, 1);
+    float before = __shfl_up_sync(0xffffffffu, upto, 1);
+    if (lane == 0) before = 0.f;
+    const float dg[2] = {later + before + through, v[1] + (next_closed ? 0.f : next) + (before + out[0]) + through};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int t = 2 * lane + i;
-      before = closed[i] ? 0.f : before + v[i];
-      cut_before |= closed[i];
-      if (t < here)
-        a.dg[gb + (long long)t * a.hv] = t >= live || closed[i] ? 0.f : cut_before ? before : all + before;
+      if (t < here) a.dg[gb + (long long)t * a.hv] = t >= live || closed[i] ? 0.f : dg[i];
     }
   }
 }

@@ -306,8 +306,7 @@ struct Strides {
 
 // One call's tensors and sizes.  n_chunks covers `time`; a row's own length
 // ends it earlier.  w and dr are [row][chunk][v][64], v padded to VP, a multiple
-// of 16; dstates has one slot more for each row than it has chunks, slot n for
-// the cotangent of the state that enters chunk n.
+// of 16.
 struct Args {
   const void *q, *k, *v, *dout;
   const float *g, *beta;
@@ -329,7 +328,7 @@ struct Args {
   float *kfac, *qfac, *vec;
   float2 *gsum;  // running sums of g inside a chunk, hi and lo
   __half *states, *dstates;  // [chunk][16 of v][hi, lo][16][KD], rows scaled, in tile_at's order
-  float *scales, *dscales, *ws, *drs, *token_maxes, *vdv;
+  float *scales, *dscales, *ws, *drs, *token_maxes;
   float *dq_part, *dk_part;  // (B, T, Hv, K) when key heads are shared
   int *error;                // the device's error word
 };

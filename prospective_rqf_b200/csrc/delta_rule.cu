@@ -110,10 +110,8 @@ size_t carve_context(void *buffer, const rqf_delta_problem *p, const Sizes &s, b
 }
 size_t carve_workspace(void *buffer, const rqf_delta_problem *p, const Sizes &s, Args *a) {
   Carver c{static_cast<unsigned char *>(buffer)};
-  const size_t slots = (size_t)s.bhn + (size_t)p->batch * p->value_heads;
-  c.take(a->dstates, slots * 2 * s.vp * s.kd);
-  c.take(a->dscales, slots * s.vp);
-  c.take(a->vdv, (size_t)s.bhn * (s.vp / 16) * kC);
+  c.take(a->dstates, (size_t)s.bhn * 2 * s.vp * s.kd);
+  c.take(a->dscales, (size_t)s.bhn * s.vp);
   c.take(a->drs, (size_t)s.bhn * s.vp * kC);
   if (s.segs > 1) {
     const size_t spans = (size_t)p->batch * p->value_heads * s.segs * p->key_dim;
@@ -278,27 +276,24 @@ int rqf_gated_delta_forward(const rqf_delta_problem *problem, const void *q, con
   });
 }
 
-int rqf_gated_delta_backward(const rqf_delta_problem *problem, const void *v, const void *context,
-                             const void *grad_o, const float *grad_final_state, void *grad_q, void *grad_k,
-                             void *grad_v, float *grad_log_decay, float *grad_beta,
-                             float *grad_initial_state, void *workspace, rqf_stream_t stream) {
+int rqf_gated_delta_backward(const rqf_delta_problem *problem, const void *context, const void *grad_o,
+                             const float *grad_final_state, void *grad_q, void *grad_k, void *grad_v,
+                             float *grad_log_decay, float *grad_beta, float *grad_initial_state,
+                             void *workspace, rqf_stream_t stream) {
   Sizes s;
   int rc = sizes_of(problem, &s);
   if (rc != RQF_OK) return rc;
   if (problem->batch == 0) return RQF_OK;
-  if (s.chunks > 0 && (!v || !context || !grad_o || !grad_q || !grad_k || !grad_v || !grad_log_decay ||
+  if (s.chunks > 0 && (!context || !grad_o || !grad_q || !grad_k || !grad_v || !grad_log_decay ||
                        !grad_beta || !workspace))
     return RQF_ERR_ARGUMENT;
-  const void *ptrs[] = {v, context, grad_o, grad_q, grad_k, grad_v, workspace};
+  const void *ptrs[] = {context, grad_o, grad_q, grad_k, grad_v, workspace};
   for (const void *p : ptrs)
     if (!aligned16(p)) return RQF_ERR_ALIGN;
-  const int64_t per = problem->dtype == RQF_F32 ? 4 : 8;
-  for (int i = 0; i < 3; ++i)
-    if (s.chunks > 0 && problem->v_stride[i] % per) return RQF_ERR_ALIGN;
   if (s.chunks == 0 && grad_initial_state == nullptr) return RQF_OK;
   Args a;
   common_args(problem, s, &a);
-  a.v = v, a.dout = grad_o, a.dsT = grad_final_state;
+  a.dout = grad_o, a.dsT = grad_final_state;
   a.dq = grad_q, a.dk = grad_k, a.dv = grad_v, a.dg = grad_log_decay, a.dbeta = grad_beta;
   a.ds0 = grad_initial_state;
   carve_context(const_cast<void *>(context), problem, s, true, &a);

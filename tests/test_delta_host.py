@@ -88,7 +88,7 @@ def test_c_entries_decide_on_the_host():
     assert 0 < size < lib.rqf_gated_delta_context_bytes(ctypes.byref(p), 1) < 1 << 24
     none = [None] * 9
     assert lib.rqf_gated_delta_forward(ctypes.byref(p), *none, 0, None) == 5
-    assert lib.rqf_gated_delta_backward(ctypes.byref(p), *[None] * 12) == 5
+    assert lib.rqf_gated_delta_backward(ctypes.byref(p), *[None] * 11) == 5
     assert lib.rqf_gated_delta_step(ctypes.byref(p), *[None] * 6, 0, 4, None, None, None) == 5
     buf = (ctypes.c_char * 64)()
     base = ctypes.addressof(buf)
