@@ -23,8 +23,8 @@
 // where gates are strong its terms are as small as it is: with E's diagonal in them (or with
 // q.dq - v.dv, which is the same sum) dg lost a digit for every e^-2.3 of decay.
 //
-// 16000 tokens of 64 heads of 128 x 128: the first 1.36 ms, bound by its chain as the forward's
-// pass is, the second 2.73 ms (4.9 GB, 1.8 TB/s): a chunk fills an SM, and its loads, products and
+// 16000 tokens of 64 heads of 128 x 128: the first 1.26 ms, bound by its chain as the forward's
+// pass is, the second 2.65 ms (3.9 GB, 1.5 TB/s): a chunk fills an SM, and its loads, products and
 // sums follow one another with barriers between.
 #pragma once
 

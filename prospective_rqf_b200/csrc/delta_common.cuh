@@ -244,9 +244,6 @@ __device__ __forceinline__ uint32_t a_cols(uint32_t base, int k0, int m0, int la
 }
 
 // ------------------------------------------------------------ asynchronous copies
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 // `bytes` of 16 from src, zeros for the rest.
 __device__ __forceinline__ void copy16z(uint32_t dst, const void *src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)

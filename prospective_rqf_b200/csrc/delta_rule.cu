@@ -31,7 +31,7 @@ struct Sizes {
 
 // Spans of the sequence.  A span costs its chunks twice (once for its ends, with K more columns,
 // once proper) and two launches, so cutting pays where rows x columns of 16 leave most of the 592
-// schedulers idle and the sequence is long: 16384 tokens of 8 heads of 128 x 128 take 0.39 ms in
+// schedulers idle and the sequence is long: 16384 tokens of 8 heads of 128 x 128 take 0.41 ms in
 // nine spans and 1.15 ms in one, 4096 tokens of 32 heads 0.30 ms in two and 0.34 in one, 777 float32
 // tokens of 9 heads with gradients 120 us of kernels in three and 151 in one, but 512 tokens of 8
 // heads of 64 x 64 45 us in two and 41 in one.
